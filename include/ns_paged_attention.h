@@ -126,6 +126,22 @@ int ns_paged_attention_call_workspace(const ns_paged_attn_args* args, uint64_t* 
  * Returns 0 on success, nonzero on invalid arguments. */
 int ns_paged_attention(const ns_paged_attn_args* args, hipStream_t stream);
 
+/* The same with a sliding window and sinks: a query at KV position p sees the positions t <= p (and
+ * t < seq_len) with t > p - window or t < sinks.  window >= 1, sinks >= 0.  What differs otherwise:
+ *   - block-table entries of blocks whose positions every query token of a workgroup has behind its
+ *     window are not read, so a released block's entry may hold anything (-1);
+ *   - query rows that are none of their sequence's query_lens tokens (rows behind the last sequence
+ *     of a padded batch) are left as they were;
+ *   - an infinite or NaN value in a position that a token does not see leaves that token's output
+ *     alone, in prefill tiles too.
+ * The work of a token is bounded by sinks + window whatever the sequence's length, and so are the
+ * workspace and the grid. */
+int ns_paged_attention_windowed(const ns_paged_attn_args* args, int32_t window, int32_t sinks, hipStream_t stream);
+
+/* Workspace bytes and counter words of such a call, as ns_paged_attention_call_workspace. */
+int ns_paged_attention_windowed_workspace(const ns_paged_attn_args* args, int32_t window, int32_t sinks,
+                                          uint64_t* bytes, uint64_t* counters);
+
 #ifdef __cplusplus
 }
 #endif

@@ -47,6 +47,12 @@ constexpr int kMaxMerge = 1024;
 constexpr int kTargetGroups = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Windows and sinks are clamped to this on the host, so that sums of the two and a position's alignment fit 32 bits.
+constexpr int kMaxWindow = 1 << 30;
+// The windowed kernels' positions: what lies between the sinks and the window is left out in whole multiples of this,
+// so that the rows of a wave's load instruction (at most 8) still lie in one block of a power-of-two size.
+constexpr int kAlign = 16;
+
 thread_local char g_err[512];
 
 int fail(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
@@ -78,6 +84,8 @@ struct PaParams {
   const int32_t* tokens;  // the query tokens the decode kernel takes (blockIdx.x indexes it), or NULL: all
   int32_t bs_shift;  // log2(block_size) when it is a power of two, else -1
   float scale_log2;  // scale * log2(e): scores in log2 units, exp2 for the softmax
+  // the windowed kernels' (WIN): a query at position p sees t <= p with t > p - window or t < sinks
+  int32_t window, sinks;   // 1 .. kMaxWindow, 0 .. kMaxWindow
 };
 
 // ---- element loads / stores -------------------------------------------------------------------
@@ -174,9 +182,33 @@ __device__ __forceinline__ float ld_dev(const float* p) {
 
 // ---- batch layout -----------------------------------------------------------------------------
 
+// With a window, a query at position q sees [0, sinks) and (q - window, q].  Its kernels walk virtual positions
+// v that leave out the hidden stretch between the two: v below sa is position v, from sa on it is v + gap.
+// sa and gap are multiples of kAlign, so up to kAlign - 1 hidden positions on either side of the gap stay in:
+// v in [sinks, h1) is hidden.  A gap of 0 comes with sa = 0.
+struct Hole {
+  int sa, gap, h1;
+  __device__ __forceinline__ int position(int v) const { return v + (v >= sa ? gap : 0); }
+};
+__device__ __forceinline__ Hole hole_of(const PaParams& p, int kv_pos) {   // kv_pos >= -1
+  const int first = kv_pos - p.window + 1;   // the window's first position
+  const int sa = (p.sinks + kAlign - 1) & -kAlign;
+  const int gap = (first & -kAlign) - sa;
+  return gap > 0 ? Hole{sa, gap, first - gap} : Hole{0, 0, first};
+}
+// Whether block-table column bi holds only positions hidden from a query at kv_pos (and so from those after it): its
+// entry is not read, a released page's -1 is no bad block.
+__device__ __forceinline__ bool hidden_block(const PaParams& p, int bi, int kv_pos) {
+  const int64_t b0 = (int64_t)bi * p.block_size;
+  return b0 >= p.sinks && b0 + p.block_size <= (int64_t)kv_pos - p.window + 1;
+}
+
 struct QueryPlace {
   int seq;
-  int kv_len;  // visible KV positions: min(kv_pos + 1, seq_len), at least 0
+  int kv_len;  // visible KV positions: min(kv_pos + 1, seq_len), at least 0; with a window, virtual ones
+  int kv_pos;  // with a window only, like the rest
+  Hole hole;
+  bool padding;   // not one of the sequence's query_lens tokens: left alone
 };
 
 // Sequence of query token qi: the largest s with query_start_loc[s] <= qi (empty sequences share
@@ -185,6 +217,7 @@ struct QueryPlace {
 // seq_len - q_len + (qi - start) (:115-131), the causal and in-sequence cuts (:64-66).
 // Searched by the whole wave, 64 entries at a time: one load for up to 64 sequences, two for up to
 // 4096, where a binary search is a chain of log2 of them.
+template <bool WIN>
 __device__ __forceinline__ QueryPlace place_query(const PaParams& p, int qi) {
   const int lane = threadIdx.x & 63;
   int lo = 0, len = p.num_seqs;
@@ -201,7 +234,86 @@ __device__ __forceinline__ QueryPlace place_query(const PaParams& p, int qi) {
   const int kv_pos = seq_len - p.qlens[lo] + (qi - p.qsl[lo]);
   int kv_len = kv_pos + 1 < seq_len ? kv_pos + 1 : seq_len;
   if (kv_len < 0) kv_len = 0;
-  return {lo, kv_len};
+  if constexpr (!WIN) {
+    return {lo, kv_len};
+  } else {
+    const int i = qi - p.qsl[lo];
+    const Hole hole = hole_of(p, kv_len - 1);
+    return {lo, kv_len - hole.gap, kv_len - 1, hole, i < 0 || i >= p.qlens[lo]};
+  }
+}
+
+// A partition's positions t0 .. t0 + n - 1 (virtual with a window) and the physical blocks of the block-table
+// columns that they span, validated once, in LDS: s_blk[column + shift], -1 for an invalid or hidden one.
+template <bool WIN>
+struct PartBlocks {
+  const int* s_blk;
+  int t0, shift_a, shift_b;
+  Hole hole;
+  __device__ __forceinline__ int at(int bi, bool far) const { return s_blk[bi + (WIN && far ? shift_b : shift_a)]; }
+};
+template <bool WIN>
+__device__ __forceinline__ PartBlocks<WIN> stage_blocks(const PaParams& p, const QueryPlace& qp, int t0, int n, int* s_blk) {
+  const int32_t* bt_row = p.bt + (int64_t)qp.seq * p.sbt;
+  const int t1 = t0 + n;
+  auto stage = [&](int bi0, int nbi, int* dst) {
+    for (int i = threadIdx.x; i < nbi; i += kThreads) {
+      const int bi = bi0 + i;
+      int blk = -1;
+      if (!WIN || !hidden_block(p, bi, qp.kv_pos)) {
+        blk = bi < p.max_blocks_per_seq ? bt_row[bi] : -1;
+        if (blk < 0 || blk >= p.num_blocks) {
+          blk = -1;
+          if (p.status) atomicOr(p.status, NS_PA_STATUS_BAD_BLOCK);
+        }
+      }
+      dst[i] = blk;
+    }
+  };
+  PartBlocks<WIN> b;
+  b.s_blk = s_blk;
+  b.t0 = t0;
+  if constexpr (!WIN) {
+    const int bi0 = t0 / p.block_size;
+    stage(bi0, (t1 - 1) / p.block_size - bi0 + 1, s_blk);
+    b.shift_a = -bi0;
+  } else {
+    // the columns below the gap, then those above it: with the parts' ends at most n / block_size + 4 entries, n of
+    // them for blocks of one position
+    b.hole = qp.hole;
+    const int sa = qp.hole.sa, gap = qp.hole.gap;
+    int na = 0, bi0 = 0;
+    if (t0 < sa) {
+      bi0 = t0 / p.block_size;
+      na = (min(t1, sa) - 1) / p.block_size - bi0 + 1;
+      stage(bi0, na, s_blk);
+    }
+    b.shift_a = -bi0;
+    b.shift_b = 0;
+    if (t1 > sa) {
+      const int bi1 = (max(t0, sa) + gap) / p.block_size;
+      stage(bi1, (t1 - 1 + gap) / p.block_size - bi1 + 1, s_blk + na);
+      b.shift_b = na - bi1;
+    }
+  }
+  return b;
+}
+// Position j of the partition: its block (-1: invalid, or hidden by the window) and its offset in the block.
+template <bool WIN>
+__device__ __forceinline__ int part_block(const PaParams& p, const PartBlocks<WIN>& b, int j, int& off) {
+  const int v = b.t0 + j;
+  const bool far = WIN && v >= b.hole.sa;
+  const int t = v + (far ? b.hole.gap : 0);
+  int bi;
+  if (p.bs_shift >= 0) {  // the usual case (16): a shift and a mask instead of an integer division
+    bi = t >> p.bs_shift;
+    off = t & (p.block_size - 1);
+  } else {
+    bi = t / p.block_size;
+    off = t - bi * p.block_size;
+  }
+  const int blk = b.at(bi, far);
+  return WIN && v >= p.sinks && v < b.hole.h1 ? -1 : blk;
 }
 
 // ---- matrix core ------------------------------------------------------------------------------
@@ -400,7 +512,7 @@ __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int 
 }
 
 // float32: vector arithmetic, a partition's scores in LDS.
-template <int D, int G>
+template <int D, int G, bool WIN>
 __global__ __launch_bounds__(kThreads) void pa_partition_kernel(PaParams p) {
   // L lanes per KV position, DS dims each: 8 lanes, or 16 for eight heads of 128 dims (the query
   // slices and accumulators of eight heads would not fit the registers at 16 dims a lane)
@@ -424,7 +536,8 @@ __global__ __launch_bounds__(kThreads) void pa_partition_kernel(PaParams p) {
   }
   const int slot = lane / L;  // position within a row of the batch
   const int dl = lane % L;     // dim slice
-  const QueryPlace qp = place_query(p, qi);
+  const QueryPlace qp = place_query<WIN>(p, qi);
+  if (WIN && qp.padding) return;
   const int n_parts = (qp.kv_len + p.part_tokens - 1) / p.part_tokens;
 
   if (part == 0 && n_parts > p.max_parts && threadIdx.x == 0 && p.status)
@@ -437,22 +550,8 @@ __global__ __launch_bounds__(kThreads) void pa_partition_kernel(PaParams p) {
     return;
   }
   const int t0 = part * p.part_tokens;
-  const int t1 = min(qp.kv_len, t0 + p.part_tokens);
-  const int n = t1 - t0;
-  const int32_t* bt_row = p.bt + (int64_t)qp.seq * p.sbt;
-
-  // the partition's slice of the block table, validated once, into LDS
-  const int bi0 = t0 / p.block_size;
-  const int nbi = (t1 - 1) / p.block_size - bi0 + 1;
-  for (int i = threadIdx.x; i < nbi; i += kThreads) {
-    const int bi = bi0 + i;
-    int blk = bi < p.max_blocks_per_seq ? bt_row[bi] : -1;
-    if (blk < 0 || blk >= p.num_blocks) {
-      blk = -1;
-      if (p.status) atomicOr(p.status, NS_PA_STATUS_BAD_BLOCK);
-    }
-    s_blk[i] = blk;
-  }
+  const int n = min(qp.kv_len, t0 + p.part_tokens) - t0;
+  const PartBlocks<WIN> blocks = stage_blocks<WIN>(p, qp, t0, n, s_blk);
 
   // query slices, pre-scaled into log2 units
   float qv[G][DS];
@@ -465,20 +564,8 @@ __global__ __launch_bounds__(kThreads) void pa_partition_kernel(PaParams p) {
   __syncthreads();
 
   // Position j of the partition for sub-row r of the batch starting at base; its physical block
-  // from LDS (-1: past the partition or an invalid entry).
-  auto block_of = [&](int j, int& off) -> int {
-    if (j >= n) return -1;
-    const int t = t0 + j;
-    int bi;
-    if (p.bs_shift >= 0) {  // the usual case (16): a shift and a mask instead of an integer division
-      bi = t >> p.bs_shift;
-      off = t & (p.block_size - 1);
-    } else {
-      bi = t / p.block_size;
-      off = t - bi * p.block_size;
-    }
-    return s_blk[bi - bi0];
-  };
+  // from LDS (-1: past the partition, an invalid entry or hidden).
+  auto block_of = [&](int j, int& off) -> int { return j >= n ? -1 : part_block<WIN>(p, blocks, j, off); };
 
   // pass 1: scores -> LDS. A wave takes batches of kBatch positions (wave w: batches w, w + 4, ...);
   // each lane requests its kSub rows of the batch before any arithmetic.
@@ -586,19 +673,18 @@ __global__ __launch_bounds__(kThreads) void pa_partition_kernel(PaParams p) {
 // for a negative one), and its weights of up to 2^8 can overflow on values near bfloat16's largest.  One thread per
 // score and per output, rows read element by element: a partition of 1024 positions takes some hundred
 // microseconds, on such values alone.  Leaves the sums in s_buf as (wave, head, dim), all in wave 0.
-template <typename T, int D, int G>
-__device__ __forceinline__ void plain_partition(const PaParams& p, int qi, int kvh, int t0, int n, const int* s_blk,
+template <typename T, int D, int G, bool WIN>
+__device__ __forceinline__ void plain_partition(const PaParams& p, int qi, int kvh, int n, const PartBlocks<WIN>& blocks,
                                                 float* s_buf, float* s_m, float* s_l) {
   using M = Mma<T>;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int bi0 = t0 / p.block_size;
   auto words = [](const void* base, int64_t elem) -> const uint32_t* {   // of a row, 16-byte aligned
     return reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(base) + elem);
   };
   for (int e = threadIdx.x; e < G * n; e += kThreads) {
     const int g = e / n, j = e - g * n;
-    const int bi = (t0 + j) / p.block_size, off = t0 + j - bi * p.block_size;
-    const int blk = s_blk[bi - bi0];
+    int off;
+    const int blk = part_block<WIN>(p, blocks, j, off);
     float sc = -INFINITY;
     if (blk >= 0) {
       const uint32_t* q = words(p.q, (int64_t)qi * p.sq_tok + (int64_t)(kvh * G + g) * p.sq_head);
@@ -637,8 +723,8 @@ __device__ __forceinline__ void plain_partition(const PaParams& p, int qi, int k
     if (e >= G * D) continue;
     const int g = e / D, d = e % D;
     for (int j = 0; j < n; ++j) {
-      const int bi = (t0 + j) / p.block_size, off = t0 + j - bi * p.block_size;
-      const int blk = s_blk[bi - bi0];
+      int off;
+      const int blk = part_block<WIN>(p, blocks, j, off);
       if (blk < 0) continue;
       const uint32_t w =
           words(p.v, (int64_t)blk * p.sv_blk + (int64_t)off * p.sv_tok + (int64_t)kvh * p.sv_head)[d >> 1];
@@ -685,7 +771,7 @@ __device__ __forceinline__ void plain_partition(const PaParams& p, int qi, int k
 // registers of 168): four spill, and an earlier form took 63 us with them at 8 x 8192, 111 at 64 x 2048 and 63
 // at 256 rows of up to 512, with two 61, 103 and 60, with three 58, 107 and 57.
 // BW as in the prefill kernel: a row's address is a scalar plus a lane's fixed offset.
-template <typename T, int D, int G, bool BW>
+template <typename T, int D, int G, bool BW, bool WIN>
 __global__ __launch_bounds__(kThreads)
     __attribute__((amdgpu_waves_per_eu(D == 128 ? 3 : 4, D == 128 ? 3 : 4))) void pa_decode_kernel(PaParams p) {
   using M = Mma<T>;
@@ -711,7 +797,8 @@ __global__ __launch_bounds__(kThreads)
     if (threadIdx.x == 0 && part == 0 && kvh == 0 && p.status) atomicOr(p.status, NS_PA_STATUS_BAD_TILE);
     return;
   }
-  const QueryPlace qp = place_query(p, qi);
+  const QueryPlace qp = place_query<WIN>(p, qi);
+  if (WIN && qp.padding) return;
   const int n_parts = (qp.kv_len + p.part_tokens - 1) / p.part_tokens;
   if (part == 0 && n_parts > p.max_parts && threadIdx.x == 0 && p.status)
     atomicOr(p.status, NS_PA_STATUS_SEQ_TOO_LONG);
@@ -724,20 +811,7 @@ __global__ __launch_bounds__(kThreads)
   }
   const int t0 = part * p.part_tokens;
   const int n = min(qp.kv_len, t0 + p.part_tokens) - t0;
-  const int32_t* bt_row = p.bt + (int64_t)qp.seq * p.sbt;
-
-  // the partition's slice of the block table, validated once, into LDS
-  const int bi0 = t0 / p.block_size;
-  const int nbi = (t0 + n - 1) / p.block_size - bi0 + 1;
-  for (int i = threadIdx.x; i < nbi; i += kThreads) {
-    const int bi = bi0 + i;
-    int blk = bi < p.max_blocks_per_seq ? bt_row[bi] : -1;
-    if (blk < 0 || blk >= p.num_blocks) {
-      blk = -1;
-      if (p.status) atomicOr(p.status, NS_PA_STATUS_BAD_BLOCK);
-    }
-    s_blk[i] = blk;
-  }
+  const PartBlocks<WIN> blocks = stage_blocks<WIN>(p, qp, t0, n, s_blk);
   if (threadIdx.x == 0) s_odd = 0;
 
   const int c16 = lane & 15, q4 = lane >> 4;
@@ -777,7 +851,9 @@ __global__ __launch_bounds__(kThreads)
     for (int i = 0; i < NL; ++i) {
       // the instruction's first row, past the end the last group again; or the lane's own row
       const int jr = base + RPI * i + (BW ? 0 : row0);
-      const int t = t0 + min(jr, BW ? (n - 1) & -RPI : n - 1);
+      int t = t0 + min(jr, BW ? (n - 1) & -RPI : n - 1);
+      const bool far = WIN && t >= blocks.hole.sa;
+      if constexpr (WIN) t += far ? blocks.hole.gap : 0;
       int bi;
       if (BW || p.bs_shift >= 0) {
         bi = t >> p.bs_shift;
@@ -786,7 +862,7 @@ __global__ __launch_bounds__(kThreads)
         bi = t / p.block_size;
         off[i] = t - bi * p.block_size;
       }
-      blk[i] = s_blk[bi - bi0];
+      blk[i] = blocks.at(bi, far);
       if constexpr (BW) blk[i] = __builtin_amdgcn_readfirstlane(blk[i]);
       if constexpr (BW) {
         ok |= blk[i] >= 0 ? ((1u << RPI) - 1u) << (RPI * i) : 0u;
@@ -798,6 +874,10 @@ __global__ __launch_bounds__(kThreads)
       if (blk[i] < 0) blk[i] = 0;   // block 0 stands in for an invalid one; its rows are not used
     }
     if (n - base < kStep) ok &= n > base ? (1u << (n - base)) - 1u : 0u;
+    if constexpr (WIN) {   // rows [sinks, h1) are hidden
+      const int a = max(p.sinks - t0 - base, 0), b = min(blocks.hole.h1 - t0 - base, kStep);
+      if (a < b) ok &= ~((0xffffffffu >> (32 - b)) & (0xffffffffu << a));
+    }
   };
   auto load_k = [&]() {
 #pragma unroll
@@ -967,7 +1047,7 @@ __global__ __launch_bounds__(kThreads)
   __syncthreads();
   finish_partition<T, D, G>(p, qi, kvh, part, n_parts, [&](int w, int g, int d) { return s_red[(w * G + g) * D + d]; },
                             s_m, s_l, s_red, &s_odd,
-                            [&]() { plain_partition<T, D, G>(p, qi, kvh, t0, n, s_blk, s_red, s_m, s_l); });
+                            [&]() { plain_partition<T, D, G, WIN>(p, qi, kvh, n, blocks, s_red, s_m, s_l); });
 }
 
 // ---- prefill kernel: query tiles on MFMA -------------------------------------------------------
@@ -1034,11 +1114,13 @@ struct PfParams {
 struct PfTile {
   int seq, t0, nq;
   int kv_pos0;   // the first token's KV position
-  int lt;        // positions the last token sees, up to the call's capacity
+  int lt;        // positions the last token sees, up to the call's capacity (virtual ones with a window)
   int steps;     // 64-position steps (at least 1), or 0: not a tile of this batch
   bool cut;      // the sequence is longer than the capacity
+  Hole hole;     // with a window: the first token's
 };
 
+template <bool WIN>
 __device__ __forceinline__ PfTile pf_tile(const PaParams& p, const PfParams& f, int tile, int bq) {
   PfTile r;
   r.seq = f.tiles[3 * tile];
@@ -1056,6 +1138,10 @@ __device__ __forceinline__ PfTile pf_tile(const PaParams& p, const PfParams& f, 
   r.kv_pos0 = seq_len - ql + (r.t0 - q0);
   int lt = r.kv_pos0 + r.nq < seq_len ? r.kv_pos0 + r.nq : seq_len;
   if (lt < 0) lt = 0;
+  if constexpr (WIN) {   // the tile's first window begins first: what it leaves out, all of them do
+    r.hole = hole_of(p, r.kv_pos0 > -1 ? r.kv_pos0 : -1);
+    lt -= r.hole.gap;
+  }
   r.cut = lt > f.cap;
   r.lt = r.cut ? (int)f.cap : lt;
   r.steps = r.lt > 0 ? (r.lt + kPfPos - 1) / kPfPos : 1;
@@ -1072,11 +1158,91 @@ __device__ __forceinline__ f32x2 ld_dev2(const float* p) {
   return f32x2{__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))};
 }
 
+// One query column of a tile by one wave in float arithmetic, one position after the other, each lane D / 64 dims:
+// what the windowed kernel falls back to for a column whose output is not finite.
+template <typename T, int D>
+__device__ __forceinline__ void plain_column(const PaParams& p, const PfTile& t, int c, int G, int kvh, int lane) {
+  using M = Mma<T>;
+  constexpr int E = D / 64;
+  const int tok = c / G;
+  if (tok >= t.nq) return;
+  const int h = kvh * G + c % G, d0 = lane * E;
+  auto element = [](const void* base, int64_t at) -> float {
+    return M::lo(reinterpret_cast<const uint16_t*>(base)[at]);
+  };
+  float q[E], o[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    q[i] = element(p.q, (int64_t)(t.t0 + tok) * p.sq_tok + (int64_t)h * p.sq_head + d0 + i) * p.scale_log2;
+    o[i] = 0.f;
+  }
+  const int n = min(t.kv_pos0 + tok + 1 - t.hole.gap, t.lt);
+  const int h1 = t.hole.h1 + tok;
+  const int32_t* bt_row = p.bt + (int64_t)t.seq * p.sbt;
+  float m = -INFINITY, l = 0.f;
+  for (int v = 0; v < n; ++v) {
+    if (v >= p.sinks && v < h1) {
+      v = h1 - 1;
+      continue;
+    }
+    const int j = t.hole.position(v);
+    const int bi = j / p.block_size, off = j - bi * p.block_size;
+    const int blk = bi < p.max_blocks_per_seq ? bt_row[bi] : -1;
+    if (blk < 0 || blk >= p.num_blocks) continue;
+    const int64_t at = (int64_t)blk * p.sk_blk + (int64_t)off * p.sk_tok + (int64_t)kvh * p.sk_head + d0;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) s = fmaf(q[i], element(p.k, at + i), s);
+    s = wave_sum(s);
+    const float mn = fmaxf(m, s);
+    const float alpha = mn == -INFINITY ? 0.f : exp2f(m - mn), w = mn == -INFINITY ? 0.f : exp2f(s - mn);
+    m = mn;
+    l = fmaf(l, alpha, w);
+    const int64_t vt = (int64_t)blk * p.sv_blk + (int64_t)off * p.sv_tok + (int64_t)kvh * p.sv_head + d0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = fmaf(w, element(p.v, vt + i), alpha == 1.f ? o[i] : o[i] * alpha);
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    store_one<T>(p.out, (int64_t)(t.t0 + tok) * p.so_tok + (int64_t)h * p.so_head + d0 + i, l > 0.f ? o[i] / l : 0.f);
+}
+
+// The columns whose written outputs are not finite, of the tiles that a workgroup finished in its run u0 .. u1 of steps
+// from step `off` of (tile, kvh) on, again in float arithmetic.  An infinite or NaN value makes NaN of the zero weight
+// that a token of the tile has which does not see it, and of the two parts of one that does where infinity is right.
+template <typename T, int D, int G>
+__device__ __forceinline__ void redo_columns(const PaParams& p, const PfParams& f, int tile, int kvh, int off, int64_t u0,
+                                             int64_t u1, int ended) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __builtin_amdgcn_s_waitcnt(0);   // the wave's own stores are out
+  for (int64_t u = u0; u < u1; off = 0, ++tile) {
+    if (tile == f.n_tiles) {
+      tile = 0;
+      ++kvh;
+    }
+    const PfTile t = pf_tile<true>(p, f, tile, kPfCols / G);
+    if (t.steps == 0) continue;
+    const int take = (int)(u1 - u < t.steps - off ? u1 - u : t.steps - off);
+    u += take;
+    if (take < t.steps && !(ended & (off > 0 ? 1 : 2))) continue;   // cut, and merged by another
+    for (int c = 32 * wave; c < 32 * wave + 32 && c / G < t.nq; ++c) {
+      const uint16_t* out = reinterpret_cast<const uint16_t*>(p.out) + (int64_t)(t.t0 + c / G) * p.so_tok +
+                            (int64_t)(kvh * G + c % G) * p.so_head;
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i)
+        odd |= !(fabsf(Mma<T>::lo(__hip_atomic_load(out + lane + 64 * i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))) <
+                 INFINITY);
+      if (__ballot(odd) != 0ull) plain_column<T, D>(p, t, c, G, kvh, lane);
+    }
+  }
+}
+
 // BW: the block size is a power of two and at least the consecutive positions one load instruction
 // of a wave covers (4 at 128 dims, 8 at 64), so these never straddle two blocks: the block is the
 // wave's, and a row's address a scalar address plus a lane's fixed offset instead of 64-bit products
 // per lane (four 512-token chunks up to 8192 positions: 257 -> 228 us).
-template <typename T, int D, int G, bool BW>
+template <typename T, int D, int G, bool BW, bool WIN>
 __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void pa_prefill_kernel(PaParams p,
                                                                                                         PfParams f) {
   using M = Mma<T>;
@@ -1097,6 +1263,9 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
   __shared__ int s_place[2];   // the workgroup's first tile and its step in it
   __shared__ int s_bad;        // an invalid block met in this segment
   __shared__ int s_last;
+  // with a window: an output that is not finite was written; the run's first tile, its KV head and its step in it;
+  // which of the run's cut tiles this workgroup merged (1: one begun by another, 2: one that it began)
+  __shared__ int s_odd, s_run[3], s_ended;
 
   const int wave = threadIdx.x >> 6;
   const int n_tiles = f.n_tiles;
@@ -1113,7 +1282,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     const int first = tid * q;
     int64_t mine = 0;
     for (int i = first; i < first + q && i < n_tiles; ++i) {
-      const PfTile t = pf_tile(p, f, i, BQ);
+      const PfTile t = pf_tile<WIN>(p, f, i, BQ);
       mine += t.steps;
       if (blockIdx.x == 0 && p.status) {
         if (t.steps == 0) atomicOr(p.status, NS_PA_STATUS_BAD_TILE);
@@ -1147,7 +1316,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
       int64_t at = rem - pre;
       int i = first;
       for (;; ++i) {   // the thread's steps hold `at`: one of its tiles does
-        const int n = pf_tile(p, f, i, BQ).steps;
+        const int n = pf_tile<WIN>(p, f, i, BQ).steps;
         if (at < n) break;
         at -= n;
       }
@@ -1160,7 +1329,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
   } else {
     tile = blockIdx.x % n_tiles;
     kvh = blockIdx.x / n_tiles;
-    const PfTile t = pf_tile(p, f, tile, BQ);
+    const PfTile t = pf_tile<WIN>(p, f, tile, BQ);
     if (threadIdx.x == 0 && kvh == 0 && p.status) {
       if (t.steps == 0) atomicOr(p.status, NS_PA_STATUS_BAD_TILE);
       if (t.cut) atomicOr(p.status, NS_PA_STATUS_SEQ_TOO_LONG);
@@ -1175,12 +1344,19 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
   const int wv = __builtin_amdgcn_readfirstlane(wave);
   const float scale = f.scale_log2;
 
+  if (WIN && threadIdx.x == 0) {   // written again only behind the barriers of a tile's steps
+    s_odd = s_ended = 0;
+    s_run[0] = tile;
+    s_run[1] = kvh;
+    s_run[2] = off;
+  }
+  if constexpr (WIN) __syncthreads();
   for (int64_t u = u0; u < u1;) {
     if (tile == n_tiles) {
       tile = 0;
       ++kvh;
     }
-    const PfTile t = pf_tile(p, f, tile, BQ);
+    const PfTile t = pf_tile<WIN>(p, f, tile, BQ);
     if (t.steps == 0) {   // not a tile of this batch: no units
       ++tile;
       continue;
@@ -1212,7 +1388,8 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     // visible positions of the lane's column (-1: a padding column, never written)
     int kvl = -1;
     if (c < BQ * G && tok < t.nq) {
-      const int kl = t.kv_pos0 + tok + 1 < t.lt ? t.kv_pos0 + tok + 1 : t.lt;
+      const int seen = t.kv_pos0 + tok + 1 - (WIN ? t.hole.gap : 0);
+      const int kl = seen < t.lt ? seen : t.lt;
       kvl = kl > 0 ? kl : 0;
     }
     const bool live = __ballot(kvl >= 0) != 0ull;   // a wave of padding columns only loads rows
@@ -1224,6 +1401,13 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     int kend_w = kvl >= 0 ? kend : INT32_MAX;
 #pragma unroll
     for (int sh = 1; sh < 64; sh <<= 1) kend_w = min(kend_w, __shfl_xor(kend_w, sh));
+    // with a window, positions from sinks on are hidden too: those below h1_t from every token of the tile, those below
+    // h1_w from some token of the wave, those below kvl - window from the column
+    int h1_t = 0, h1_w = 0;
+    if constexpr (WIN) {
+      h1_t = t.hole.h1;
+      h1_w = h1_t + min((wv * 32 + 31) / G, t.nq - 1);
+    }
     const int32_t* bt_row = p.bt + (int64_t)t.seq * p.sbt;
     const char* kbase = reinterpret_cast<const char*>(p.k) + (int64_t)kvh * p.sk_head * 2;
     const char* vbase = reinterpret_cast<const char*>(p.v) + (int64_t)kvh * p.sv_head * 2;
@@ -1246,6 +1430,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     // step ahead of the rows, the rows one step ahead of the products.  Chunk r of the thread is
     // position (tid + kPfThreads r) / CPP of a step.
     auto split = [&](int j, int& o) -> int {
+      if constexpr (WIN) j = t.hole.position(j);
       int bi;
       if (BW || p.bs_shift >= 0) { bi = j >> p.bs_shift; o = j & (p.block_size - 1); }
       else { bi = j / p.block_size; o = j - bi * p.block_size; }
@@ -1266,16 +1451,18 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     };
     auto load_rows = [&](int jt) {
       bad_rows = 0u;
+      [[maybe_unused]] bool loud = false;   // one of them is not merely hidden by the window
 #pragma unroll
       for (int r = 0; r < LPT; ++r) {
         int o;
-        split(BW ? group_of(jt, r) : min(jt + (tid + kPfThreads * r) / CPP, j1 - 1), o);
+        [[maybe_unused]] const int bi = split(BW ? group_of(jt, r) : min(jt + (tid + kPfThreads * r) / CPP, j1 - 1), o);
         int b = BW ? __builtin_amdgcn_readfirstlane(blk[r]) : blk[r];
         // an invalid entry of the segment (past its end, its last one again): block 0 stands in, the
         // rows are not used
         const bool bad = (uint32_t)b >= (uint32_t)p.num_blocks;
         b = bad ? 0 : b;
         bad_rows |= bad ? 1u << r : 0u;
+        if (WIN && bad && !hidden_block(p, bi, t.kv_pos0)) loud = true;
         if constexpr (BW) {   // block strides below 2^31: one 32 x 32 bit product each
           kreg[r] = *reinterpret_cast<const u32x4*>(
               kbase + ((uint64_t)(uint32_t)b * (uint32_t)p.sk_blk + (uint32_t)(o * sk_tok)) * 2 + koff);
@@ -1286,7 +1473,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
           vreg[r] = *reinterpret_cast<const u32x4*>(vbase + ((int64_t)b * p.sv_blk + o * sv_tok) * 2 + 16 * dc0);
         }
       }
-      if (bad_rows != 0u) {
+      if (WIN ? loud : bad_rows != 0u) {
         s_bad = 1;
         if (p.status) atomicOr(p.status, NS_PA_STATUS_BAD_BLOCK);
       }
@@ -1296,6 +1483,13 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
         for (int r = 0; r < LPT; ++r)
           if (((bad_rows >> r) & 1u) || jt + (tid + kPfThreads * r) / CPP >= j1) vreg[r] = u32x4{0u, 0u, 0u, 0u};
+      }
+      if (WIN && jt < h1_t && jt + kPfPos > p.sinks) {   // nor of a row that every token of the tile has hidden
+#pragma unroll
+        for (int r = 0; r < LPT; ++r) {
+          const int j = jt + (tid + kPfThreads * r) / CPP;
+          if (j >= p.sinks && j < h1_t) vreg[r] = u32x4{0u, 0u, 0u, 0u};
+        }
       }
 #pragma unroll
       for (int r = 0; r < LPT; ++r) {
@@ -1350,15 +1544,30 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
         // the online softmax of the lane's column over the step's 64 positions (element e of block
         // rb: position 32 rb + 8 (e / 4) + 4 h + e % 4; the other half in lane ^ 32)
         const bool bad = s_bad != 0;
-        if (jt + kPfPos > kend_w || bad) {   // a position of the step hidden from a column
+        const bool behind = WIN && jt < h1_w && jt + kPfPos > p.sinks;   // some of it behind a window
+        if (jt + kPfPos > kend_w || bad || behind) {   // a position of the step hidden from a column
+          [[maybe_unused]] const uint32_t hlen = (uint32_t)max(kvl - p.window - p.sinks, 0);
 #pragma unroll
           for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const int r = 32 * rb + 8 * (e >> 2) + 4 * h + (e & 3);
               st[rb][e] = jt + r < kend ? st[rb][e] : -INFINITY;
+              if constexpr (WIN) st[rb][e] = (uint32_t)(jt - p.sinks + r) >= hlen ? st[rb][e] : -INFINITY;
             }
-          if (bad) {   // look the step's blocks up again
+          if constexpr (WIN) {
+            if (bad) {   // look the step's blocks up again, a position a lane
+              int o;
+              const int bi = split(min(jt + lane, j1 - 1), o);
+              const int b = bi < p.max_blocks_per_seq ? bt_row[bi] : -1;
+              const uint64_t gone = __ballot((uint32_t)b >= (uint32_t)p.num_blocks) >> (4 * h);
+#pragma unroll
+              for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  if ((uint32_t)(gone >> (32 * rb + 8 * (e >> 2) + (e & 3))) & 1u) st[rb][e] = -INFINITY;
+            }
+          } else if (bad) {   // look the step's blocks up again
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
@@ -1449,6 +1658,14 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
             for (int i = 0; i < 4; ++i) store_one<T>(p.out, d + i, x[i]);
           }
         }
+      if constexpr (WIN) {
+        float z = 0.f;   // NaN with an output that is not finite
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z = fmaf(o[db][e], 0.f, z);
+        if (z != 0.f) s_odd = 1;
+      }
     };
     if (take == t.steps) {
       write_out(acc, l);
@@ -1479,6 +1696,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
       if (tid == 0) s_last = atomicAdd(counter, 1) == arrivals - 1;
       __syncthreads();
       if (s_last) {
+        if (WIN && tid == 0) s_ended |= w == wa ? 2 : 1;
         if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (live) {
           float mx = -INFINITY;
@@ -1493,16 +1711,27 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
             const int64_t slot = __builtin_amdgcn_readfirstlane(i == wa ? begin_slot : i);
             const float* src = f.ws_acc + (slot * kPfWaves + wv) * SW + 2 * lane;
             const f32x2 ml = ld_dev2(f.ws_ml + (slot * kPfCols + c) * 2);
-            f32x2 a[D / 4];   // all of a segment's loads issued before the first is used
+            // a segment's loads are issued before the first is used (with a window, half of them at a time: all
+            // at once need one register more than there is at 128 dims)
+            constexpr int NA = D / (WIN ? 8 : 4);
+            f32x2 a[NA];
 #pragma unroll
-            for (int e = 0; e < D / 4; ++e) a[e] = ld_dev2(src + e * 128);
+            for (int e = 0; e < NA; ++e) a[e] = ld_dev2(src + e * 128);
             // a segment whose keys were all skipped (m = -inf) weighs 0
             const float wt = ml[0] == -INFINITY ? 0.f : exp2f(ml[0] - mx);
             L = fmaf(wt, ml[1], L);
 #pragma unroll
-            for (int e = 0; e < D / 4; ++e) {
-              acc[e / 8][2 * (e % 8)] = fmaf(wt, a[e][0], acc[e / 8][2 * (e % 8)]);
-              acc[e / 8][2 * (e % 8) + 1] = fmaf(wt, a[e][1], acc[e / 8][2 * (e % 8) + 1]);
+            for (int e0 = 0; e0 < D / 4; e0 += NA) {
+              if (e0 > 0) {
+#pragma unroll
+                for (int e = 0; e < NA; ++e) a[e] = ld_dev2(src + (e0 + e) * 128);
+              }
+#pragma unroll
+              for (int e1 = 0; e1 < NA; ++e1) {
+                const int e = e0 + e1;
+                acc[e / 8][2 * (e % 8)] = fmaf(wt, a[e1][0], acc[e / 8][2 * (e % 8)]);
+                acc[e / 8][2 * (e % 8) + 1] = fmaf(wt, a[e1][1], acc[e / 8][2 * (e % 8) + 1]);
+              }
             }
           }
           write_out(acc, L);
@@ -1512,6 +1741,16 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     u += take;
     off = 0;
     ++tile;
+  }
+  if constexpr (WIN) {
+    __syncthreads();
+    if (__builtin_expect(s_odd != 0, 0)) {
+      // The arguments are read anew, hidden from the compiler, which would hold them in registers throughout.
+      uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+      asm volatile("" : "+s"(args));
+      const PaParams pa = *reinterpret_cast<const PaParams*>(args);
+      redo_columns<T, D, G>(pa, f, s_run[0], s_run[1], s_run[2], u0, u1, s_ended);
+    }
   }
 }
 
@@ -1592,75 +1831,94 @@ uint64_t workspace_bytes(int32_t total_q, int32_t hq, int32_t hkv, int32_t head_
 
 // n_tokens decode workgroups along x (p.tokens or the first n_tokens tokens); the prefill tiles
 // when f.tiles is set (16-bit types only)
-template <typename T, int D, int G>
+template <typename T, int D, int G, bool WIN>
 void launch(const PaParams& p, const PfParams& f, int n_tokens, int n_tiles, hipStream_t stream) {
   const dim3 grid(n_tokens, p.hkv, p.max_parts > 0 ? p.max_parts : 1);
   if constexpr (Elem<T>::bytes == 4) {
-    if (n_tokens > 0) hipLaunchKernelGGL((pa_partition_kernel<D, G>), grid, dim3(kThreads), 0, stream, p);
+    if (n_tokens > 0) hipLaunchKernelGGL((pa_partition_kernel<D, G, WIN>), grid, dim3(kThreads), 0, stream, p);
   } else {
     // scalar row addresses: power-of-two blocks that hold a wave's load, block strides in 32 bits
     const bool by_wave = p.bs_shift >= 0 && p.block_size >= 512 / D && p.sk_blk >= 0 && p.sv_blk >= 0 &&
                          p.sk_blk < INT32_MAX && p.sv_blk < INT32_MAX;
     const dim3 tiles((unsigned)(f.grid > 0 ? f.grid : n_tiles * p.hkv));
     if (n_tokens > 0) {
-      if (by_wave) hipLaunchKernelGGL((pa_decode_kernel<T, D, G, true>), grid, dim3(kThreads), 0, stream, p);
-      else hipLaunchKernelGGL((pa_decode_kernel<T, D, G, false>), grid, dim3(kThreads), 0, stream, p);
+      if (by_wave) hipLaunchKernelGGL((pa_decode_kernel<T, D, G, true, WIN>), grid, dim3(kThreads), 0, stream, p);
+      else hipLaunchKernelGGL((pa_decode_kernel<T, D, G, false, WIN>), grid, dim3(kThreads), 0, stream, p);
     }
     if (n_tiles > 0) {
-      if (by_wave) hipLaunchKernelGGL((pa_prefill_kernel<T, D, G, true>), tiles, dim3(kPfThreads), 0, stream, p, f);
-      else hipLaunchKernelGGL((pa_prefill_kernel<T, D, G, false>), tiles, dim3(kPfThreads), 0, stream, p, f);
+      if (by_wave) hipLaunchKernelGGL((pa_prefill_kernel<T, D, G, true, WIN>), tiles, dim3(kPfThreads), 0, stream, p, f);
+      else hipLaunchKernelGGL((pa_prefill_kernel<T, D, G, false, WIN>), tiles, dim3(kPfThreads), 0, stream, p, f);
     }
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool WIN>
 void launch_g(const PaParams& p, const PfParams& f, int n_tokens, int n_tiles, int g, hipStream_t stream) {
   switch (g) {
-    case 1: launch<T, D, 1>(p, f, n_tokens, n_tiles, stream); break;
-    case 2: launch<T, D, 2>(p, f, n_tokens, n_tiles, stream); break;
-    case 3: launch<T, D, 3>(p, f, n_tokens, n_tiles, stream); break;
-    case 4: launch<T, D, 4>(p, f, n_tokens, n_tiles, stream); break;
-    default: launch<T, D, 8>(p, f, n_tokens, n_tiles, stream); break;
+    case 1: launch<T, D, 1, WIN>(p, f, n_tokens, n_tiles, stream); break;
+    case 2: launch<T, D, 2, WIN>(p, f, n_tokens, n_tiles, stream); break;
+    case 3: launch<T, D, 3, WIN>(p, f, n_tokens, n_tiles, stream); break;
+    case 4: launch<T, D, 4, WIN>(p, f, n_tokens, n_tiles, stream); break;
+    default: launch<T, D, 8, WIN>(p, f, n_tokens, n_tiles, stream); break;
   }
 }
 
 template <typename T>
 void launch_d(const PaParams& p, const PfParams& f, int n_tokens, int n_tiles, int d, int g, hipStream_t stream) {
-  if (d == 64) launch_g<T, 64>(p, f, n_tokens, n_tiles, g, stream);
-  else launch_g<T, 128>(p, f, n_tokens, n_tiles, g, stream);
+  const bool win = p.window > 0;
+  if (d == 64) {
+    if (win) launch_g<T, 64, true>(p, f, n_tokens, n_tiles, g, stream);
+    else launch_g<T, 64, false>(p, f, n_tokens, n_tiles, g, stream);
+  } else {
+    if (win) launch_g<T, 128, true>(p, f, n_tokens, n_tiles, g, stream);
+    else launch_g<T, 128, false>(p, f, n_tokens, n_tiles, g, stream);
+  }
 }
 
-}  // namespace
+// The positions that a query token, or a tile of up to `tokens` consecutive ones, can have to walk: max_seq_len, with a
+// window (0: none) at most the sinks, the window and the tokens, with their ends rounded to kAlign.
+int32_t walked(int32_t max_seq_len, int32_t window, int32_t sinks, int32_t tokens) {
+  if (window == 0) return max_seq_len;
+  const int64_t most = (((int64_t)sinks + kAlign - 1) & -kAlign) + window + kAlign - 1 + tokens - 1;
+  return most < max_seq_len ? (int32_t)most : max_seq_len;
+}
 
-extern "C" {
-
-int ns_pa_abi_version(void) { return NS_PA_ABI_VERSION; }
-
-const char* ns_pa_last_error(void) { return g_err; }
-
-int ns_paged_attention_workspace_bytes(int32_t total_q, int32_t num_heads_q, int32_t num_kv_heads,
-                                       int32_t head_dim, int32_t max_seq_len, uint64_t* bytes) {
-  if (!bytes) return fail("bytes is NULL");
-  if (check_sizes(total_q, num_heads_q, num_kv_heads, head_dim, max_seq_len)) return 1;
-  *bytes = workspace_bytes(total_q, num_heads_q, num_kv_heads, head_dim, max_seq_len);
+int check_window(int32_t& window, int32_t& sinks) {
+  if (window < 1) return fail("window must be at least 1 (got %d)", window);
+  if (sinks < 0) return fail("sinks must be >= 0 (got %d)", sinks);
+  if (window > kMaxWindow) window = kMaxWindow;
+  if (sinks > kMaxWindow) sinks = kMaxWindow;
   return 0;
 }
 
-int ns_paged_attention_call_workspace(const ns_paged_attn_args* a, uint64_t* bytes, uint64_t* counters) {
-  if (!a || !bytes || !counters) return fail("a pointer argument is NULL");
+struct Sizes {
+  int32_t n_tokens, n_tiles;       // workgroups along x of the per-token kernel, tiles
+  int32_t token_len, tile_len;     // positions that one of them can have to walk
+  uint64_t token_bytes, tile_bytes;   // of workspace
+};
+
+Sizes sizes_of(const ns_paged_attn_args* a, int32_t window, int32_t sinks) {
+  Sizes z;
+  z.n_tokens = a->decode_tokens ? a->n_decode_tokens : a->total_q;
+  z.n_tiles = a->prefill_tiles ? a->n_prefill_tiles : 0;
+  z.token_len = walked(a->max_seq_len, window, sinks, 1);
+  z.tile_len = walked(a->max_seq_len, window, sinks, kPfCols / (a->num_heads_q / a->num_kv_heads));
+  z.token_bytes = workspace_bytes(a->total_q, a->num_heads_q, a->num_kv_heads, a->head_dim, z.token_len, z.n_tokens);
+  z.tile_bytes = pf_workspace_bytes(z.n_tiles, a->num_kv_heads, a->head_dim, z.tile_len);
+  return z;
+}
+
+int call_workspace(const ns_paged_attn_args* a, int32_t window, int32_t sinks, uint64_t* bytes, uint64_t* counters) {
   if (check_sizes(a->total_q, a->num_heads_q, a->num_kv_heads, a->head_dim, a->max_seq_len)) return 1;
   if (a->n_decode_tokens < 0 || a->n_prefill_tiles < 0) return fail("token and tile counts must be >= 0");
-  const int32_t n_tokens = a->decode_tokens ? a->n_decode_tokens : a->total_q;
-  const uint64_t dec =
-      workspace_bytes(a->total_q, a->num_heads_q, a->num_kv_heads, a->head_dim, a->max_seq_len, n_tokens);
-  const int32_t tiles = a->prefill_tiles ? a->n_prefill_tiles : 0;
-  *bytes = dec + pf_workspace_bytes(tiles, a->num_kv_heads, a->head_dim, a->max_seq_len);
-  *counters = (uint64_t)a->total_q * a->num_kv_heads + (uint64_t)tiles * a->num_kv_heads;
+  const Sizes z = sizes_of(a, window, sinks);
+  *bytes = z.token_bytes + z.tile_bytes;
+  *counters = (uint64_t)a->total_q * a->num_kv_heads + (uint64_t)z.n_tiles * a->num_kv_heads;
   return 0;
 }
 
-int ns_paged_attention(const ns_paged_attn_args* a, hipStream_t stream) {
-  if (!a) return fail("args is NULL");
+// A call, checked and launched; window 0: without one.
+int attend(const ns_paged_attn_args* a, int32_t window, int32_t sinks, hipStream_t stream) {
   if (check_sizes(a->total_q, a->num_heads_q, a->num_kv_heads, a->head_dim, a->max_seq_len)) return 1;
   if (a->dtype != NS_PA_DTYPE_F32 && a->dtype != NS_PA_DTYPE_BF16 && a->dtype != NS_PA_DTYPE_F16)
     return fail("dtype must be NS_PA_DTYPE_F32, _BF16 or _F16 (got %d)", a->dtype);
@@ -1691,21 +1949,19 @@ int ns_paged_attention(const ns_paged_attn_args* a, hipStream_t stream) {
     return fail("prefill tiles take bfloat16 or float16 (float32 queries go through the per-token kernel)");
   if (a->prefill_tiles && !a->decode_tokens)
     return fail("a call with prefill tiles lists its other query tokens in decode_tokens");
-  const int32_t n_tiles = a->prefill_tiles ? a->n_prefill_tiles : 0;
-  const int32_t n_tokens = a->decode_tokens ? a->n_decode_tokens : a->total_q;
-  const uint64_t need =
-      workspace_bytes(a->total_q, a->num_heads_q, a->num_kv_heads, a->head_dim, a->max_seq_len, n_tokens);
+  const Sizes z = sizes_of(a, window, sinks);
+  const int32_t n_tiles = z.n_tiles, n_tokens = z.n_tokens;
+  const uint64_t need = z.token_bytes, pf_need = z.tile_bytes;
   if (need > 0 && !a->counters) return fail("a call with split rows needs the zero-filled counters buffer");
-  const int part = part_tokens_for(n_tokens, a->num_kv_heads, a->max_seq_len);
-  const int64_t max_parts = ((int64_t)a->max_seq_len + part - 1) / part;
+  const int part = part_tokens_for(n_tokens, a->num_kv_heads, z.token_len);
+  const int64_t max_parts = ((int64_t)z.token_len + part - 1) / part;
   if (max_parts > 65535) return fail("max_seq_len too large");
-  const uint64_t pf_need = pf_workspace_bytes(n_tiles, a->num_kv_heads, a->head_dim, a->max_seq_len);
   if (need + pf_need > 0 && (!a->workspace || a->workspace_bytes < need + pf_need))
     return fail("workspace of %llu bytes needed (got %llu)", (unsigned long long)(need + pf_need),
                 (unsigned long long)a->workspace_bytes);
   if (pf_need > 0 && !a->counters) return fail("a call with split tiles needs the zero-filled counters buffer");
-  const int pf_part = pf_part_tokens_for(n_tiles, a->num_kv_heads, a->max_seq_len);
-  const int64_t pf_max_parts = ((int64_t)a->max_seq_len + pf_part - 1) / pf_part;
+  const int pf_part = pf_part_tokens_for(n_tiles, a->num_kv_heads, z.tile_len);
+  const int64_t pf_max_parts = ((int64_t)z.tile_len + pf_part - 1) / pf_part;
   if (pf_max_parts > 65535) return fail("max_seq_len too large");
 
   PaParams p;
@@ -1749,11 +2005,13 @@ int ns_paged_attention(const ns_paged_attn_args* a, hipStream_t stream) {
   p.scale_log2 = a->scale * kLog2e;
   p.total_q = a->total_q;
   p.tokens = a->decode_tokens;
+  p.window = window;
+  p.sinks = sinks;
 
   PfParams f;
   f.tiles = a->prefill_tiles;
   char* ws = reinterpret_cast<char*>(a->workspace);
-  f.grid = pf_grid_for(n_tiles, a->num_kv_heads, a->max_seq_len);
+  f.grid = pf_grid_for(n_tiles, a->num_kv_heads, z.tile_len);
   if (((uintptr_t)a->workspace + need) % 8 != 0) f.grid = 0;   // the partials go in 8-byte pieces
   f.n_tiles = n_tiles;
   f.ws_acc = pf_need ? reinterpret_cast<float*>(ws + need) : nullptr;
@@ -1774,6 +2032,44 @@ int ns_paged_attention(const ns_paged_attn_args* a, hipStream_t stream) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail("kernel launch failed: %s", hipGetErrorString(e));
   return 0;
+}
+}  // namespace
+
+extern "C" {
+
+int ns_pa_abi_version(void) { return NS_PA_ABI_VERSION; }
+
+const char* ns_pa_last_error(void) { return g_err; }
+
+int ns_paged_attention_workspace_bytes(int32_t total_q, int32_t num_heads_q, int32_t num_kv_heads,
+                                       int32_t head_dim, int32_t max_seq_len, uint64_t* bytes) {
+  if (!bytes) return fail("bytes is NULL");
+  if (check_sizes(total_q, num_heads_q, num_kv_heads, head_dim, max_seq_len)) return 1;
+  *bytes = workspace_bytes(total_q, num_heads_q, num_kv_heads, head_dim, max_seq_len);
+  return 0;
+}
+
+int ns_paged_attention_call_workspace(const ns_paged_attn_args* a, uint64_t* bytes, uint64_t* counters) {
+  if (!a || !bytes || !counters) return fail("a pointer argument is NULL");
+  return call_workspace(a, 0, 0, bytes, counters);
+}
+
+int ns_paged_attention_windowed_workspace(const ns_paged_attn_args* a, int32_t window, int32_t sinks, uint64_t* bytes,
+                                          uint64_t* counters) {
+  if (!a || !bytes || !counters) return fail("a pointer argument is NULL");
+  if (check_window(window, sinks)) return 1;
+  return call_workspace(a, window, sinks, bytes, counters);
+}
+
+int ns_paged_attention(const ns_paged_attn_args* a, hipStream_t stream) {
+  if (!a) return fail("args is NULL");
+  return attend(a, 0, 0, stream);
+}
+
+int ns_paged_attention_windowed(const ns_paged_attn_args* a, int32_t window, int32_t sinks, hipStream_t stream) {
+  if (!a) return fail("args is NULL");
+  if (check_window(window, sinks)) return 1;
+  return attend(a, window, sinks, stream);
 }
 
 }  // extern "C"

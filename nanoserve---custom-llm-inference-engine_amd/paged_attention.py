@@ -18,6 +18,10 @@ Differences from the reference's launcher, all on the host side:
     ``PREFILL_MIN_QUERY`` query tokens (bfloat16 and float16) are cut into query tiles of
     ``128 // G`` tokens for the MFMA prefill kernel, which reads each key and value row once per
     tile; the other query tokens go to the per-token kernel.
+
+``window`` and ``sinks``: attention with a sliding window and a few first tokens that stay visible
+(the reference attends to the whole context).  The cache pages between the two are not read, so they
+can be released (``kv_cache.PagePool.release``).
 """
 from __future__ import annotations
 
@@ -41,7 +45,8 @@ TILE_COLUMNS = 128         # query columns of a prefill tile (NS_PA_TILE_COLUMNS
 PREFILL_MIN_QUERY = 2      # sequences with at least this many query tokens go by tile
 
 EXPORTS = ("ns_pa_abi_version", "ns_pa_last_error", "ns_paged_attention_workspace_bytes",
-           "ns_paged_attention_call_workspace", "ns_paged_attention")
+           "ns_paged_attention_call_workspace", "ns_paged_attention", "ns_paged_attention_windowed_workspace",
+           "ns_paged_attention_windowed")
 
 
 class PagedAttentionError(RuntimeError):
@@ -116,6 +121,13 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
                                                       ctypes.POINTER(ctypes.c_uint64)]
     lib.ns_paged_attention.restype = ctypes.c_int
     lib.ns_paged_attention.argtypes = [ctypes.POINTER(NsPagedAttnArgs), ctypes.c_void_p]
+    lib.ns_paged_attention_windowed_workspace.restype = ctypes.c_int
+    lib.ns_paged_attention_windowed_workspace.argtypes = [ctypes.POINTER(NsPagedAttnArgs), ctypes.c_int32,
+                                                          ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64),
+                                                          ctypes.POINTER(ctypes.c_uint64)]
+    lib.ns_paged_attention_windowed.restype = ctypes.c_int
+    lib.ns_paged_attention_windowed.argtypes = [ctypes.POINTER(NsPagedAttnArgs), ctypes.c_int32, ctypes.c_int32,
+                                                ctypes.c_void_p]
     if lib.ns_pa_abi_version() != ABI_VERSION:
         raise PagedAttentionError(f"ABI {lib.ns_pa_abi_version()} in {path}, expected {ABI_VERSION}")
     _LIB = lib
@@ -230,7 +242,7 @@ def _i32(t, device):
 def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
                         scale: float, block_size: int, *, max_seq_len: Optional[int] = None,
                         max_query_len: Optional[int] = None, plan: Optional[PagedAttentionPlan] = None,
-                        out=None, workspace=None, counters=None, status=None, stream=None):
+                        window: Optional[int] = None, sinks: int = 0, out=None, workspace=None, counters=None, status=None, stream=None):
     """Attention of every query token over its sequence's paged KV (the reference's
     ``paged_attention_triton``; same arguments, same result up to float32 rounding order).
 
@@ -246,10 +258,19 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
     ``PagedAttentionPlan`` of this batch layout (then nothing is read on the host).  ``stream``: a
     ``torch.cuda.Stream`` or a raw HIP stream handle, default the current stream; the call's own temporaries
     are made on it, so nothing orders them against another.
+
+    ``window`` (at least 1; None: the whole context): a query at KV position p sees the ``window`` positions up to
+    its own, t > p - window, and the sequence's first ``sinks`` positions.  Block-table entries of blocks that no
+    token of the call sees are not read, so they may hold anything (a released block's -1).  Query rows that are
+    none of a sequence's ``query_lens`` tokens (a padded batch's) are left as they were.
     """
     import torch
 
     lib = load()
+    if window is not None and not 1 <= window < 2 ** 31:
+        raise PagedAttentionError(f"window must be at least 1 and below 2^31 (got {window})")
+    if not 0 <= sinks < 2 ** 31:
+        raise PagedAttentionError(f"sinks must lie in [0, 2^31) (got {sinks})")
     dev = query.device
     if dev.type != "cuda":
         raise PagedAttentionError("paged_attention_hip needs device tensors")
@@ -257,8 +278,8 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
         s = torch.cuda.current_stream(dev)
         if dev.index == torch.cuda.current_device():   # already where the call goes: no stream to switch to and back
             return _paged_attention_on(lib, s, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc,
-                                       query_lens, scale, block_size, max_seq_len, max_query_len, plan, out,
-                                       workspace, counters, status)
+                                       query_lens, scale, block_size, max_seq_len, max_query_len, plan, window,
+                                       sinks, out, workspace, counters, status)
     elif isinstance(stream, torch.cuda.Stream):
         s = stream
     elif int(stream) == 0:
@@ -270,12 +291,13 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
         s = torch.cuda.ExternalStream(int(stream), device=dev)
     with torch.cuda.stream(s):
         return _paged_attention_on(lib, s, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc,
-                                   query_lens, scale, block_size, max_seq_len, max_query_len, plan, out,
-                                   workspace, counters, status)
+                                   query_lens, scale, block_size, max_seq_len, max_query_len, plan, window,
+                                   sinks, out, workspace, counters, status)
 
 
 def _paged_attention_on(lib, s, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
-                        scale, block_size, max_seq_len, max_query_len, plan, out, workspace, counters, status):
+                        scale, block_size, max_seq_len, max_query_len, plan, window, sinks, out, workspace,
+                        counters, status):
     """paged_attention_hip with ``s`` the current stream: every temporary below is made on it."""
     import torch
 
@@ -306,7 +328,8 @@ def _paged_attention_on(lib, s, query, k_cache, v_cache, block_tables, seq_lens,
     # prefill tiles: 16-bit types, unless the caller declares a decode step
     tiles = tokens = None
     if plan is not None:
-        if plan.total_q != total_q or plan.num_heads_q != hq or plan.num_kv_heads != hkv:
+        # (a padded batch's rows behind the plan's are left alone with a window)
+        if plan.total_q > total_q or (window is None and plan.total_q < total_q) or plan.num_heads_q != hq or plan.num_kv_heads != hkv:
             raise PagedAttentionError("the plan was made for another batch layout or head layout")
         if max_seq_len is None:
             max_seq_len = plan.max_seq_len
@@ -342,7 +365,11 @@ def _paged_attention_on(lib, s, query, k_cache, v_cache, block_tables, seq_lens,
         a.decode_tokens, a.n_decode_tokens = tokens
         a.prefill_tiles, a.n_prefill_tiles = tiles
     need_b, need_c = ctypes.c_uint64(0), ctypes.c_uint64(0)
-    _check(lib.ns_paged_attention_call_workspace(ctypes.byref(a), ctypes.byref(need_b), ctypes.byref(need_c)))
+    if window is None:
+        _check(lib.ns_paged_attention_call_workspace(ctypes.byref(a), ctypes.byref(need_b), ctypes.byref(need_c)))
+    else:
+        _check(lib.ns_paged_attention_windowed_workspace(ctypes.byref(a), window, sinks, ctypes.byref(need_b),
+                                                         ctypes.byref(need_c)))
     need, ncount = int(need_b.value), int(need_c.value)
     if need and workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
@@ -357,7 +384,11 @@ def _paged_attention_on(lib, s, query, k_cache, v_cache, block_tables, seq_lens,
         raise PagedAttentionError(f"counters must be an int32 device tensor of at least {ncount} entries")
     if need:
         a.workspace, a.workspace_bytes, a.counters = workspace.data_ptr(), need, counters.data_ptr()
-    _check(lib.ns_paged_attention(ctypes.byref(a), ctypes.c_void_p(int(s.cuda_stream))))
+    handle = ctypes.c_void_p(int(s.cuda_stream))
+    if window is None:
+        _check(lib.ns_paged_attention(ctypes.byref(a), handle))
+    else:
+        _check(lib.ns_paged_attention_windowed(ctypes.byref(a), window, sinks, handle))
     return out
 
 

@@ -41,14 +41,17 @@ def query_places(seq_lens, query_start_loc, query_lens):
 
 
 def paged_attention(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
-                    scale: float, block_size: int, terms: bool = False):
+                    scale: float, block_size: int, terms: bool = False, window=None, sinks: int = 0):
     """float64 (total_q, Hq, D) attention output (paged_attention_triton.py:19-106).
 
     ``terms``: also return, per output element, the condition term ``S * dev + Vabs`` that scales a
     float computation's rounding error: S = max over visible keys of ``scale * sum_i |q_i k_i|``
     (a dot product's error is at most proportional to it, and it moves the output by the softmax
     weights times ``v - o``), dev = ``sum_t w_t |v_t - o|``, Vabs = ``sum_t w_t |v_t|`` (the
-    weighted sum's own error bound, w the normalised weights)."""
+    weighted sum's own error bound, w the normalised weights).
+
+    ``window``, ``sinks``: a query at position p sees t <= p with t > p - window or t < sinks (window
+    None: all t <= p); nothing of the others, block-table entry included, is looked at."""
     q = np.asarray(query, dtype=np.float64)
     kc = np.asarray(k_cache, dtype=np.float64)
     vc = np.asarray(v_cache, dtype=np.float64)
@@ -62,6 +65,8 @@ def paged_attention(query, k_cache, v_cache, block_tables, seq_lens, query_start
         if kv_len == 0:
             continue
         t = np.arange(kv_len)
+        if window is not None:
+            t = t[(t > kv_len - 1 - window) | (t < sinks)]
         blk = bt[s, t // block_size]
         slot = t % block_size
         k = kc[blk, slot]  # (kv_len, Hkv, D)

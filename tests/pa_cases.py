@@ -43,6 +43,16 @@ def make_case(seed, seq_lens, query_lens, hq=24, hkv=8, d=128, block_size=16, dt
                 block_size=block_size)
 
 
+def release_hidden(case, window, sinks, entry=-1):
+    """Overwrites the block-table entries of the blocks that no query token of the case sees."""
+    bs, bt = case["block_size"], case["block_tables"]
+    for s, (n, m) in enumerate(zip(case["seq_lens"].tolist(), case["query_lens"].tolist())):
+        first = n - m - window + 1
+        for j in range(-(-sinks // bs), max(0, first) // bs):
+            bt[s, j] = entry
+    return case
+
+
 def oracle_args(case):
     """The case as float64/int numpy arrays for the oracle."""
     out = {}
