@@ -20,6 +20,9 @@ OUT = os.path.join(HERE, "libns_sampling.so")
 # paged attention (its own ABI, include/ns_paged_attention.h)
 PA_SRC = os.path.join(HERE, "csrc", "ns_paged_attention.hip")
 PA_OUT = os.path.join(HERE, "libns_paged_attention.so")
+# the paged KV cache: the store of new rows and the pages (include/ns_kv_cache.h)
+KV_SRC = os.path.join(HERE, "csrc", "ns_kv_cache.hip")
+KV_OUT = os.path.join(HERE, "libns_kv_cache.so")
 # the benchmark's bandwidth reference (not part of the sampler's ABI)
 PROBE_SRC = os.path.join(HERE, "csrc", "ns_probe.hip")
 PROBE_OUT = os.path.join(HERE, "libns_probe.so")
@@ -49,8 +52,8 @@ def _command(src: str, out: str, defines=()) -> list:
 
 
 def build(verbose: bool = False) -> str:
-    """Compile every library, the four hipcc processes side by side."""
-    jobs = [(SRC, OUT, ()), (PA_SRC, PA_OUT, ()), (PROBE_SRC, PROBE_OUT, ()),
+    """Compile every library, the hipcc processes side by side."""
+    jobs = [(SRC, OUT, ()), (PA_SRC, PA_OUT, ()), (KV_SRC, KV_OUT, ()), (PROBE_SRC, PROBE_OUT, ()),
             (SRC, STAMPS_OUT, ("NS_PHASE_STAMPS",))]
     procs = []
     for src, out, defines in jobs:
