@@ -19,6 +19,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 from typing import Optional
 
 import torch
@@ -70,6 +71,10 @@ class NsKvPool(ctypes.Structure):
                 + [(n, ctypes.c_int32) for n in ("num_rows", "num_cols", "num_pages", "num_tensors", "block_size")])
 
 
+# NsKvStoreArgs as packed bytes: a third of the time that filling the structure takes
+_STORE = struct.Struct("@12P15q9i")
+_STORE_PAD = bytes(ctypes.sizeof(NsKvStoreArgs) - _STORE.size)
+
 _LIB: Optional[ctypes.CDLL] = None
 
 
@@ -83,7 +88,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib = ctypes.CDLL(path)
     p, i, pool = ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(NsKvPool)
     for name, args in (("ns_kv_abi_version", []), ("ns_kv_last_error", []),
-                       ("ns_kv_store", [ctypes.POINTER(NsKvStoreArgs), p]),
+                       ("ns_kv_store", [ctypes.c_char_p, p]),
                        ("ns_kv_scratch_bytes", [i, i, ctypes.POINTER(ctypes.c_uint64)]),
                        ("ns_kv_extend", [pool, p, p, i, p]), ("ns_kv_fork", [pool, p, p, i, p]),
                        ("ns_kv_free", [pool, p, i, p]), ("ns_kv_release", [pool, p, i, i, i, p]),
@@ -102,13 +107,16 @@ def _check(rc: int) -> None:
         raise KvCacheError(load().ns_kv_last_error().decode())
 
 
-def _on(dev, stream):
-    """(HIP stream handle, context) of a call: the current stream of ``dev``, a torch stream or a raw handle (0: the
-    default stream).  Inside the context the call's temporaries are made on that stream."""
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on(dev: int, stream):
+    """(HIP stream handle, context) of a call on device ``dev``: its current stream, a torch stream or a raw handle (0:
+    the default stream).  Inside the context the call's temporaries are made on that stream."""
     if stream is None:
+        if dev == torch.cuda.current_device():
+            return torch._C._cuda_getCurrentRawStream(dev), _NO_SWITCH
         s = torch.cuda.current_stream(dev)
-        if dev.index == torch.cuda.current_device():
-            return s.cuda_stream, contextlib.nullcontext()
     elif isinstance(stream, torch.cuda.Stream):
         s = stream
     elif int(stream) == 0:
@@ -121,7 +129,7 @@ def _on(dev, stream):
 def _i32(t, dev, name):
     if t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
         return t
-    if t.is_floating_point() or t.is_complex():
+    if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
         raise KvCacheError(f"{name} must be an integer tensor")
     return t.to(device=dev, dtype=torch.int32).contiguous()
 
@@ -143,76 +151,94 @@ def store_kv_hip(key, value, k_cache, v_cache, block_tables, seq_lens, query_sta
     STATUS_BAD_PAGE is ORed into when a token has no valid page (its row is then not stored).  ``stream``: a
     ``torch.cuda.Stream`` or a raw handle, default the current stream.
     """
-    lib = load()
-    dev = k_cache.device
-    if key.dim() != 3 or key.shape != value.shape or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
-        raise KvCacheError(f"key {tuple(key.shape)} and value {tuple(value.shape)} must match, and k_cache "
-                           f"{tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)}")
-    total, hkv, d = key.shape
-    nb, bs, h, dc = k_cache.shape
-    if (h, dc) != (hkv, d):
-        raise KvCacheError(f"the caches' rows ({h}, {dc}) are not the keys' ({hkv}, {d})")
-    if bs != block_size:
-        raise KvCacheError(f"block_size {block_size} != the cache's {bs}")
-    dtype = k_cache.dtype
-    if dtype not in _DTYPES:
-        raise KvCacheError(f"unsupported dtype {dtype} (float32, bfloat16, float16)")
-    if query is None:
-        if out is not None:
-            raise KvCacheError("out is where the rotated query goes: it needs query")
-        hq = 0
-    else:
-        if inv_freq is None:
-            raise KvCacheError("a query is there to be rotated: it needs inv_freq")
-        if query.dim() != 3 or query.shape[0] != total or query.shape[2] != d:
-            raise KvCacheError(f"query {tuple(query.shape)} does not match the keys' {tuple(key.shape)}")
-        hq = query.shape[1]
-    if inv_freq is not None and (inv_freq.dtype is not torch.float32 or inv_freq.shape != (d // 2,)
-                                 or not inv_freq.is_contiguous()):
-        raise KvCacheError(f"inv_freq must be a contiguous float32 tensor of {d // 2} elements")
-    if out is not None and out.shape != query.shape:
-        raise KvCacheError("out must match query's shape")
-    for name, t in (("key", key), ("value", value), ("k_cache", k_cache), ("v_cache", v_cache), ("query", query),
-                    ("out", out)):
-        if t is None:
-            continue
-        if t.dtype is not dtype or t.device != dev:
-            raise KvCacheError(f"{name} must share the cache's dtype and device")
-        if t.stride(-1) != 1:
-            raise KvCacheError(f"{name} must have a unit head_dim stride")
-    if inv_freq is not None and inv_freq.device != dev:
-        raise KvCacheError("inv_freq must be on the cache's device")
-    if status is not None and (status.dtype is not torch.int32 or status.device != dev or status.numel() < 1):
+    lib = _LIB or load()
+    shape, pages, dtype, dev = key.shape, k_cache.shape, k_cache.dtype, k_cache.get_device()
+    ks, vs, kc, vc = key.stride(), value.stride(), k_cache.stride(), v_cache.stride()
+    # one pass over what has to hold; a call that fails it is looked at again for its message
+    if not (len(shape) == 3 and value.shape == shape and len(pages) == 4 and v_cache.shape == pages
+            and pages[2:] == shape[1:] and pages[1] == block_size and dtype in _DTYPES and key.dtype is dtype
+            and value.dtype is dtype and v_cache.dtype is dtype and key.get_device() == dev
+            and value.get_device() == dev and v_cache.get_device() == dev and ks[2] == vs[2] == kc[3] == vc[3] == 1):
+        _refuse_store(key, value, k_cache, v_cache, block_size)
+    total, hkv, d = shape
+    if status is not None and (status.dtype is not torch.int32 or status.get_device() != dev or status.numel() < 1):
         raise KvCacheError("status must be an int32 device tensor")
     if block_tables.dim() != 2:
         raise KvCacheError("block_tables must have two dimensions")
-    num_seqs = block_tables.shape[0]
+    num_seqs, cols = block_tables.shape
     if seq_lens.numel() != num_seqs or query_lens.numel() != num_seqs or query_start_loc.numel() != num_seqs + 1:
         raise KvCacheError("seq_lens/query_lens need num_seqs entries and query_start_loc num_seqs + 1")
-    if dev.type != "cuda":
+    if inv_freq is not None and (inv_freq.dtype is not torch.float32 or inv_freq.shape != (d // 2,)
+                                 or inv_freq.get_device() != dev or not inv_freq.is_contiguous()):
+        raise KvCacheError(f"inv_freq must be a contiguous float32 tensor of {d // 2} elements on the cache's device")
+    hq = q_at = out_at = qs0 = qs1 = os0 = os1 = 0
+    if query is not None:
+        if inv_freq is None:
+            raise KvCacheError("a query is there to be rotated: it needs inv_freq")
+        q_shape = query.shape
+        if len(q_shape) != 3 or q_shape[0] != total or q_shape[2] != d:
+            raise KvCacheError(f"query {tuple(q_shape)} does not match the keys' {tuple(shape)}")
+        _row_tensor("query", query, dtype, dev)
+        hq = q_shape[1]
+        if out is not None:
+            if out.shape != q_shape:
+                raise KvCacheError("out must match query's shape")
+            _row_tensor("out", out, dtype, dev)
+    elif out is not None:
+        raise KvCacheError("out is where the rotated query goes: it needs query")
+    if dev < 0:
         raise KvCacheError("store_kv_hip needs device tensors")
     handle, on = _on(dev, stream)
-    with on:
-        if query is not None and out is None:
-            out = torch.empty(query.shape, dtype=dtype, device=dev)
-        if total == 0:
-            return out
-        bt = block_tables
-        if bt.dtype is not torch.int32 or bt.device != dev or bt.stride(1) != 1:
-            bt = _i32(bt, dev, "block_tables")
-        sl, qsl, ql = (_i32(t, dev, n) for t, n in ((seq_lens, "seq_lens"), (query_start_loc, "query_start_loc"),
-                                                    (query_lens, "query_lens")))
-        qs, os_ = (query.stride(), out.stride()) if query is not None else ((0, 0), (0, 0))
-        ks, vs, kc, vc = key.stride(), value.stride(), k_cache.stride(), v_cache.stride()
-        a = NsKvStoreArgs(
-            query.data_ptr() if query is not None else None, key.data_ptr(), value.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), out.data_ptr() if query is not None else None,
-            inv_freq.data_ptr() if inv_freq is not None else None, bt.data_ptr(), sl.data_ptr(), qsl.data_ptr(),
-            ql.data_ptr(), status.data_ptr() if status is not None else None,
-            qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], os_[0], os_[1],
-            bt.stride(0), total, num_seqs, hq, hkv, d, bs, nb, bt.shape[1], _DTYPES[dtype])
-        _check(lib.ns_kv_store(ctypes.byref(a), handle))
+    if on is not _NO_SWITCH:
+        with on:
+            return store_kv_hip(key, value, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
+                                block_size, query=query, inv_freq=inv_freq, out=out, status=status)
+    if query is not None:
+        if out is None:
+            out = torch.empty_like(query)
+            if out.stride(2) != 1 and total:
+                out = torch.empty(q_shape, dtype=dtype, device=query.device)
+        q_at, out_at = query.data_ptr(), out.data_ptr()
+        (qs0, qs1, _), (os0, os1, _) = query.stride(), out.stride()
+    if total == 0:
+        return out
+    if block_tables.dtype is not torch.int32 or block_tables.get_device() != dev or block_tables.stride(1) != 1:
+        block_tables = _i32(block_tables, k_cache.device, "block_tables")
+    sl, qsl, ql = seq_lens, query_start_loc, query_lens
+    if not (sl.dtype is qsl.dtype is ql.dtype is torch.int32 and sl.get_device() == qsl.get_device() == ql.get_device()
+            == dev and sl.is_contiguous() and qsl.is_contiguous() and ql.is_contiguous()):
+        sl, qsl, ql = (_i32(t, k_cache.device, n) for t, n in ((sl, "seq_lens"), (qsl, "query_start_loc"),
+                                                               (ql, "query_lens")))
+    _check(lib.ns_kv_store(_STORE.pack(
+        q_at, key.data_ptr(), value.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out_at,
+        0 if inv_freq is None else inv_freq.data_ptr(), block_tables.data_ptr(), sl.data_ptr(), qsl.data_ptr(),
+        ql.data_ptr(), 0 if status is None else status.data_ptr(),
+        qs0, qs1, ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], os0, os1,
+        block_tables.stride(0), total, num_seqs, hq, hkv, d, block_size, pages[0], cols, _DTYPES[dtype]) + _STORE_PAD,
+        handle))
     return out
+
+
+def _row_tensor(name, t, dtype, dev):
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise KvCacheError(f"{name} must share the cache's dtype and device")
+    if t.stride(-1) != 1:
+        raise KvCacheError(f"{name} must have a unit head_dim stride")
+
+
+def _refuse_store(key, value, k_cache, v_cache, block_size):
+    """Why the rows and caches of a store do not fit one another."""
+    if key.dim() != 3 or key.shape != value.shape or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise KvCacheError(f"key {tuple(key.shape)} and value {tuple(value.shape)} must match, and k_cache "
+                           f"{tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)}")
+    if k_cache.shape[2:] != key.shape[1:]:
+        raise KvCacheError(f"the caches' rows {tuple(k_cache.shape[2:])} are not the keys' {tuple(key.shape[1:])}")
+    if k_cache.shape[1] != block_size:
+        raise KvCacheError(f"block_size {block_size} != the cache's {k_cache.shape[1]}")
+    if k_cache.dtype not in _DTYPES:
+        raise KvCacheError(f"unsupported dtype {k_cache.dtype} (float32, bfloat16, float16)")
+    for name, t in (("key", key), ("value", value), ("k_cache", k_cache), ("v_cache", v_cache)):
+        _row_tensor(name, t, k_cache.dtype, k_cache.get_device())
 
 
 class PagePool:
@@ -268,6 +294,7 @@ class PagePool:
         self.k_caches, self.v_caches = list(k_caches), list(v_caches)
         self.block_tables, self.seq_lens, self.page_refs = block_tables, seq_lens, page_refs
         self.device, self.block_size, self.num_pages = dev, bs, pages
+        self._dev = first.get_device()
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._scratch = torch.zeros(int(need.value), dtype=torch.uint8, device=dev)
         self._tensors = torch.tensor([[c.data_ptr(), c.stride(0) * c.element_size()] for c in caches],
@@ -289,6 +316,9 @@ class PagePool:
                    torch.zeros(max_seqs, dtype=torch.int32, device=dev), refs)
 
     def _list(self, x, name):
+        if isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.dim() == 1 and x.get_device() == self._dev \
+                and x.is_contiguous():
+            return x
         if not isinstance(x, torch.Tensor):
             x = torch.tensor(list(x), dtype=torch.int32)
         if x.dim() != 1:
@@ -305,7 +335,7 @@ class PagePool:
         """Row ``rows[i]`` grows to ``lens[i]`` tokens (its length grows with it) and gets the pages for them, the
         lowest free ones first.  A row is served if the pages that it and the rows listed before it ask for are all
         there; else it is left as it was (NO_PAGES).  At most MAX_ROWS rows a call."""
-        handle, on = _on(self.device, stream)
+        handle, on = _on(self._dev, stream)
         with on:
             rows, lens = self._two(rows, lens, ("rows", "lens"))
             _check(self._lib.ns_kv_extend(self._ref, rows.data_ptr(), lens.data_ptr(), rows.numel(), handle))
@@ -314,14 +344,14 @@ class PagePool:
         """Row ``children[i]``, an empty one, becomes a copy of row ``parents[i]``: full pages are shared, the tokens
         of a last page that is not full are copied, in every layer, to a page of the child's own.  A child for which
         no page is left stays empty (NO_PAGES).  At most MAX_ROWS pairs, and no more than rows, a call."""
-        handle, on = _on(self.device, stream)
+        handle, on = _on(self._dev, stream)
         with on:
             parents, children = self._two(parents, children, ("parents", "children"))
             _check(self._lib.ns_kv_fork(self._ref, parents.data_ptr(), children.data_ptr(), parents.numel(), handle))
 
     def free(self, rows, stream=None) -> None:
         """The rows give up their pages and become empty; a page that no row names any more is free."""
-        handle, on = _on(self.device, stream)
+        handle, on = _on(self._dev, stream)
         with on:
             rows = self._list(rows, "rows")
             _check(self._lib.ns_kv_free(self._ref, rows.data_ptr(), rows.numel(), handle))
@@ -333,7 +363,7 @@ class PagePool:
             raise KvCacheError(f"window must be at least 1 and below 2^31 (got {window})")
         if not 0 <= sinks < 2 ** 31:
             raise KvCacheError(f"sinks must lie in [0, 2^31) (got {sinks})")
-        handle, on = _on(self.device, stream)
+        handle, on = _on(self._dev, stream)
         with on:
             rows = self._list(rows, "rows")
             _check(self._lib.ns_kv_release(self._ref, rows.data_ptr(), rows.numel(), window, sinks, handle))
@@ -348,7 +378,7 @@ class PagePool:
             src, dst = list(src), list(dst)
             if len(set(dst)) != len(dst) or set(src) & set(dst):
                 raise KvCacheError("a page is named twice by dst, or by src and dst")
-        handle, on = _on(self.device, stream)
+        handle, on = _on(self._dev, stream)
         with on:
             src, dst = self._two(src, dst, ("src", "dst"))
             _check(self._lib.ns_kv_copy(self._ref, to._ref, src.data_ptr(), dst.data_ptr(), src.numel(), handle))
@@ -382,7 +412,7 @@ class PagePool:
             raise KvCacheError("the pools' caches differ in layers, page shape, dtype or device")
 
     def _compact(self, to, stream):
-        handle, on = _on(self.device, stream)
+        handle, on = _on(self._dev, stream)
         with on:
             page_map = torch.empty(self.num_pages, dtype=torch.int32, device=self.device)
             _check(self._lib.ns_kv_compact(self._ref, to._ref if to is not None else None, page_map.data_ptr(), handle))
