@@ -29,7 +29,7 @@ extern "C" {
 #define NS_KV_DTYPE_F16 2
 
 /* rows of one ns_kv_extend or ns_kv_fork call */
-#define NS_KV_MAX_ROWS 8192
+#define NS_KV_MAX_ROWS 4096
 
 /* status bits, OR-ed into the word that `status` points to (when not NULL) */
 #define NS_KV_STATUS_BAD_PAGE 1    /* a page number outside the cache, or a position past the table's columns:
@@ -88,7 +88,7 @@ typedef struct ns_kv_pool {
   int32_t*       page_refs;        /* (num_pages), 16-byte aligned */
   int32_t*       status;           /* optional */
   const uint64_t* tensors;         /* (num_tensors, 2): each cache tensor's address and bytes from page to page */
-  int32_t*       scratch;          /* ns_kv_scratch_bytes() bytes, zero-filled once, this pool's own */
+  int32_t*       scratch;          /* ns_kv_scratch_bytes() bytes, any contents, this pool's own */
   uint64_t       scratch_bytes;
   int64_t        stride_bt_row;
   int64_t        slot_bytes;       /* bytes of a token in a page of one tensor, a multiple of 16 */
@@ -105,8 +105,8 @@ const char* ns_kv_last_error(void);
 /* Every function below returns 0, or nonzero on invalid arguments. */
 int ns_kv_store(const ns_kv_store_args* args, hipStream_t stream);
 
-/* Bytes of a pool's scratch memory. */
-int ns_kv_scratch_bytes(int32_t num_rows, int32_t num_pages, uint64_t* bytes);
+/* Bytes of the scratch memory of a pool of num_pages pages. */
+int ns_kv_scratch_bytes(int32_t num_pages, uint64_t* bytes);
 
 /* Rows rows[0 .. n-1] grow to lens[0 .. n-1] tokens and get the pages that these need, the lowest free pages
  * first, in the order of the list.  A row is served if the pages that it and the rows listed before it ask for

@@ -210,10 +210,11 @@ __global__ __launch_bounds__(kStoreThreads) void store_kernel(ns_kv_store_args a
 
 // ---- pages ------------------------------------------------------------------------------------------------
 
-constexpr int kPlan = 1024;          // threads of the planning kernels' one workgroup
+constexpr int kPlan = 1024;          // threads of a planning workgroup
 constexpr int kPlanWaves = kPlan / 64;
-constexpr int kScan = kPlan * 16;    // pages that it looks at together
+constexpr int kGroup = 1024;         // pages that a wave looks at together, 16 consecutive ones a lane
 constexpr int kCopy = 256;
+constexpr int kMaxRows = NS_KV_MAX_ROWS;
 
 __device__ __forceinline__ int pages_of(int tokens, int block_size) {
   return tokens > 0 ? (tokens - 1) / block_size + 1 : 0;
@@ -228,18 +229,12 @@ __device__ __forceinline__ void sync_memory() {
   __syncthreads();
 }
 
-// Exclusive prefix sum of x over the workgroup's threads; *total: the sum.
-__device__ __forceinline__ int block_prefix(int x, int* total) {
+// Sum of a wave's shares before this wave (every lane passes its wave's); *total: of all waves.
+__device__ __forceinline__ int wave_prefix(int x, int* total) {
   __shared__ int s_sum[kPlanWaves];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int in = x;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int y = __shfl_up(in, s);
-    if (lane >= s) in += y;
-  }
+  const int wave = threadIdx.x >> 6;
   __syncthreads();   // an earlier call's sums are read
-  if (lane == 63) s_sum[wave] = in;
+  if ((threadIdx.x & 63) == 0) s_sum[wave] = x;
   __syncthreads();
   int before = 0, all = 0;
 #pragma unroll
@@ -248,69 +243,92 @@ __device__ __forceinline__ int block_prefix(int x, int* total) {
     all += s_sum[w];
   }
   *total = all;
-  return before + in - x;
+  return before;
 }
-
-// Visits the pages with pred(page, count) in ascending order, visit(page, rank), up to `limit` of them; returns how
-// many there are (at least `limit`, or all).  16384 pages at a time: a wave takes 1024 consecutive ones, four loads of
-// 16 bytes a lane, and the lanes' counts of the four loads are summed as 16-bit fields of one word.
-template <typename Pred, typename Visit>
-__device__ __forceinline__ int scan_pages(const int32_t* refs, int n, int limit, Pred pred, Visit visit) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  int found = 0;
-  for (int64_t c0 = 0; c0 < n && found < limit; c0 += kScan) {
-    const int64_t w0 = c0 + wave * 1024;
-    uint32_t bits = 0u;   // bit 4 j + i: page w0 + 256 j + 4 lane + i
+// Exclusive prefix sum of x over the workgroup's threads; *total: the sum.
+__device__ __forceinline__ int block_prefix(int x, int* total) {
+  const int lane = threadIdx.x & 63;
+  int in = x;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t p0 = w0 + 256 * j + 4 * lane;
-      i32x4 x = {0, 0, 0, 0};
-      if (p0 + 3 < n) {
-        x = *reinterpret_cast<const i32x4*>(refs + p0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (p0 + i < n) x[i] = refs[p0 + i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (p0 + i < n && pred((int)(p0 + i), x[i])) bits |= 1u << (4 * j + i);
-    }
-    uint64_t mine = 0ull;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) mine |= (uint64_t)__popc((bits >> (4 * j)) & 15u) << (16 * j);
-    uint64_t in = mine;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const uint64_t y = __shfl_up(in, s);
-      if (lane >= s) in += y;
-    }
-    const uint64_t all = __shfl(in, 63), before = in - mine;
-    int sums[5] = {0};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sums[j + 1] = sums[j] + (int)((all >> (16 * j)) & 0xffffull);
-    int total;
-    // every lane of a wave passes the same share, so that the prefix before it counts whole waves
-    const int at = block_prefix(lane == 0 ? sums[4] : 0, &total);
-    const int wave_at = __shfl(at, 0);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      int r = found + wave_at + sums[j] + (int)((before >> (16 * j)) & 0xffffull);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if ((bits >> (4 * j + i)) & 1u) {
-          if (r < limit) visit((int)(w0 + 256 * j + 4 * lane + i), r);
-          ++r;
-        }
-    }
-    found += total;
+  for (int s = 1; s < 64; s <<= 1) {
+    const int y = __shfl_up(in, s);
+    if (lane >= s) in += y;
   }
-  return found;
+  return wave_prefix(__shfl(in, 63), total) + in - x;
 }
 
-// The request that rank r falls to: the largest i with off[i] <= r.
-__device__ __forceinline__ int request_of(const int* off, int n, int r) {
-  int lo = 0, hi = n;   // off[lo] <= r, off[hi] > r
+// Which of a lane's 16 pages p0 .. p0 + 15 have pred(page, count): bit i for page p0 + i.
+template <typename Pred>
+__device__ __forceinline__ uint32_t pages_with(const int32_t* refs, int n, int64_t p0, Pred pred) {
+  i32x4 x[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[j] = i32x4{0, 0, 0, 0};
+    if (p0 + 4 * j + 3 < n) {
+      x[j] = *reinterpret_cast<const i32x4*>(refs + p0 + 4 * j);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (p0 + 4 * j + i < n) x[j][i] = refs[p0 + 4 * j + i];
+    }
+  }
+  uint32_t bits = 0u;
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (p0 + j < n && pred((int)(p0 + j), x[j / 4][j % 4])) bits |= 1u << j;
+  return bits;
+}
+
+__device__ __forceinline__ int wave_inclusive(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int y = __shfl_up(x, s);
+    if (lane >= s) x += y;
+  }
+  return x;
+}
+
+// What a planning kernel leaves in the pool's scratch memory for the kernel after it: a line for each list entry, and of
+// every group of 1024 pages which are free and how many.
+struct Plan {
+  int32_t* total;    // pages that the list asks for
+  int32_t* off;      // by list entry: the first rank that falls to it
+  int32_t* row;      // its row, -1: nothing to do
+  int32_t* col;      // the column that the first of its pages goes to
+  int32_t* len;      // its new length
+  i32x4* pair;       // of a fork: parent's row, tokens (0: nothing to do), the copy's rank (-1: none), its source
+  int32_t* count;    // by group
+  uint16_t* free;    // by 16 pages, 64 a group
+  int groups;
+  __device__ __forceinline__ explicit Plan(const ns_kv_pool& p) {
+    total = p.scratch;
+    off = total + 4;
+    row = off + kMaxRows;
+    col = row + kMaxRows;
+    len = col + kMaxRows;
+    pair = reinterpret_cast<i32x4*>(off);
+    count = off + 4 * kMaxRows;
+    groups = (int)(((int64_t)p.num_pages + kGroup - 1) / kGroup);
+    free = reinterpret_cast<uint16_t*>(count + groups);
+  }
+};
+constexpr uint64_t plan_ints(uint64_t pages) { return 4 + 4 * (uint64_t)kMaxRows + (pages + kGroup - 1) / kGroup * 33; }
+
+// The groups' free pages, a group a wave, by the workgroups after the first.
+__device__ __forceinline__ void find_free(const ns_kv_pool& p, const Plan& plan) {
+  const int lane = threadIdx.x & 63;
+  const int64_t g = (int64_t)(blockIdx.x - 1) * kPlanWaves + (threadIdx.x >> 6);
+  if (g >= plan.groups) return;
+  const uint32_t bits = pages_with(p.page_refs, p.num_pages, g * kGroup + 16 * lane, [](int, int refs) { return refs == 0; });
+  plan.free[g * 64 + lane] = (uint16_t)bits;
+  const int upto = wave_inclusive(__popc(bits));
+  if (lane == 63) plan.count[g] = upto;
+}
+
+// The request that rank r falls to: the largest i with off[i] <= r, at least lo.
+__device__ __forceinline__ int request_of(const int* off, int lo, int n, int r) {
+  int hi = n;   // off[lo] <= r, off[hi] > r
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (off[mid] <= r) lo = mid;
@@ -319,164 +337,249 @@ __device__ __forceinline__ int request_of(const int* off, int n, int r) {
   return lo;
 }
 
-// The list's rows: claim[row] holds n - i of the first listing i, zero between calls.
-__device__ __forceinline__ void claim_rows(const ns_kv_pool& p, const int32_t* rows, int n) {
-  for (int i = threadIdx.x; i < n; i += kPlan) {
-    const int row = rows[i];
-    if (row >= 0 && row < p.num_rows) atomicMax(p.scratch + row, n - i);
+// A list's rows, each counted where it is listed first: a table of the list's places, hashed by row, in LDS (places of
+// one row meet in one slot, which keeps the lowest).
+constexpr int kSlots = 2 * kMaxRows;   // a power of two, at most half full
+constexpr int kEach = kMaxRows / kPlan;   // list entries a thread takes at most, consecutive ones
+struct Rows {
+  int row[kMaxRows];   // -1: not in the tables
+  int slot[kSlots];
+};
+static_assert((kSlots & (kSlots - 1)) == 0 && kEach * kPlan == kMaxRows, "sizes");
+
+// Fills row with the thread's entries first .. last - 1 (-1: not in the tables); bit k of the result set where entry
+// first + k is its row's first listing.
+__device__ __forceinline__ uint32_t first_listings(Rows& s, const int32_t* rows, int num_rows, int first, int last,
+                                                   int (&row)[kEach]) {
+  for (int i = threadIdx.x; i < kSlots; i += kPlan) s.slot[i] = -1;
+  int at[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    row[k] = first + k < last ? rows[first + k] : -1;
+    if (row[k] >= num_rows || row[k] < 0) row[k] = -1;
+    if (first + k < last) s.row[first + k] = row[k];
   }
-  sync_memory();
-}
-__device__ __forceinline__ bool own_row(const ns_kv_pool& p, const int32_t* rows, int n, int i) {
-  const int row = rows[i];
-  if (row < 0 || row >= p.num_rows) return false;
-  return __hip_atomic_load(p.scratch + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - i;
-}
-__device__ __forceinline__ void drop_claims(const ns_kv_pool& p, const int32_t* rows, int n) {
-  for (int i = threadIdx.x; i < n; i += kPlan) {
-    const int row = rows[i];
-    if (row >= 0 && row < p.num_rows) __hip_atomic_store(p.scratch + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    at[k] = (int)(((uint32_t)row[k] * 2654435769u) >> 16) & (kSlots - 1);
+    while (row[k] >= 0) {   // at most half of the slots are taken, so one is met that is free or the row's own
+      const int held = atomicCAS(&s.slot[at[k]], -1, first + k);
+      if (held < 0) break;
+      if (s.row[held] == row[k]) {
+        atomicMin(&s.slot[at[k]], first + k);
+        break;
+      }
+      at[k] = (at[k] + 1) & (kSlots - 1);
+    }
   }
+  __syncthreads();
+  uint32_t own = 0u;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k)
+    if (row[k] >= 0 && s.slot[at[k]] == first + k) own |= 1u << k;
+  return own;
 }
 
-// One workgroup: the pages that each row needs, their prefix sums, then the free pages in ascending order, each to
-// the row and column that its rank falls to.
-__global__ __launch_bounds__(kPlan) void extend_kernel(ns_kv_pool p, const int32_t* rows, const int32_t* lens, int n) {
-  __shared__ int s_off[NS_KV_MAX_ROWS];
-  const int tid = threadIdx.x;
-  claim_rows(p, rows, n);
+// Extending takes two launches.  The first: one workgroup sums up what the rows ask for, the others find the free
+// pages.  All of it in one workgroup is bound by what one CU gets through (2.8 us for 16,384 pages' counts): a call for
+// 10,400 pages took 18.6 us with 27,000 pages and 38.9 with 160,000 of which a tenth were free, one page 9.1; so 11.6,
+// 11.6 and 10.1 (each with the 5 us that an idle queue takes to start it).
+__global__ __launch_bounds__(kPlan) void extend_plan_kernel(ns_kv_pool p, const int32_t* rows, const int32_t* lens, int n) {
+  __shared__ Rows s;
+  const Plan plan(p);
+  if (blockIdx.x > 0) {
+    find_free(p, plan);
+    return;
+  }
   const int per = (n + kPlan - 1) / kPlan;
-  int mine = 0;
-  for (int i = tid * per; i < min(n, tid * per + per); ++i) {
-    int need = 0;
-    if (!own_row(p, rows, n, i)) {
-      flag(p.status, NS_KV_STATUS_BAD_ROW);
+  const int first = min(n, (int)threadIdx.x * per), last = min(n, first + per);
+  int row[kEach], need[kEach], mine = 0;
+  const uint32_t own = first_listings(s, rows, p.num_rows, first, last, row);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    need[k] = 0;
+    if (first + k >= last) continue;
+    int col = 0, now = 0;
+    if ((own >> k) & 1u) {
+      const int old = p.seq_lens[row[k]];
+      now = lens[first + k];
+      if (old < 0 || now < old || now > (int64_t)p.num_cols * p.block_size) {
+        flag(p.status, NS_KV_STATUS_BAD_LENGTH);
+        row[k] = -1;
+      } else {
+        col = pages_of(old, p.block_size);
+        need[k] = pages_of(now, p.block_size) - col;
+        mine += need[k];
+      }
     } else {
-      const int old = p.seq_lens[rows[i]], now = lens[i];
-      if (old < 0 || now < old || now > (int64_t)p.num_cols * p.block_size) flag(p.status, NS_KV_STATUS_BAD_LENGTH);
-      else need = pages_of(now, p.block_size) - pages_of(old, p.block_size);
+      flag(p.status, NS_KV_STATUS_BAD_ROW);
+      row[k] = -1;
     }
-    s_off[i] = need;
-    mine += need;
+    plan.row[first + k] = row[k];
+    plan.col[first + k] = col;
+    plan.len[first + k] = now;
   }
   int total;
   int at = block_prefix(mine, &total);
-  for (int i = tid * per; i < min(n, tid * per + per); ++i) {
-    const int need = s_off[i];
-    s_off[i] = at;
-    at += need;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k)
+    if (first + k < last) {
+      plan.off[first + k] = at;
+      at += need[k];
+    }
+  if (threadIdx.x == 0) *plan.total = total;
+}
+
+// The second: a wave a group of pages.  Its free pages' ranks follow from the counts of the groups before it; each goes
+// to the row and column that its rank falls to, if all that the row asks for is there.  The first workgroup also sets
+// the rows' lengths.
+__global__ __launch_bounds__(kCopy) void extend_kernel(ns_kv_pool p, int n) {
+  __shared__ int s_off[kMaxRows];
+  const Plan plan(p);
+  const int lane = threadIdx.x & 63;
+  const int64_t g = (int64_t)blockIdx.x * (kCopy / 64) + (threadIdx.x >> 6);
+  const uint32_t bits = g < plan.groups ? plan.free[g * 64 + lane] : 0u;
+  for (int i = threadIdx.x; i < n; i += kCopy) s_off[i] = plan.off[i];
+  const int total = *plan.total;
+  int found = 0, before = 0;
+  for (int c = lane; c < plan.groups; c += 64) {
+    const int x = plan.count[c];
+    found += x;
+    before += c < g ? x : 0;
   }
-  sync_memory();
-  const int found = scan_pages(p.page_refs, p.num_pages, total, [](int, int refs) { return refs == 0; },
-                               [&](int page, int r) {
-                                 const int i = request_of(s_off, n, r);
-                                 const int row = rows[i];
-                                 const int col = pages_of(p.seq_lens[row], p.block_size) + r - s_off[i];
-                                 p.block_tables[(int64_t)row * p.stride_bt_row + col] = page;
-                                 p.page_refs[page] = 1;
-                               });
-  sync_memory();
-  for (int i = tid; i < n; i += kPlan) {
-    if (!own_row(p, rows, n, i)) continue;
-    const int row = rows[i], old = p.seq_lens[row], now = lens[i];
-    if (old < 0 || now < old || now > (int64_t)p.num_cols * p.block_size) continue;
-    const int end = i + 1 < n ? s_off[i + 1] : total;
-    if (end == s_off[i] || end <= found) {
-      p.seq_lens[row] = now;
+  found = __shfl(wave_inclusive(found), 63);
+  before = __shfl(wave_inclusive(before), 63);
+  __syncthreads();
+  auto end_of = [&](int i) -> int { return i + 1 < n ? s_off[i + 1] : total; };
+  const int most = min(total, found);
+  int r = before + wave_inclusive(__popc(bits)) - __popc(bits);
+  int i = -1, end = 0;
+  int32_t* to = nullptr;
+  for (uint32_t left = bits; left != 0u && r < most; left &= left - 1u, ++r) {
+    if (i < 0 || r >= end) {
+      i = request_of(s_off, max(i, 0), n, r);
+      end = end_of(i);
+      if (end > found) break;   // not served, nor are those after it
+      to = p.block_tables + (int64_t)plan.row[i] * p.stride_bt_row + plan.col[i] - s_off[i];
+    }
+    const int page = (int)(g * kGroup) + 16 * lane + __ffs(left) - 1;
+    to[r] = page;
+    p.page_refs[page] = 1;
+  }
+  if (blockIdx.x > 0) return;
+  for (int k = threadIdx.x; k < n; k += kCopy) {
+    const int row = plan.row[k];
+    if (row < 0) continue;
+    if (end_of(k) == s_off[k] || end_of(k) <= found) p.seq_lens[row] = plan.len[k];
+    else flag(p.status, NS_KV_STATUS_NO_PAGES);
+  }
+}
+
+// A fork's first launch, as extending's.
+__global__ __launch_bounds__(kPlan) void fork_plan_kernel(ns_kv_pool p, const int32_t* parents, const int32_t* children, int n) {
+  __shared__ Rows s;
+  const Plan plan(p);
+  if (blockIdx.x > 0) {
+    find_free(p, plan);
+    return;
+  }
+  const int per = (n + kPlan - 1) / kPlan;
+  const int first = min(n, (int)threadIdx.x * per), last = min(n, first + per);
+  int row[kEach], mine = 0;
+  const uint32_t own = first_listings(s, children, p.num_rows, first, last, row);
+  i32x4 x[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    x[k] = i32x4{0, 0, -1, -1};
+    if (first + k >= last) continue;
+    const int parent = parents[first + k];
+    if (!((own >> k) & 1u) || parent < 0 || parent >= p.num_rows || p.seq_lens[row[k]] != 0) {
+      flag(p.status, NS_KV_STATUS_BAD_ROW);
       continue;
     }
-    // not served: what it got of the last free pages goes back
-    flag(p.status, NS_KV_STATUS_NO_PAGES);
-    int32_t* entry = p.block_tables + (int64_t)row * p.stride_bt_row + pages_of(old, p.block_size);
-    for (int r = s_off[i]; r < found; ++r, ++entry) {
-      p.page_refs[*entry] = 0;
-      *entry = -1;
+    x[k][0] = parent;
+    x[k][1] = max(0, (int)min((int64_t)p.seq_lens[parent], (int64_t)p.num_cols * p.block_size));
+    if (x[k][1] % p.block_size != 0) {
+      x[k][3] = p.block_tables[(int64_t)parent * p.stride_bt_row + x[k][1] / p.block_size];
+      if (x[k][3] >= 0 && x[k][3] < p.num_pages) ++mine;
+      else x[k][3] = -1;
     }
-  }
-  sync_memory();   // every claim is read
-  drop_claims(p, rows, n);
-}
-
-// Planning a fork: plan[4 i ..] = parent's row, tokens (0: nothing to do), page of the copy (-1: none), its source.
-__global__ __launch_bounds__(kPlan) void fork_plan_kernel(ns_kv_pool p, const int32_t* parents, const int32_t* children, int n) {
-  __shared__ int s_off[NS_KV_MAX_ROWS];
-  const int tid = threadIdx.x;
-  i32x4* plan = reinterpret_cast<i32x4*>(p.scratch + ((p.num_rows + 3) & -4));
-  claim_rows(p, children, n);
-  const int per = (n + kPlan - 1) / kPlan;
-  int mine = 0;
-  for (int i = tid * per; i < min(n, tid * per + per); ++i) {
-    i32x4 x = {parents[i], 0, -1, -1};
-    int need = 0;
-    if (!own_row(p, children, n, i) || x[0] < 0 || x[0] >= p.num_rows || p.seq_lens[children[i]] != 0) {
-      flag(p.status, NS_KV_STATUS_BAD_ROW);
-      x[0] = 0;
-    } else {
-      const int len = min((int64_t)p.seq_lens[x[0]], (int64_t)p.num_cols * p.block_size);
-      x[1] = max(len, 0);
-      if (x[1] % p.block_size != 0) {
-        x[3] = p.block_tables[(int64_t)x[0] * p.stride_bt_row + x[1] / p.block_size];
-        if (x[3] >= 0 && x[3] < p.num_pages) need = 1;
-        else x[3] = -1;
-      }
-    }
-    plan[i] = x;
-    s_off[i] = need;
-    mine += need;
   }
   int total;
   int at = block_prefix(mine, &total);
-  for (int i = tid * per; i < min(n, tid * per + per); ++i) {
-    const int need = s_off[i];
-    s_off[i] = at;
-    at += need;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    if (first + k >= last) continue;
+    if (x[k][3] >= 0) x[k][2] = at++;
+    plan.pair[first + k] = x[k];
   }
-  sync_memory();
-  const int found = scan_pages(p.page_refs, p.num_pages, total, [](int, int refs) { return refs == 0; },
-                               [&](int page, int r) {
-                                 const int i = request_of(s_off, n, r);
-                                 reinterpret_cast<int32_t*>(plan + i)[2] = page;
-                                 p.page_refs[page] = 1;
-                               });
-  sync_memory();
-  for (int i = tid; i < n; i += kPlan) {
-    i32x4 x = plan[i];
-    if (x[3] >= 0 && s_off[i] >= found) {   // no page was left
-      flag(p.status, NS_KV_STATUS_NO_PAGES);
-      x[1] = 0;
-      plan[i] = x;
+}
+
+// The free page of rank r, by a whole wave; -1: there are no more than r.
+__device__ __forceinline__ int free_page(const Plan& plan, int r) {
+  const int lane = threadIdx.x & 63;
+  for (int g0 = 0; g0 < plan.groups; g0 += 64) {
+    const int x = g0 + lane < plan.groups ? plan.count[g0 + lane] : 0;
+    const int upto = wave_inclusive(x);
+    const uint64_t past = __ballot(upto > r);
+    if (past == 0ull) {
+      r -= __shfl(upto, 63);
+      continue;
     }
-    if (x[1] > 0) p.seq_lens[children[i]] = x[1];
+    const int at = __ffsll((unsigned long long)past) - 1;
+    r -= __shfl(upto - x, at);
+    uint32_t bits = plan.free[(int64_t)(g0 + at) * 64 + lane];
+    const int sum = wave_inclusive(__popc(bits));
+    const int who = __ffsll((unsigned long long)__ballot(sum > r)) - 1;
+    r -= __shfl(sum - __popc(bits), who);
+    bits = __shfl(bits, who);
+    for (; r > 0; --r) bits &= bits - 1u;
+    return (g0 + at) * kGroup + 16 * who + __ffs(bits) - 1;
   }
-  sync_memory();   // every claim is read
-  drop_claims(p, children, n);
+  return -1;
 }
 
-// `bytes` (a multiple of 16) from src to dst by the workgroup
+// `bytes` (a multiple of 16) from src to dst by the workgroup, eight loads a thread in flight
 __device__ __forceinline__ void copy_bytes(char* dst, const char* src, int64_t bytes) {
-  for (int64_t i = (int64_t)threadIdx.x * 16; i < bytes; i += kCopy * 16)
-    *reinterpret_cast<u32x4*>(dst + i) = *reinterpret_cast<const u32x4*>(src + i);
+  constexpr int kStep = kCopy * 16;
+  int64_t i = (int64_t)threadIdx.x * 16;
+  for (; i + 7 * kStep < bytes; i += 8 * kStep) {
+    u32x4 x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + i + u * kStep));
+#pragma unroll
+    for (int u = 0; u < 8; ++u) __builtin_nontemporal_store(x[u], reinterpret_cast<u32x4*>(dst + i + u * kStep));
+  }
+  for (; i < bytes; i += kStep) *reinterpret_cast<u32x4*>(dst + i) = *reinterpret_cast<const u32x4*>(src + i);
 }
 
-// blockIdx.x: the pair; blockIdx.y 0: the child's table row and the shared pages' counts, else the copy in one tensor
+// A fork's second launch.  blockIdx.x: the pair; blockIdx.y 0: the child's table row and length and the shared pages'
+// counts, else the copy in one tensor.  Every wave finds the copy's page for itself.
 __global__ __launch_bounds__(kCopy) void fork_kernel(ns_kv_pool p, const int32_t* children) {
   const int i = blockIdx.x, t = (int)blockIdx.y - 1;
-  const i32x4 x = reinterpret_cast<const i32x4*>(p.scratch + ((p.num_rows + 3) & -4))[i];
-  if (x[1] == 0) return;
+  const Plan plan(p);
+  const i32x4 x = plan.pair[i];
+  if (x[1] == 0 || (t >= 0 && x[2] < 0)) return;
+  const int page = x[2] >= 0 ? free_page(plan, x[2]) : -1;
+  if (x[2] >= 0 && page < 0) {   // no page was left: the child stays empty
+    if (t < 0 && threadIdx.x == 0) flag(p.status, NS_KV_STATUS_NO_PAGES);
+    return;
+  }
   if (t >= 0) {
-    if (x[2] < 0) return;
     const uint64_t base = p.tensors[2 * t], stride = p.tensors[2 * t + 1];
-    copy_bytes(reinterpret_cast<char*>(base + x[2] * stride), reinterpret_cast<const char*>(base + x[3] * stride),
+    copy_bytes(reinterpret_cast<char*>(base + page * stride), reinterpret_cast<const char*>(base + x[3] * stride),
                (int64_t)(x[1] % p.block_size) * p.slot_bytes);
     return;
   }
   const int32_t* from = p.block_tables + (int64_t)x[0] * p.stride_bt_row;
   int32_t* to = p.block_tables + (int64_t)children[i] * p.stride_bt_row;
-  const int last = x[2] >= 0 ? x[1] / p.block_size : -1;
+  const int last = page >= 0 ? x[1] / p.block_size : -1;
   const int cols = held_cols(p, x[1]);
   for (int j = threadIdx.x; j < cols; j += kCopy) {
     if (j == last) {
-      to[j] = x[2];
+      to[j] = page;
+      p.page_refs[page] = 1;
       continue;
     }
     int e = from[j];
@@ -487,6 +590,7 @@ __global__ __launch_bounds__(kCopy) void fork_kernel(ns_kv_pool p, const int32_t
     to[j] = e;
     if (e >= 0) atomicAdd(p.page_refs + e, 1);
   }
+  if (threadIdx.x == 0) p.seq_lens[children[i]] = x[1];
 }
 
 // A workgroup a listed row: its entries in [first, last) of its columns become -1, their pages' counts fall.  An entry
@@ -506,12 +610,23 @@ __global__ __launch_bounds__(kCopy) void drop_kernel(ns_kv_pool p, const int32_t
     last = gone > 0 ? min((int64_t)last, gone / p.block_size) : 0;
   }
   int32_t* bt = p.block_tables + (int64_t)row * p.stride_bt_row;
-  for (int j = first + threadIdx.x; j < last; j += kCopy) {
-    if (bt[j] < 0) continue;
-    const int e = atomicExch(bt + j, -1);
-    if (e < 0) continue;
-    if (e >= p.num_pages) flag(p.status, NS_KV_STATUS_BAD_PAGE);
-    else atomicSub(p.page_refs + e, 1);
+  // eight columns a thread at a time: their reads, then the exchanges, then the counts
+  for (int j0 = first + threadIdx.x; j0 < last; j0 += 8 * kCopy) {
+    int e[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int j = j0 + u * kCopy;
+      e[u] = j < last ? bt[j] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (e[u] >= 0) e[u] = atomicExch(bt + j0 + u * kCopy, -1);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (e[u] < 0) continue;
+      if (e[u] >= p.num_pages) flag(p.status, NS_KV_STATUS_BAD_PAGE);
+      else atomicSub(p.page_refs + e[u], 1);
+    }
   }
   if (ALL) {
     __syncthreads();
@@ -535,7 +650,7 @@ __global__ __launch_bounds__(kCopy) void copy_kernel(ns_kv_pool p, const uint64_
 // as many, and one ascending scan lists both: list[0 .. h-1] holes, list[h .. 2h-1] movers.  head[0]: moves, or all
 // pages in use with `to`; -1: `to` is too small.
 __global__ __launch_bounds__(kPlan) void compact_plan_kernel(ns_kv_pool p, int32_t* to_refs, int to_pages, int32_t* map) {
-  int32_t* head = p.scratch + ((p.num_rows + 3) & -4);
+  int32_t* head = p.scratch;
   int32_t* list = head + 4;
   const int tid = threadIdx.x;
   int mine = 0;
@@ -550,9 +665,17 @@ __global__ __launch_bounds__(kPlan) void compact_plan_kernel(ns_kv_pool p, int32
     for (int i = tid; i < p.num_pages; i += kPlan) map[i] = -1;
     return;
   }
-  const int both = scan_pages(p.page_refs, p.num_pages, p.num_pages,
-                              [m](int page, int refs) { return (page < m) == (refs == 0); },
-                              [&](int page, int r) { list[r] = page; });
+  // 16 groups at a time, each a wave's
+  int both = 0;
+  for (int64_t c0 = 0; c0 < p.num_pages; c0 += kPlanWaves * kGroup) {
+    const int64_t p0 = c0 + 16 * tid;
+    const uint32_t bits =
+        pages_with(p.page_refs, p.num_pages, p0, [m](int page, int refs) { return (page < m) == (refs == 0); });
+    int all;
+    int r = both + block_prefix(__popc(bits), &all);
+    for (uint32_t left = bits; left != 0u; left &= left - 1u) list[r++] = (int)p0 + __ffs(left) - 1;
+    both += all;
+  }
   const int h = both / 2;
   for (int i = tid; i < p.num_pages; i += kPlan) map[i] = i < m && p.page_refs[i] != 0 ? i : -1;
   if (to_refs != nullptr)
@@ -576,7 +699,7 @@ __global__ __launch_bounds__(kPlan) void compact_plan_kernel(ns_kv_pool p, int32
 
 // The first num_rows workgroups rewrite a table row each; the others take (page, tensor) pieces in turn.
 __global__ __launch_bounds__(kCopy) void compact_kernel(ns_kv_pool p, ns_kv_pool to, const int32_t* map, int into) {
-  const int32_t* head = p.scratch + ((p.num_rows + 3) & -4);
+  const int32_t* head = p.scratch;
   const int32_t* list = head + 4;
   const int h = head[0];
   if (h < 0) return;
@@ -637,13 +760,13 @@ void launch_store_d(const ns_kv_store_args& a, hipStream_t stream) {
   else launch_store<T, 128>(a, stream);
 }
 
-uint64_t scratch_bytes(int32_t num_rows, int32_t num_pages) {
-  // the claims, then a fork's plan or a compaction's head and list
-  const uint64_t rows = ((uint64_t)num_rows + 3) & ~3ull;
-  const uint64_t plan = 4ull * (num_rows < NS_KV_MAX_ROWS ? num_rows : NS_KV_MAX_ROWS);
-  const uint64_t list = 4ull + (uint64_t)num_pages;
-  return 4ull * (rows + (plan > list ? plan : list));
+uint64_t scratch_bytes(int32_t num_pages) {
+  // a plan, or a compaction's head and list
+  const uint64_t plan = plan_ints(num_pages), list = 4ull + (uint64_t)num_pages;
+  return 4ull * (plan > list ? plan : list);
 }
+
+int plan_groups(int32_t num_pages) { return 1 + (int)(((int64_t)num_pages + kPlanWaves * kGroup - 1) / (kPlanWaves * kGroup)); }
 
 int check_pool(const ns_kv_pool* p) {
   if (!p) return fail("pool is NULL");
@@ -657,8 +780,8 @@ int check_pool(const ns_kv_pool* p) {
   if (p->slot_bytes < 16 || p->slot_bytes % 16 != 0) return fail("slot_bytes must be a positive multiple of 16 (got %lld)", (long long)p->slot_bytes);
   if ((uintptr_t)p->page_refs % 16 != 0 || (uintptr_t)p->scratch % 16 != 0)
     return fail("page_refs and scratch must be 16-byte aligned");
-  if (p->scratch_bytes < scratch_bytes(p->num_rows, p->num_pages))
-    return fail("scratch of %llu bytes needed (got %llu)", (unsigned long long)scratch_bytes(p->num_rows, p->num_pages),
+  if (p->scratch_bytes < scratch_bytes(p->num_pages))
+    return fail("scratch of %llu bytes needed (got %llu)", (unsigned long long)scratch_bytes(p->num_pages),
                 (unsigned long long)p->scratch_bytes);
   return 0;
 }
@@ -721,25 +844,27 @@ int ns_kv_store(const ns_kv_store_args* a, hipStream_t stream) {
   return launched();
 }
 
-int ns_kv_scratch_bytes(int32_t num_rows, int32_t num_pages, uint64_t* bytes) {
+int ns_kv_scratch_bytes(int32_t num_pages, uint64_t* bytes) {
   if (!bytes) return fail("bytes is NULL");
-  if (num_rows < 1 || num_pages < 1) return fail("a pool needs rows and pages (got %d, %d)", num_rows, num_pages);
-  *bytes = scratch_bytes(num_rows, num_pages);
+  if (num_pages < 1) return fail("a pool needs pages (got %d)", num_pages);
+  *bytes = scratch_bytes(num_pages);
   return 0;
 }
 
 int ns_kv_extend(const ns_kv_pool* p, const int32_t* rows, const int32_t* lens, int32_t n, hipStream_t stream) {
-  if (check_list(p, rows, lens, n, NS_KV_MAX_ROWS)) return 1;
+  if (check_list(p, rows, lens, n, kMaxRows)) return 1;
   if ((int64_t)n * p->num_cols >= ((int64_t)1 << 31)) return fail("rows times columns must lie below 2^31");
   if (n == 0) return 0;
-  hipLaunchKernelGGL(extend_kernel, dim3(1), dim3(kPlan), 0, stream, *p, rows, lens, n);
+  hipLaunchKernelGGL(extend_plan_kernel, dim3(plan_groups(p->num_pages)), dim3(kPlan), 0, stream, *p, rows, lens, n);
+  const int64_t groups = ((int64_t)p->num_pages + kGroup - 1) / kGroup;
+  hipLaunchKernelGGL(extend_kernel, dim3((unsigned)((groups + kCopy / 64 - 1) / (kCopy / 64))), dim3(kCopy), 0, stream, *p, n);
   return launched();
 }
 
 int ns_kv_fork(const ns_kv_pool* p, const int32_t* parents, const int32_t* children, int32_t n, hipStream_t stream) {
-  if (check_list(p, parents, children, n, p && p->num_rows < NS_KV_MAX_ROWS ? p->num_rows : NS_KV_MAX_ROWS)) return 1;
+  if (check_list(p, parents, children, n, kMaxRows)) return 1;
   if (n == 0) return 0;
-  hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPlan), 0, stream, *p, parents, children, n);
+  hipLaunchKernelGGL(fork_plan_kernel, dim3(plan_groups(p->num_pages)), dim3(kPlan), 0, stream, *p, parents, children, n);
   hipLaunchKernelGGL(fork_kernel, dim3(n, p->num_tensors + 1), dim3(kCopy), 0, stream, *p, children);
   return launched();
 }

@@ -31,7 +31,7 @@ ABI_VERSION = 1
 NS_KV_DTYPE_F32 = 0
 NS_KV_DTYPE_BF16 = 1
 NS_KV_DTYPE_F16 = 2
-MAX_ROWS = 8192           # rows of one extend or fork call (NS_KV_MAX_ROWS)
+MAX_ROWS = 4096           # rows of one extend or fork call (NS_KV_MAX_ROWS)
 STATUS_BAD_PAGE = 1
 STATUS_NO_PAGES = 2
 STATUS_BAD_ROW = 4
@@ -89,7 +89,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     p, i, pool = ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(NsKvPool)
     for name, args in (("ns_kv_abi_version", []), ("ns_kv_last_error", []),
                        ("ns_kv_store", [ctypes.c_char_p, p]),
-                       ("ns_kv_scratch_bytes", [i, i, ctypes.POINTER(ctypes.c_uint64)]),
+                       ("ns_kv_scratch_bytes", [i, ctypes.POINTER(ctypes.c_uint64)]),
                        ("ns_kv_extend", [pool, p, p, i, p]), ("ns_kv_fork", [pool, p, p, i, p]),
                        ("ns_kv_free", [pool, p, i, p]), ("ns_kv_release", [pool, p, i, i, i, p]),
                        ("ns_kv_copy", [pool, pool, p, p, i, p]), ("ns_kv_compact", [pool, pool, p, p])):
@@ -290,13 +290,13 @@ class PagePool:
             raise KvCacheError("PagePool needs device tensors")
         self._lib = load()
         need = ctypes.c_uint64(0)
-        _check(self._lib.ns_kv_scratch_bytes(block_tables.shape[0], pages, ctypes.byref(need)))
+        _check(self._lib.ns_kv_scratch_bytes(pages, ctypes.byref(need)))
         self.k_caches, self.v_caches = list(k_caches), list(v_caches)
         self.block_tables, self.seq_lens, self.page_refs = block_tables, seq_lens, page_refs
         self.device, self.block_size, self.num_pages = dev, bs, pages
         self._dev = first.get_device()
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._scratch = torch.zeros(int(need.value), dtype=torch.uint8, device=dev)
+        self._scratch = torch.empty(int(need.value), dtype=torch.uint8, device=dev)
         self._tensors = torch.tensor([[c.data_ptr(), c.stride(0) * c.element_size()] for c in caches],
                                      dtype=torch.int64, device=dev)
         self._pool = NsKvPool(block_tables.data_ptr(), seq_lens.data_ptr(), page_refs.data_ptr(), self.status.data_ptr(),
@@ -343,7 +343,7 @@ class PagePool:
     def fork(self, parents, children, stream=None) -> None:
         """Row ``children[i]``, an empty one, becomes a copy of row ``parents[i]``: full pages are shared, the tokens
         of a last page that is not full are copied, in every layer, to a page of the child's own.  A child for which
-        no page is left stays empty (NO_PAGES).  At most MAX_ROWS pairs, and no more than rows, a call."""
+        no page is left stays empty (NO_PAGES).  At most MAX_ROWS pairs a call."""
         handle, on = _on(self._dev, stream)
         with on:
             parents, children = self._two(parents, children, ("parents", "children"))

@@ -242,7 +242,6 @@ class Both:
         # the counts are those of the tables, the reserved pages' aside
         count = np.bincount(t[t >= 0], minlength=self.shape[2])
         assert np.array_equal(count[1:], self.ref.refs[1:])
-        assert torch.count_nonzero(self.pool._scratch[:4 * self.shape[0]]).item() == 0   # the claims are dropped
 
 
 @pytest.mark.parametrize("bs,pages,layers", [(16, 300, 2), (1, 700, 1), (7, 200, 3), (32, 90, 5)])

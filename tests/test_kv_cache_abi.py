@@ -129,7 +129,7 @@ def test_list_refusals_and_empty_lists():
     refused(lib.ns_kv_extend(p, 4096, None, 1, None), "NULL")
     refused(lib.ns_kv_extend(p, 4096, 4096, -1, None), "length")
     refused(lib.ns_kv_extend(p, 4096, 4096, KV.MAX_ROWS + 1, None), "at most")
-    refused(lib.ns_kv_fork(p, 4096, 4096, 5, None), "at most 4")
+    refused(lib.ns_kv_fork(p, 4096, 4096, KV.MAX_ROWS + 1, None), "at most")
     refused(lib.ns_kv_free(p, None, 3, None), "NULL")
     refused(lib.ns_kv_release(p, 4096, 1, 0, 0, None), "window")
     refused(lib.ns_kv_release(p, 4096, 1, 1, -1, None), "sinks")
@@ -147,12 +147,12 @@ def test_list_refusals_and_empty_lists():
 def test_scratch_holds_every_list():
     lib = built()
     out = ctypes.c_uint64()
-    for rows, pages in ((1, 1), (3, 5), (4096, 100), (10, 150000), (20000, 10)):
-        assert lib.ns_kv_scratch_bytes(rows, pages, ctypes.byref(out)) == 0
-        claims = (rows + 3) // 4 * 4
-        assert out.value >= 4 * (claims + 4 * min(rows, KV.MAX_ROWS))   # a fork's plan
-        assert out.value >= 4 * (claims + 4 + pages)                    # a compaction's list
-    assert lib.ns_kv_scratch_bytes(0, 5, ctypes.byref(out)) != 0
+    for pages in (1, 5, 100, 1024, 1025, 150000):
+        assert lib.ns_kv_scratch_bytes(pages, ctypes.byref(out)) == 0
+        groups = -(-pages // 1024)      # a count and 64 masks of 16 pages each
+        assert out.value >= 16 + 16 * KV.MAX_ROWS + 4 * groups + 128 * groups
+        assert out.value >= 4 * (4 + pages)               # a compaction's head and list
+    assert lib.ns_kv_scratch_bytes(0, ctypes.byref(out)) != 0
 
 
 def test_wrapper_refusals():
