@@ -1,4 +1,4 @@
-"""Build the gfx950 sampler library in-tree: csrc/*.hip -> libns_sampling.so.
+"""Build the gfx950 libraries in-tree (csrc/*.hip -> libns_*.so), and the host module (csrc/ns_host.cpp).
 
     python build.py            # from the package directory, or
     python -c "import build; build.build()"
@@ -12,6 +12,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -23,6 +24,9 @@ PA_OUT = os.path.join(HERE, "libns_paged_attention.so")
 # the paged KV cache: the store of new rows and the pages (include/ns_kv_cache.h)
 KV_SRC = os.path.join(HERE, "csrc", "ns_kv_cache.hip")
 KV_OUT = os.path.join(HERE, "libns_kv_cache.so")
+# the host side of the attention's and the cache's calls, a Python module over torch's C++ interface
+HOST_SRC = os.path.join(HERE, "csrc", "ns_host.cpp")
+HOST_OUT = os.path.join(HERE, "_ns_host.so")
 # the benchmark's bandwidth reference (not part of the sampler's ABI)
 PROBE_SRC = os.path.join(HERE, "csrc", "ns_probe.hip")
 PROBE_OUT = os.path.join(HERE, "libns_probe.so")
@@ -51,13 +55,29 @@ def _command(src: str, out: str, defines=()) -> list:
     ]
 
 
+def _host_command(src: str, out: str) -> list:
+    import torch
+    from torch.utils import cpp_extension
+
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    return [
+        "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+        "-I", os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"],
+        *[x for d in (*cpp_extension.include_paths(), os.path.join(rocm, "include")) for x in ("-isystem", d)],
+        src, "-o", out + ".tmp", "-L", os.path.join(os.path.dirname(torch.__file__), "lib"),
+        "-ltorch_python", "-ltorch_cpu", "-lc10",
+    ]
+
+
 def build(verbose: bool = False) -> str:
-    """Compile every library, the hipcc processes side by side."""
-    jobs = [(SRC, OUT, ()), (PA_SRC, PA_OUT, ()), (KV_SRC, KV_OUT, ()), (PROBE_SRC, PROBE_OUT, ()),
-            (SRC, STAMPS_OUT, ("NS_PHASE_STAMPS",))]
+    """Compile every library, the compilers side by side."""
+    jobs = [(out, _command(src, out, defines)) for src, out, defines in
+            ((SRC, OUT, ()), (PA_SRC, PA_OUT, ()), (KV_SRC, KV_OUT, ()), (PROBE_SRC, PROBE_OUT, ()),
+             (SRC, STAMPS_OUT, ("NS_PHASE_STAMPS",)))]
+    jobs.append((HOST_OUT, _host_command(HOST_SRC, HOST_OUT)))
     procs = []
-    for src, out, defines in jobs:
-        cmd = _command(src, out, defines)
+    for out, cmd in jobs:
         if verbose:
             print(" ".join(cmd), flush=True)
         procs.append((out, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
@@ -70,7 +90,7 @@ def build(verbose: bool = False) -> str:
         else:
             os.replace(out + ".tmp", out)
     if failed:
-        raise RuntimeError(f"hipcc failed for {', '.join(failed)}")
+        raise RuntimeError(f"compiling failed for {', '.join(failed)}")
     return OUT
 
 

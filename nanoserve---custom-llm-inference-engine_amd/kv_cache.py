@@ -19,10 +19,11 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
-import struct
 from typing import Optional
 
 import torch
+
+from .paged_attention import host_module
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libns_kv_cache.so")
@@ -71,16 +72,13 @@ class NsKvPool(ctypes.Structure):
                 + [(n, ctypes.c_int32) for n in ("num_rows", "num_cols", "num_pages", "num_tensors", "block_size")])
 
 
-# NsKvStoreArgs as packed bytes: a third of the time that filling the structure takes
-_STORE = struct.Struct("@12P15q9i")
-_STORE_PAD = bytes(ctypes.sizeof(NsKvStoreArgs) - _STORE.size)
-
 _LIB: Optional[ctypes.CDLL] = None
+_STORE = None    # the host module's function, and the addresses of the library's that it calls
 
 
 def load(path: str = LIB_PATH) -> ctypes.CDLL:
     """Load the HIP library (raises when it is not built: there is no fallback)."""
-    global _LIB
+    global _LIB, _STORE
     if _LIB is not None:
         return _LIB
     if not os.path.exists(path):
@@ -88,7 +86,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib = ctypes.CDLL(path)
     p, i, pool = ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(NsKvPool)
     for name, args in (("ns_kv_abi_version", []), ("ns_kv_last_error", []),
-                       ("ns_kv_store", [ctypes.c_char_p, p]),
+                       ("ns_kv_store", [ctypes.POINTER(NsKvStoreArgs), p]),
                        ("ns_kv_scratch_bytes", [i, ctypes.POINTER(ctypes.c_uint64)]),
                        ("ns_kv_extend", [pool, p, p, i, p]), ("ns_kv_fork", [pool, p, p, i, p]),
                        ("ns_kv_free", [pool, p, i, p]), ("ns_kv_release", [pool, p, i, i, i, p]),
@@ -98,6 +96,9 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.ns_kv_last_error.restype = ctypes.c_char_p
     if lib.ns_kv_abi_version() != ABI_VERSION:
         raise KvCacheError(f"ABI {lib.ns_kv_abi_version()} in {path}, expected {ABI_VERSION}")
+    host = host_module(KvCacheError)
+    host.set_errors(None, KvCacheError)
+    _STORE = (host.store, *(ctypes.cast(f, p).value for f in (lib.ns_kv_store, lib.ns_kv_last_error)))
     _LIB = lib
     return lib
 
@@ -151,94 +152,20 @@ def store_kv_hip(key, value, k_cache, v_cache, block_tables, seq_lens, query_sta
     STATUS_BAD_PAGE is ORed into when a token has no valid page (its row is then not stored).  ``stream``: a
     ``torch.cuda.Stream`` or a raw handle, default the current stream.
     """
-    lib = _LIB or load()
-    shape, pages, dtype, dev = key.shape, k_cache.shape, k_cache.dtype, k_cache.get_device()
-    ks, vs, kc, vc = key.stride(), value.stride(), k_cache.stride(), v_cache.stride()
-    # one pass over what has to hold; a call that fails it is looked at again for its message
-    if not (len(shape) == 3 and value.shape == shape and len(pages) == 4 and v_cache.shape == pages
-            and pages[2:] == shape[1:] and pages[1] == block_size and dtype in _DTYPES and key.dtype is dtype
-            and value.dtype is dtype and v_cache.dtype is dtype and key.get_device() == dev
-            and value.get_device() == dev and v_cache.get_device() == dev and ks[2] == vs[2] == kc[3] == vc[3] == 1):
-        _refuse_store(key, value, k_cache, v_cache, block_size)
-    total, hkv, d = shape
-    if status is not None and (status.dtype is not torch.int32 or status.get_device() != dev or status.numel() < 1):
-        raise KvCacheError("status must be an int32 device tensor")
-    if block_tables.dim() != 2:
-        raise KvCacheError("block_tables must have two dimensions")
-    num_seqs, cols = block_tables.shape
-    if seq_lens.numel() != num_seqs or query_lens.numel() != num_seqs or query_start_loc.numel() != num_seqs + 1:
-        raise KvCacheError("seq_lens/query_lens need num_seqs entries and query_start_loc num_seqs + 1")
-    if inv_freq is not None and (inv_freq.dtype is not torch.float32 or inv_freq.shape != (d // 2,)
-                                 or inv_freq.get_device() != dev or not inv_freq.is_contiguous()):
-        raise KvCacheError(f"inv_freq must be a contiguous float32 tensor of {d // 2} elements on the cache's device")
-    hq = q_at = out_at = qs0 = qs1 = os0 = os1 = 0
-    if query is not None:
-        if inv_freq is None:
-            raise KvCacheError("a query is there to be rotated: it needs inv_freq")
-        q_shape = query.shape
-        if len(q_shape) != 3 or q_shape[0] != total or q_shape[2] != d:
-            raise KvCacheError(f"query {tuple(q_shape)} does not match the keys' {tuple(shape)}")
-        _row_tensor("query", query, dtype, dev)
-        hq = q_shape[1]
-        if out is not None:
-            if out.shape != q_shape:
-                raise KvCacheError("out must match query's shape")
-            _row_tensor("out", out, dtype, dev)
-    elif out is not None:
-        raise KvCacheError("out is where the rotated query goes: it needs query")
+    if _STORE is None:
+        load()
+    store, entry, why = _STORE
+    dev = k_cache.get_device()
     if dev < 0:
-        raise KvCacheError("store_kv_hip needs device tensors")
-    handle, on = _on(dev, stream)
-    if on is not _NO_SWITCH:
-        with on:
-            return store_kv_hip(key, value, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
-                                block_size, query=query, inv_freq=inv_freq, out=out, status=status)
-    if query is not None:
-        if out is None:
-            out = torch.empty_like(query)
-            if out.stride(2) != 1 and total:
-                out = torch.empty(q_shape, dtype=dtype, device=query.device)
-        q_at, out_at = query.data_ptr(), out.data_ptr()
-        (qs0, qs1, _), (os0, os1, _) = query.stride(), out.stride()
-    if total == 0:
-        return out
-    if block_tables.dtype is not torch.int32 or block_tables.get_device() != dev or block_tables.stride(1) != 1:
-        block_tables = _i32(block_tables, k_cache.device, "block_tables")
-    sl, qsl, ql = seq_lens, query_start_loc, query_lens
-    if not (sl.dtype is qsl.dtype is ql.dtype is torch.int32 and sl.get_device() == qsl.get_device() == ql.get_device()
-            == dev and sl.is_contiguous() and qsl.is_contiguous() and ql.is_contiguous()):
-        sl, qsl, ql = (_i32(t, k_cache.device, n) for t, n in ((sl, "seq_lens"), (qsl, "query_start_loc"),
-                                                               (ql, "query_lens")))
-    _check(lib.ns_kv_store(_STORE.pack(
-        q_at, key.data_ptr(), value.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out_at,
-        0 if inv_freq is None else inv_freq.data_ptr(), block_tables.data_ptr(), sl.data_ptr(), qsl.data_ptr(),
-        ql.data_ptr(), 0 if status is None else status.data_ptr(),
-        qs0, qs1, ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], os0, os1,
-        block_tables.stride(0), total, num_seqs, hq, hkv, d, block_size, pages[0], cols, _DTYPES[dtype]) + _STORE_PAD,
-        handle))
-    return out
-
-
-def _row_tensor(name, t, dtype, dev):
-    if t.dtype is not dtype or t.get_device() != dev:
-        raise KvCacheError(f"{name} must share the cache's dtype and device")
-    if t.stride(-1) != 1:
-        raise KvCacheError(f"{name} must have a unit head_dim stride")
-
-
-def _refuse_store(key, value, k_cache, v_cache, block_size):
-    """Why the rows and caches of a store do not fit one another."""
-    if key.dim() != 3 or key.shape != value.shape or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
-        raise KvCacheError(f"key {tuple(key.shape)} and value {tuple(value.shape)} must match, and k_cache "
-                           f"{tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)}")
-    if k_cache.shape[2:] != key.shape[1:]:
-        raise KvCacheError(f"the caches' rows {tuple(k_cache.shape[2:])} are not the keys' {tuple(key.shape[1:])}")
-    if k_cache.shape[1] != block_size:
-        raise KvCacheError(f"block_size {block_size} != the cache's {k_cache.shape[1]}")
-    if k_cache.dtype not in _DTYPES:
-        raise KvCacheError(f"unsupported dtype {k_cache.dtype} (float32, bfloat16, float16)")
-    for name, t in (("key", key), ("value", value), ("k_cache", k_cache), ("v_cache", v_cache)):
-        _row_tensor(name, t, k_cache.dtype, k_cache.get_device())
+        handle, on = -1, _NO_SWITCH      # checked, and refused
+    elif stream is None and dev == torch.cuda.current_device():
+        return store(entry, why, key, value, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
+                     block_size, query, inv_freq, out, status, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        handle, on = _on(dev, stream)
+    with on:
+        return store(entry, why, key, value, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
+                     block_size, query, inv_freq, out, status, handle)
 
 
 class PagePool:

@@ -26,8 +26,8 @@ can be released (``kv_cache.PagePool.release``).
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
-import struct
 from typing import Optional
 
 import numpy as np
@@ -99,10 +99,17 @@ class NsPagedAttnArgs(ctypes.Structure):
     ]
 
 
-# NsPagedAttnArgs as packed bytes: a third of the time that filling the structure takes
-_ARGS = struct.Struct("@10PQP11q10if4xPi4xPi4x")
-
 _LIB: Optional[ctypes.CDLL] = None
+_ATTEND = None    # the host module's function, and the addresses of the library's that it calls
+
+
+def host_module(error):
+    """The compiled host side of the attention's and the cache store's calls (csrc/ns_host.cpp)."""
+    import torch  # noqa: F401  (its libraries are the module's)
+
+    if not os.path.exists(os.path.join(HERE, "_ns_host.so")):
+        raise error(f"{os.path.join(HERE, '_ns_host.so')} is not built (run __graft_entry__.build())")
+    return importlib.import_module("._ns_host", __package__)
 
 
 def load(path: str = LIB_PATH) -> ctypes.CDLL:
@@ -120,19 +127,32 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.ns_paged_attention_workspace_bytes.restype = ctypes.c_int
     lib.ns_paged_attention_workspace_bytes.argtypes = [ctypes.c_int32] * 5 + [ctypes.POINTER(ctypes.c_uint64)]
     lib.ns_paged_attention_call_workspace.restype = ctypes.c_int
-    # the arguments: an NsPagedAttnArgs by reference, or its bytes
-    lib.ns_paged_attention_call_workspace.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+    lib.ns_paged_attention_call_workspace.argtypes = [ctypes.POINTER(NsPagedAttnArgs),
+                                                      ctypes.POINTER(ctypes.c_uint64),
+                                                      ctypes.POINTER(ctypes.c_uint64)]
     lib.ns_paged_attention.restype = ctypes.c_int
-    lib.ns_paged_attention.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    lib.ns_paged_attention.argtypes = [ctypes.POINTER(NsPagedAttnArgs), ctypes.c_void_p]
     lib.ns_paged_attention_windowed_workspace.restype = ctypes.c_int
-    lib.ns_paged_attention_windowed_workspace.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
-                                                          ctypes.c_void_p, ctypes.c_void_p]
+    lib.ns_paged_attention_windowed_workspace.argtypes = [ctypes.POINTER(NsPagedAttnArgs), ctypes.c_int32,
+                                                          ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64),
+                                                          ctypes.POINTER(ctypes.c_uint64)]
     lib.ns_paged_attention_windowed.restype = ctypes.c_int
-    lib.ns_paged_attention_windowed.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
+    lib.ns_paged_attention_windowed.argtypes = [ctypes.POINTER(NsPagedAttnArgs), ctypes.c_int32, ctypes.c_int32,
+                                                ctypes.c_void_p]
     if lib.ns_pa_abi_version() != ABI_VERSION:
         raise PagedAttentionError(f"ABI {lib.ns_pa_abi_version()} in {path}, expected {ABI_VERSION}")
     _LIB = lib
     return lib
+
+
+def load_host() -> None:
+    """The library and the host module that calls it."""
+    global _ATTEND
+    lib, host = load(), host_module(PagedAttentionError)
+    host.set_errors(PagedAttentionError, None)
+    _ATTEND = (host.attend, *(ctypes.cast(f, ctypes.c_void_p).value for f in (
+        lib.ns_paged_attention_call_workspace, lib.ns_paged_attention, lib.ns_paged_attention_windowed_workspace,
+        lib.ns_paged_attention_windowed, lib.ns_pa_last_error)))
 
 
 def _check(rc: int) -> None:
@@ -220,26 +240,6 @@ class PagedAttentionPlan:
             self.tiles = (self.staged.data_ptr() + 4 * int(h_tokens.size), int(h_tiles.shape[0]))
 
 
-def _dtype_code(dtype) -> int:
-    import torch
-
-    if dtype is torch.bfloat16:
-        return NS_PA_DTYPE_BF16
-    if dtype is torch.float16:
-        return NS_PA_DTYPE_F16
-    if dtype is torch.float32:
-        return NS_PA_DTYPE_F32
-    raise PagedAttentionError(f"unsupported dtype {dtype} (float32, bfloat16, float16)")
-
-
-def _i32(t, device):
-    import torch
-
-    if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
-        return t
-    return t.to(device=device, dtype=torch.int32).contiguous()
-
-
 def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
                         scale: float, block_size: int, *, max_seq_len: Optional[int] = None,
                         max_query_len: Optional[int] = None, plan: Optional[PagedAttentionPlan] = None,
@@ -267,7 +267,8 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
     """
     import torch
 
-    lib = _LIB or load()
+    if _ATTEND is None:
+        load_host()
     if window is not None and not 1 <= window < 2 ** 31:
         raise PagedAttentionError(f"window must be at least 1 and below 2^31 (got {window})")
     if not 0 <= sinks < 2 ** 31:
@@ -277,7 +278,7 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
         raise PagedAttentionError("paged_attention_hip needs device tensors")
     if stream is None:
         if index == torch.cuda.current_device():   # already where the call goes: no stream to switch to and back
-            return _paged_attention_on(lib, index, torch._C._cuda_getCurrentRawStream(index), query, k_cache, v_cache,
+            return _paged_attention_on(index, torch._C._cuda_getCurrentRawStream(index), query, k_cache, v_cache,
                                        block_tables, seq_lens, query_start_loc, query_lens, scale, block_size,
                                        max_seq_len, max_query_len, plan, window, sinks, out, workspace, counters, status)
         s = torch.cuda.current_stream(query.device)
@@ -291,109 +292,50 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
     else:
         s = torch.cuda.ExternalStream(int(stream), device=query.device)
     with torch.cuda.stream(s):
-        return _paged_attention_on(lib, index, s.cuda_stream, query, k_cache, v_cache, block_tables, seq_lens,
+        return _paged_attention_on(index, s.cuda_stream, query, k_cache, v_cache, block_tables, seq_lens,
                                    query_start_loc, query_lens, scale, block_size, max_seq_len, max_query_len, plan,
                                    window, sinks, out, workspace, counters, status)
 
 
-def _paged_attention_on(lib, index, handle, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
+def _paged_attention_on(index, handle, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
                         scale, block_size, max_seq_len, max_query_len, plan, window, sinks, out, workspace, counters,
                         status):
-    """paged_attention_hip with the stream of ``handle`` the current one: every temporary below is made on it."""
+    """paged_attention_hip with the stream of ``handle`` the current one: every temporary is made on it."""
     import torch
 
-    total_q, hq, d = q_shape = query.shape
-    nb, bs, hkv, dk = k_shape = k_cache.shape
-    dtype = query.dtype
-    if v_cache.shape != k_shape or dk != d:
-        raise PagedAttentionError(f"cache shapes {tuple(k_cache.shape)}, {tuple(v_cache.shape)} do not match "
-                                  f"the query's head_dim {d}")
-    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
-        raise PagedAttentionError("query and caches must share one dtype")
-    if bs != block_size:
-        raise PagedAttentionError(f"block_size {block_size} != the cache's {bs}")
-    if not k_cache.get_device() == v_cache.get_device() == index:
-        raise PagedAttentionError("query and caches must be on one device")
-    if total_q == 0:  # nothing to attend (an empty tensor's strides are arbitrary)
-        return torch.empty_like(query) if out is None else out
-    q_stride, k_stride, v_stride = query.stride(), k_cache.stride(), v_cache.stride()
-    if not q_stride[-1] == k_stride[-1] == v_stride[-1] == 1:
-        name = "query" if q_stride[-1] != 1 else "k_cache" if k_stride[-1] != 1 else "v_cache"
-        raise PagedAttentionError(f"{name} must have a unit head_dim stride")
-    bt, sl, qsl, ql = block_tables, seq_lens, query_start_loc, query_lens
-    i32 = torch.int32
-    if not (bt.dtype is sl.dtype is qsl.dtype is ql.dtype is i32 and bt.get_device() == sl.get_device()
-            == qsl.get_device() == ql.get_device() == index and bt.is_contiguous() and sl.is_contiguous()
-            and qsl.is_contiguous() and ql.is_contiguous()):
-        dev = query.device
-        bt, sl, qsl, ql = _i32(bt, dev), _i32(sl, dev), _i32(qsl, dev), _i32(ql, dev)
-    bt_shape = bt.shape
-    num_seqs = bt_shape[0]
-    if sl.numel() != num_seqs or ql.numel() != num_seqs or qsl.numel() != num_seqs + 1:
-        raise PagedAttentionError("seq_lens/query_lens need num_seqs entries and query_start_loc num_seqs + 1")
-    # prefill tiles: 16-bit types, unless the caller declares a decode step
-    tiles = None
-    tokens = tiles_at = n_tokens = n_tiles = 0
+    attend, *entries = _ATTEND
+    tokens = tiles = (0, 0)
+    made = plan is None and query.dtype is not torch.float32 and (max_query_len is None
+                                                                  or max_query_len >= PREFILL_MIN_QUERY)
+    if made or plan is None and max_seq_len is None:
+        # the batch layout is read on the host, once the call is known to be in order
+        attend(*entries, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens, scale, block_size,
+               0, 0, 0, 0, 0, 0, 0, out, workspace, counters, status, False, -1)
+        if query.shape[0] > 0 and made:
+            plan = PagedAttentionPlan(seq_lens, query_start_loc, query_lens, query.shape[1], k_cache.shape[2],
+                                      query.device)
+        elif max_seq_len is None:
+            max_seq_len = int(seq_lens.max().item()) if seq_lens.numel() else 0
     if plan is not None:
         # (a padded batch's rows behind the plan's are left alone with a window)
-        if plan.total_q > total_q or (window is None and plan.total_q < total_q) or plan.num_heads_q != hq \
-                or plan.num_kv_heads != hkv:
+        total_q = query.shape[0]
+        if not made and total_q > 0 and (plan.total_q > total_q or (window is None and plan.total_q < total_q)
+                                         or plan.num_heads_q != query.shape[1] or plan.num_kv_heads != k_cache.shape[2]):
             raise PagedAttentionError("the plan was made for another batch layout or head layout")
         if max_seq_len is None:
             max_seq_len = plan.max_seq_len
-    elif dtype is not torch.float32 and (max_query_len is None or max_query_len >= PREFILL_MIN_QUERY):
-        plan = PagedAttentionPlan(sl, qsl, ql, hq, hkv, query.device)   # one read of the batch layout
-        if max_seq_len is None:
-            max_seq_len = plan.max_seq_len
-    if plan is not None and plan.tiles is not None and dtype is not torch.float32:
-        (tokens, n_tokens), (tiles_at, n_tiles) = plan.tokens, plan.tiles
-        tiles = plan.tiles
-    if max_seq_len is None:
-        max_seq_len = int(sl.max().item()) if num_seqs else 0
-    if out is None:
-        out = torch.empty_like(query)
-    elif out.shape != q_shape or out.dtype is not dtype or out.get_device() != index:
-        raise PagedAttentionError("out must match query's shape, dtype and device")
-    o_stride = out.stride()
-    if o_stride[-1] != 1:
-        raise PagedAttentionError("out must have a unit head_dim stride")
-    if status is not None and (status.dtype is not i32 or status.get_device() != index or status.numel() < 1):
-        raise PagedAttentionError("status must be an int32 device tensor")
-    at = (query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), bt.data_ptr(), sl.data_ptr(),
-          qsl.data_ptr(), ql.data_ptr(), 0 if status is None else status.data_ptr())
-    rest = (q_stride[0], q_stride[1], k_stride[0], k_stride[1], k_stride[2],
-            v_stride[0], v_stride[1], v_stride[2], o_stride[0], o_stride[1],
-            bt_shape[1] if len(bt_shape) == 2 else 0,   # contiguous
-            total_q, num_seqs, hq, hkv, d, bs, nb, bt_shape[1] if len(bt_shape) == 2 else 0, max_seq_len,
-            _dtype_code(dtype), scale, tokens, n_tokens, tiles_at, n_tiles)
-    args = _ARGS.pack(*at, 0, 0, 0, *rest)
-    sizes = (ctypes.c_uint64 * 2)()
-    second = ctypes.addressof(sizes) + 8
-    if window is None:
-        _check(lib.ns_paged_attention_call_workspace(args, sizes, second))
-    else:
-        _check(lib.ns_paged_attention_windowed_workspace(args, window, sinks, sizes, second))
-    need, ncount = sizes
-    if need:
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=query.device)
-        elif workspace.numel() * workspace.element_size() < need:
-            raise PagedAttentionError(
-                f"workspace of {need} bytes needed, {workspace.numel() * workspace.element_size()} given (total_q "
-                f"{total_q}, max_seq_len {max_seq_len}, {n_tokens if tiles is not None else total_q} "
-                f"per-token queries, {n_tiles} prefill tiles)")
-        if counters is None:
-            counters = _COUNTERS.get((index, handle))
-            if counters is None or counters.numel() < ncount:
-                counters = counters_for(query.device, ncount)
-        elif counters.dtype is not i32 or counters.get_device() != index or counters.numel() < ncount:
-            raise PagedAttentionError(f"counters must be an int32 device tensor of at least {ncount} entries")
-        args = _ARGS.pack(*at, workspace.data_ptr(), need, counters.data_ptr(), *rest)
-    if window is None:
-        _check(lib.ns_paged_attention(args, handle))
-    else:
-        _check(lib.ns_paged_attention_windowed(args, window, sinks, handle))
-    return out
+        if plan.tiles is not None and query.dtype is not torch.float32:
+            tokens, tiles = plan.tokens, plan.tiles
+    own = counters is None
+    if own:
+        counters = _COUNTERS.get((index, handle))
+    while True:
+        got = attend(*entries, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens, scale,
+                     block_size, max_seq_len, tokens[0], tokens[1], tiles[0], tiles[1], window or 0, sinks, out,
+                     workspace, counters, status, own, handle)
+        if type(got) is not int:
+            return got
+        counters = counters_for(query.device, got)
 
 
 # the reference's name, so that nanoserve/model/attention.py:21 can import this module unchanged
