@@ -1109,6 +1109,7 @@ struct PfParams {
   float scale_log2;       // |scale| * log2(e); 1 for a scale of 0
   uint32_t q_and, q_xor;  // applied to the query words: a negative scale flips their signs, a zero scale clears them
   int32_t out_vec;        // output rows 8-byte aligned: four elements a store
+  int32_t parts;          // with a window: workgroups that share a (tile, KV head)'s steps
 };
 
 struct PfTile {
@@ -1158,91 +1159,11 @@ __device__ __forceinline__ f32x2 ld_dev2(const float* p) {
   return f32x2{__uint_as_float((uint32_t)w), __uint_as_float((uint32_t)(w >> 32))};
 }
 
-// One query column of a tile by one wave in float arithmetic, one position after the other, each lane D / 64 dims:
-// what the windowed kernel falls back to for a column whose output is not finite.
-template <typename T, int D>
-__device__ __forceinline__ void plain_column(const PaParams& p, const PfTile& t, int c, int G, int kvh, int lane) {
-  using M = Mma<T>;
-  constexpr int E = D / 64;
-  const int tok = c / G;
-  if (tok >= t.nq) return;
-  const int h = kvh * G + c % G, d0 = lane * E;
-  auto element = [](const void* base, int64_t at) -> float {
-    return M::lo(reinterpret_cast<const uint16_t*>(base)[at]);
-  };
-  float q[E], o[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    q[i] = element(p.q, (int64_t)(t.t0 + tok) * p.sq_tok + (int64_t)h * p.sq_head + d0 + i) * p.scale_log2;
-    o[i] = 0.f;
-  }
-  const int n = min(t.kv_pos0 + tok + 1 - t.hole.gap, t.lt);
-  const int h1 = t.hole.h1 + tok;
-  const int32_t* bt_row = p.bt + (int64_t)t.seq * p.sbt;
-  float m = -INFINITY, l = 0.f;
-  for (int v = 0; v < n; ++v) {
-    if (v >= p.sinks && v < h1) {
-      v = h1 - 1;
-      continue;
-    }
-    const int j = t.hole.position(v);
-    const int bi = j / p.block_size, off = j - bi * p.block_size;
-    const int blk = bi < p.max_blocks_per_seq ? bt_row[bi] : -1;
-    if (blk < 0 || blk >= p.num_blocks) continue;
-    const int64_t at = (int64_t)blk * p.sk_blk + (int64_t)off * p.sk_tok + (int64_t)kvh * p.sk_head + d0;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) s = fmaf(q[i], element(p.k, at + i), s);
-    s = wave_sum(s);
-    const float mn = fmaxf(m, s);
-    const float alpha = mn == -INFINITY ? 0.f : exp2f(m - mn), w = mn == -INFINITY ? 0.f : exp2f(s - mn);
-    m = mn;
-    l = fmaf(l, alpha, w);
-    const int64_t vt = (int64_t)blk * p.sv_blk + (int64_t)off * p.sv_tok + (int64_t)kvh * p.sv_head + d0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = fmaf(w, element(p.v, vt + i), alpha == 1.f ? o[i] : o[i] * alpha);
-  }
-#pragma unroll
-  for (int i = 0; i < E; ++i)
-    store_one<T>(p.out, (int64_t)(t.t0 + tok) * p.so_tok + (int64_t)h * p.so_head + d0 + i, l > 0.f ? o[i] / l : 0.f);
-}
-
-// The columns whose written outputs are not finite, of the tiles that a workgroup finished in its run u0 .. u1 of steps
-// from step `off` of (tile, kvh) on, again in float arithmetic.  An infinite or NaN value makes NaN of the zero weight
-// that a token of the tile has which does not see it, and of the two parts of one that does where infinity is right.
-template <typename T, int D, int G>
-__device__ __forceinline__ void redo_columns(const PaParams& p, const PfParams& f, int tile, int kvh, int off, int64_t u0,
-                                             int64_t u1, int ended) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  __builtin_amdgcn_s_waitcnt(0);   // the wave's own stores are out
-  for (int64_t u = u0; u < u1; off = 0, ++tile) {
-    if (tile == f.n_tiles) {
-      tile = 0;
-      ++kvh;
-    }
-    const PfTile t = pf_tile<true>(p, f, tile, kPfCols / G);
-    if (t.steps == 0) continue;
-    const int take = (int)(u1 - u < t.steps - off ? u1 - u : t.steps - off);
-    u += take;
-    if (take < t.steps && !(ended & (off > 0 ? 1 : 2))) continue;   // cut, and merged by another
-    for (int c = 32 * wave; c < 32 * wave + 32 && c / G < t.nq; ++c) {
-      const uint16_t* out = reinterpret_cast<const uint16_t*>(p.out) + (int64_t)(t.t0 + c / G) * p.so_tok +
-                            (int64_t)(kvh * G + c % G) * p.so_head;
-      bool odd = false;
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i)
-        odd |= !(fabsf(Mma<T>::lo(__hip_atomic_load(out + lane + 64 * i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))) <
-                 INFINITY);
-      if (__ballot(odd) != 0ull) plain_column<T, D>(p, t, c, G, kvh, lane);
-    }
-  }
-}
-
 // BW: the block size is a power of two and at least the consecutive positions one load instruction
 // of a wave covers (4 at 128 dims, 8 at 64), so these never straddle two blocks: the block is the
 // wave's, and a row's address a scalar address plus a lane's fixed offset instead of 64-bit products
 // per lane (four 512-token chunks up to 8192 positions: 257 -> 228 us).
-template <typename T, int D, int G, bool BW, bool WIN>
+template <typename T, int D, int G, bool BW>
 __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void pa_prefill_kernel(PaParams p,
                                                                                                         PfParams f) {
   using M = Mma<T>;
@@ -1263,9 +1184,6 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
   __shared__ int s_place[2];   // the workgroup's first tile and its step in it
   __shared__ int s_bad;        // an invalid block met in this segment
   __shared__ int s_last;
-  // with a window: an output that is not finite was written; the run's first tile, its KV head and its step in it;
-  // which of the run's cut tiles this workgroup merged (1: one begun by another, 2: one that it began)
-  __shared__ int s_odd, s_run[3], s_ended;
 
   const int wave = threadIdx.x >> 6;
   const int n_tiles = f.n_tiles;
@@ -1282,7 +1200,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     const int first = tid * q;
     int64_t mine = 0;
     for (int i = first; i < first + q && i < n_tiles; ++i) {
-      const PfTile t = pf_tile<WIN>(p, f, i, BQ);
+      const PfTile t = pf_tile<false>(p, f, i, BQ);
       mine += t.steps;
       if (blockIdx.x == 0 && p.status) {
         if (t.steps == 0) atomicOr(p.status, NS_PA_STATUS_BAD_TILE);
@@ -1316,7 +1234,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
       int64_t at = rem - pre;
       int i = first;
       for (;; ++i) {   // the thread's steps hold `at`: one of its tiles does
-        const int n = pf_tile<WIN>(p, f, i, BQ).steps;
+        const int n = pf_tile<false>(p, f, i, BQ).steps;
         if (at < n) break;
         at -= n;
       }
@@ -1329,7 +1247,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
   } else {
     tile = blockIdx.x % n_tiles;
     kvh = blockIdx.x / n_tiles;
-    const PfTile t = pf_tile<WIN>(p, f, tile, BQ);
+    const PfTile t = pf_tile<false>(p, f, tile, BQ);
     if (threadIdx.x == 0 && kvh == 0 && p.status) {
       if (t.steps == 0) atomicOr(p.status, NS_PA_STATUS_BAD_TILE);
       if (t.cut) atomicOr(p.status, NS_PA_STATUS_SEQ_TOO_LONG);
@@ -1344,19 +1262,12 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
   const int wv = __builtin_amdgcn_readfirstlane(wave);
   const float scale = f.scale_log2;
 
-  if (WIN && threadIdx.x == 0) {   // written again only behind the barriers of a tile's steps
-    s_odd = s_ended = 0;
-    s_run[0] = tile;
-    s_run[1] = kvh;
-    s_run[2] = off;
-  }
-  if constexpr (WIN) __syncthreads();
   for (int64_t u = u0; u < u1;) {
     if (tile == n_tiles) {
       tile = 0;
       ++kvh;
     }
-    const PfTile t = pf_tile<WIN>(p, f, tile, BQ);
+    const PfTile t = pf_tile<false>(p, f, tile, BQ);
     if (t.steps == 0) {   // not a tile of this batch: no units
       ++tile;
       continue;
@@ -1388,8 +1299,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     // visible positions of the lane's column (-1: a padding column, never written)
     int kvl = -1;
     if (c < BQ * G && tok < t.nq) {
-      const int seen = t.kv_pos0 + tok + 1 - (WIN ? t.hole.gap : 0);
-      const int kl = seen < t.lt ? seen : t.lt;
+      const int kl = t.kv_pos0 + tok + 1 < t.lt ? t.kv_pos0 + tok + 1 : t.lt;
       kvl = kl > 0 ? kl : 0;
     }
     const bool live = __ballot(kvl >= 0) != 0ull;   // a wave of padding columns only loads rows
@@ -1401,13 +1311,6 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     int kend_w = kvl >= 0 ? kend : INT32_MAX;
 #pragma unroll
     for (int sh = 1; sh < 64; sh <<= 1) kend_w = min(kend_w, __shfl_xor(kend_w, sh));
-    // with a window, positions from sinks on are hidden too: those below h1_t from every token of the tile, those below
-    // h1_w from some token of the wave, those below kvl - window from the column
-    int h1_t = 0, h1_w = 0;
-    if constexpr (WIN) {
-      h1_t = t.hole.h1;
-      h1_w = h1_t + min((wv * 32 + 31) / G, t.nq - 1);
-    }
     const int32_t* bt_row = p.bt + (int64_t)t.seq * p.sbt;
     const char* kbase = reinterpret_cast<const char*>(p.k) + (int64_t)kvh * p.sk_head * 2;
     const char* vbase = reinterpret_cast<const char*>(p.v) + (int64_t)kvh * p.sv_head * 2;
@@ -1430,7 +1333,6 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     // step ahead of the rows, the rows one step ahead of the products.  Chunk r of the thread is
     // position (tid + kPfThreads r) / CPP of a step.
     auto split = [&](int j, int& o) -> int {
-      if constexpr (WIN) j = t.hole.position(j);
       int bi;
       if (BW || p.bs_shift >= 0) { bi = j >> p.bs_shift; o = j & (p.block_size - 1); }
       else { bi = j / p.block_size; o = j - bi * p.block_size; }
@@ -1451,18 +1353,16 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     };
     auto load_rows = [&](int jt) {
       bad_rows = 0u;
-      [[maybe_unused]] bool loud = false;   // one of them is not merely hidden by the window
 #pragma unroll
       for (int r = 0; r < LPT; ++r) {
         int o;
-        [[maybe_unused]] const int bi = split(BW ? group_of(jt, r) : min(jt + (tid + kPfThreads * r) / CPP, j1 - 1), o);
+        split(BW ? group_of(jt, r) : min(jt + (tid + kPfThreads * r) / CPP, j1 - 1), o);
         int b = BW ? __builtin_amdgcn_readfirstlane(blk[r]) : blk[r];
         // an invalid entry of the segment (past its end, its last one again): block 0 stands in, the
         // rows are not used
         const bool bad = (uint32_t)b >= (uint32_t)p.num_blocks;
         b = bad ? 0 : b;
         bad_rows |= bad ? 1u << r : 0u;
-        if (WIN && bad && !hidden_block(p, bi, t.kv_pos0)) loud = true;
         if constexpr (BW) {   // block strides below 2^31: one 32 x 32 bit product each
           kreg[r] = *reinterpret_cast<const u32x4*>(
               kbase + ((uint64_t)(uint32_t)b * (uint32_t)p.sk_blk + (uint32_t)(o * sk_tok)) * 2 + koff);
@@ -1473,7 +1373,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
           vreg[r] = *reinterpret_cast<const u32x4*>(vbase + ((int64_t)b * p.sv_blk + o * sv_tok) * 2 + 16 * dc0);
         }
       }
-      if (WIN ? loud : bad_rows != 0u) {
+      if (bad_rows != 0u) {
         s_bad = 1;
         if (p.status) atomicOr(p.status, NS_PA_STATUS_BAD_BLOCK);
       }
@@ -1483,13 +1383,6 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
 #pragma unroll
         for (int r = 0; r < LPT; ++r)
           if (((bad_rows >> r) & 1u) || jt + (tid + kPfThreads * r) / CPP >= j1) vreg[r] = u32x4{0u, 0u, 0u, 0u};
-      }
-      if (WIN && jt < h1_t && jt + kPfPos > p.sinks) {   // nor of a row that every token of the tile has hidden
-#pragma unroll
-        for (int r = 0; r < LPT; ++r) {
-          const int j = jt + (tid + kPfThreads * r) / CPP;
-          if (j >= p.sinks && j < h1_t) vreg[r] = u32x4{0u, 0u, 0u, 0u};
-        }
       }
 #pragma unroll
       for (int r = 0; r < LPT; ++r) {
@@ -1544,30 +1437,15 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
         // the online softmax of the lane's column over the step's 64 positions (element e of block
         // rb: position 32 rb + 8 (e / 4) + 4 h + e % 4; the other half in lane ^ 32)
         const bool bad = s_bad != 0;
-        const bool behind = WIN && jt < h1_w && jt + kPfPos > p.sinks;   // some of it behind a window
-        if (jt + kPfPos > kend_w || bad || behind) {   // a position of the step hidden from a column
-          [[maybe_unused]] const uint32_t hlen = (uint32_t)max(kvl - p.window - p.sinks, 0);
+        if (jt + kPfPos > kend_w || bad) {   // a position of the step hidden from a column
 #pragma unroll
           for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const int r = 32 * rb + 8 * (e >> 2) + 4 * h + (e & 3);
               st[rb][e] = jt + r < kend ? st[rb][e] : -INFINITY;
-              if constexpr (WIN) st[rb][e] = (uint32_t)(jt - p.sinks + r) >= hlen ? st[rb][e] : -INFINITY;
             }
-          if constexpr (WIN) {
-            if (bad) {   // look the step's blocks up again, a position a lane
-              int o;
-              const int bi = split(min(jt + lane, j1 - 1), o);
-              const int b = bi < p.max_blocks_per_seq ? bt_row[bi] : -1;
-              const uint64_t gone = __ballot((uint32_t)b >= (uint32_t)p.num_blocks) >> (4 * h);
-#pragma unroll
-              for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                  if ((uint32_t)(gone >> (32 * rb + 8 * (e >> 2) + (e & 3))) & 1u) st[rb][e] = -INFINITY;
-            }
-          } else if (bad) {   // look the step's blocks up again
+          if (bad) {   // look the step's blocks up again
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
@@ -1658,14 +1536,6 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
             for (int i = 0; i < 4; ++i) store_one<T>(p.out, d + i, x[i]);
           }
         }
-      if constexpr (WIN) {
-        float z = 0.f;   // NaN with an output that is not finite
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) z = fmaf(o[db][e], 0.f, z);
-        if (z != 0.f) s_odd = 1;
-      }
     };
     if (take == t.steps) {
       write_out(acc, l);
@@ -1696,7 +1566,6 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
       if (tid == 0) s_last = atomicAdd(counter, 1) == arrivals - 1;
       __syncthreads();
       if (s_last) {
-        if (WIN && tid == 0) s_ended |= w == wa ? 2 : 1;
         if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (live) {
           float mx = -INFINITY;
@@ -1711,27 +1580,16 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
             const int64_t slot = __builtin_amdgcn_readfirstlane(i == wa ? begin_slot : i);
             const float* src = f.ws_acc + (slot * kPfWaves + wv) * SW + 2 * lane;
             const f32x2 ml = ld_dev2(f.ws_ml + (slot * kPfCols + c) * 2);
-            // a segment's loads are issued before the first is used (with a window, half of them at a time: all
-            // at once need one register more than there is at 128 dims)
-            constexpr int NA = D / (WIN ? 8 : 4);
-            f32x2 a[NA];
+            f32x2 a[D / 4];   // all of a segment's loads issued before the first is used
 #pragma unroll
-            for (int e = 0; e < NA; ++e) a[e] = ld_dev2(src + e * 128);
+            for (int e = 0; e < D / 4; ++e) a[e] = ld_dev2(src + e * 128);
             // a segment whose keys were all skipped (m = -inf) weighs 0
             const float wt = ml[0] == -INFINITY ? 0.f : exp2f(ml[0] - mx);
             L = fmaf(wt, ml[1], L);
 #pragma unroll
-            for (int e0 = 0; e0 < D / 4; e0 += NA) {
-              if (e0 > 0) {
-#pragma unroll
-                for (int e = 0; e < NA; ++e) a[e] = ld_dev2(src + (e0 + e) * 128);
-              }
-#pragma unroll
-              for (int e1 = 0; e1 < NA; ++e1) {
-                const int e = e0 + e1;
-                acc[e / 8][2 * (e % 8)] = fmaf(wt, a[e1][0], acc[e / 8][2 * (e % 8)]);
-                acc[e / 8][2 * (e % 8) + 1] = fmaf(wt, a[e1][1], acc[e / 8][2 * (e % 8) + 1]);
-              }
+            for (int e = 0; e < D / 4; ++e) {
+              acc[e / 8][2 * (e % 8)] = fmaf(wt, a[e][0], acc[e / 8][2 * (e % 8)]);
+              acc[e / 8][2 * (e % 8) + 1] = fmaf(wt, a[e][1], acc[e / 8][2 * (e % 8) + 1]);
             }
           }
           write_out(acc, L);
@@ -1742,17 +1600,13 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2
     off = 0;
     ++tile;
   }
-  if constexpr (WIN) {
-    __syncthreads();
-    if (__builtin_expect(s_odd != 0, 0)) {
-      // The arguments are read anew, hidden from the compiler, which would hold them in registers throughout.
-      uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
-      asm volatile("" : "+s"(args));
-      const PaParams pa = *reinterpret_cast<const PaParams*>(args);
-      redo_columns<T, D, G>(pa, f, s_run[0], s_run[1], s_run[2], u0, u1, s_ended);
-    }
-  }
 }
+
+}  // namespace
+
+#include "ns_pa_window.h"
+
+namespace {
 
 // ---- host side ---------------------------------------------------------------------------------
 
@@ -1791,6 +1645,34 @@ uint64_t pf_workspace_bytes(int32_t n_tiles, int32_t hkv, int32_t head_dim, int3
   if (grid == 0) return 0;
   const int64_t th = (int64_t)n_tiles * hkv;
   return (uint64_t)(grid + (grid < th ? grid : th)) * kPfCols * (head_dim + 2) * sizeof(float);
+}
+
+// The workgroups that share a (tile, KV head) of a windowed call, so that few tiles still fill the GPU.  The cost of a
+// count is estimated for the busiest CU, in tenths of a microsecond at 128 dims: its workgroups run two at a time, 2.8 us
+// for a step of both, 1.8 for one alone; each has some 2.5 us around its steps, and parts cost 4 and more to merge.  More
+// parts have to gain a twentieth.  Measured (24 / 8 heads of 128 dims, bf16; 1, 2, 3, 4 parts): one 512-token chunk at
+// window 2048 74, 48, 52, 44 us (4 are taken), two of them 74, 66, 74, 73 (2), three 103, 95, 89, 91 (3), four
+// 112, 116, 112, 119 (1), ten at window 1024 138, 163, 180, 206 (1); one of 17 tokens at window 4096 121 by itself, 35 in
+// eight parts.
+int pw_parts_for(int32_t n_tiles, int32_t hkv, int32_t tile_len) {
+  const int64_t pairs = (int64_t)n_tiles * hkv, steps = ((int64_t)tile_len + kPfPos - 1) / kPfPos;
+  int64_t best = 0;
+  int parts = 1;
+  for (int k = 1; k <= 16 && k <= steps; ++k) {
+    const int64_t w = (pairs * k + 255) / 256;   // workgroups of the busiest CU
+    if (k > 1 && w > 16) break;
+    const int64_t cost = (w / 2 * 28 + w % 2 * 18) * ((steps + k - 1) / k) + 25 * w + (k > 1 ? 40 + 5 * k : 0);
+    if (k == 1 || cost * 20 < best * 19) {
+      best = cost;
+      parts = k;
+    }
+  }
+  return parts;
+}
+// Bytes of their partials.
+uint64_t pw_workspace_bytes(int32_t n_tiles, int32_t hkv, int32_t head_dim, int32_t tile_len) {
+  const int64_t parts = pw_parts_for(n_tiles, hkv, tile_len);
+  return parts <= 1 ? 0 : (uint64_t)n_tiles * hkv * parts * kPfCols * (head_dim + 2) * sizeof(float);
 }
 
 int part_tokens_for(int32_t total_q, int32_t hkv, int32_t max_seq_len) {
@@ -1846,8 +1728,13 @@ void launch(const PaParams& p, const PfParams& f, int n_tokens, int n_tiles, hip
       else hipLaunchKernelGGL((pa_decode_kernel<T, D, G, false, WIN>), grid, dim3(kThreads), 0, stream, p);
     }
     if (n_tiles > 0) {
-      if (by_wave) hipLaunchKernelGGL((pa_prefill_kernel<T, D, G, true, WIN>), tiles, dim3(kPfThreads), 0, stream, p, f);
-      else hipLaunchKernelGGL((pa_prefill_kernel<T, D, G, false, WIN>), tiles, dim3(kPfThreads), 0, stream, p, f);
+      if constexpr (WIN) {
+        hipLaunchKernelGGL((pa_window_kernel<T, D, G>), dim3((unsigned)(n_tiles * p.hkv * f.parts)), dim3(kPfThreads), 0,
+                           stream, p, f);
+      } else {
+        if (by_wave) hipLaunchKernelGGL((pa_prefill_kernel<T, D, G, true>), tiles, dim3(kPfThreads), 0, stream, p, f);
+        else hipLaunchKernelGGL((pa_prefill_kernel<T, D, G, false>), tiles, dim3(kPfThreads), 0, stream, p, f);
+      }
     }
   }
 }
@@ -1904,7 +1791,8 @@ Sizes sizes_of(const ns_paged_attn_args* a, int32_t window, int32_t sinks) {
   z.token_len = walked(a->max_seq_len, window, sinks, 1);
   z.tile_len = walked(a->max_seq_len, window, sinks, kPfCols / (a->num_heads_q / a->num_kv_heads));
   z.token_bytes = workspace_bytes(a->total_q, a->num_heads_q, a->num_kv_heads, a->head_dim, z.token_len, z.n_tokens);
-  z.tile_bytes = pf_workspace_bytes(z.n_tiles, a->num_kv_heads, a->head_dim, z.tile_len);
+  z.tile_bytes = window > 0 ? pw_workspace_bytes(z.n_tiles, a->num_kv_heads, a->head_dim, z.tile_len)
+                            : pf_workspace_bytes(z.n_tiles, a->num_kv_heads, a->head_dim, z.tile_len);
   return z;
 }
 
@@ -2013,6 +1901,7 @@ int attend(const ns_paged_attn_args* a, int32_t window, int32_t sinks, hipStream
   char* ws = reinterpret_cast<char*>(a->workspace);
   f.grid = pf_grid_for(n_tiles, a->num_kv_heads, z.tile_len);
   if (((uintptr_t)a->workspace + need) % 8 != 0) f.grid = 0;   // the partials go in 8-byte pieces
+  f.parts = pf_need > 0 && ((uintptr_t)a->workspace + need) % 8 == 0 ? pw_parts_for(n_tiles, a->num_kv_heads, z.tile_len) : 1;
   f.n_tiles = n_tiles;
   f.ws_acc = pf_need ? reinterpret_cast<float*>(ws + need) : nullptr;
   f.ws_ml = pf_need ? f.ws_acc + pf_need / sizeof(float) / (a->head_dim + 2) * a->head_dim : nullptr;
