@@ -284,7 +284,8 @@ def kernel_source_hash():
 
     h = hashlib.sha256()
     for name in sorted(os.listdir(CSRC)):
-        if name.endswith((".hip", ".h")) and name not in ("ns_probe.hip", "ns_paged_attention.hip"):
+        if name.endswith((".hip", ".h")) and name not in (
+                "ns_probe.hip", "ns_paged_attention.hip", "ns_pa_window.h", "ns_kv_cache.hip"):
             with open(os.path.join(CSRC, name), "rb") as f:
                 h.update(name.encode() + b"\0" + f.read())
     return h.hexdigest()[:16]

@@ -4,10 +4,13 @@
 // come in as addresses.
 
 #include <Python.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 
+#include <exception>
 #include <string>
+#include <utility>
 
 #include "ns_kv_cache.h"
 #include "ns_paged_attention.h"
@@ -66,10 +69,8 @@ PyObject* guarded(PyObject* error, Body body) {
     return body();
   } catch (const Refused& r) {
     if (!PyErr_Occurred()) PyErr_SetString(error != nullptr ? error : PyExc_RuntimeError, r.why.c_str());
-  } catch (const c10::Error& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
-  } catch (const std::exception& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {   // torch's own, out of memory among them
+    if (!PyErr_Occurred()) torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }
@@ -80,6 +81,8 @@ bool arguments(Py_ssize_t got, Py_ssize_t want) {
   return false;
 }
 
+// The library's functions come as addresses (ctypes has them), the stream as its handle.
+//
 // store(ns_kv_store, ns_kv_last_error, key, value, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
 //       block_size, query, inv_freq, out, status, stream handle or -1) -> out, or None
 // With a handle of -1 the arguments are only checked.

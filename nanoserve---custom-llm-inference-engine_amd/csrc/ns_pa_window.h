@@ -12,7 +12,7 @@
 //     products of these, in an order that the compiler is held to: left to itself it waits for each read before its
 //     product.
 //   * Rows that no token of the tile sees are zeroed on their way to LDS, and a column whose output is not finite is
-//     computed again in float arithmetic (redo_columns): a weight of 0 times an infinite or NaN value that only other
+//     computed again in float arithmetic (plain_column): a weight of 0 times an infinite or NaN value that only other
 //     tokens of the tile see must not reach it.
 #pragma once
 
@@ -20,72 +20,72 @@ namespace {
 
 constexpr int kAheadK = 4, kAheadV = 2;   // LDS reads ahead of their products
 
-// One query column of a tile by one wave in float arithmetic, one position after the other, each lane D / 64 dims:
-// what the windowed kernel falls back to for a column whose output is not finite.
+// One query column of a tile by one wave in float arithmetic, 64 positions at a time: a lane a position for the scores,
+// D / 64 dims a lane for the values.  What the windowed kernel falls back to for a column whose output is not finite
+// though its sum is.
 template <typename T, int D>
 __device__ __forceinline__ void plain_column(const PaParams& p, const PfTile& t, int c, int G, int kvh, int lane) {
   using M = Mma<T>;
   constexpr int E = D / 64;
-  const int tok = c / G;
-  if (tok >= t.nq) return;
-  const int h = kvh * G + c % G, d0 = lane * E;
+  const int tok = c / G, h = kvh * G + c % G;
   auto element = [](const void* base, int64_t at) -> float {
     return M::lo(reinterpret_cast<const uint16_t*>(base)[at]);
   };
-  float q[E], o[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    q[i] = element(p.q, (int64_t)(t.t0 + tok) * p.sq_tok + (int64_t)h * p.sq_head + d0 + i) * p.scale_log2;
-    o[i] = 0.f;
-  }
-  const int n = min(t.kv_pos0 + tok + 1 - t.hole.gap, t.lt);
-  const int h1 = t.hole.h1 + tok;
+  const int64_t q0 = (int64_t)(t.t0 + tok) * p.sq_tok + (int64_t)h * p.sq_head;
+  const int n = min(t.kv_pos0 + tok + 1 - t.hole.gap, t.lt), h1 = t.hole.h1 + tok;
   const int32_t* bt_row = p.bt + (int64_t)t.seq * p.sbt;
-  float m = -INFINITY, l = 0.f;
-  for (int v = 0; v < n; ++v) {
-    if (v >= p.sinks && v < h1) {
-      v = h1 - 1;
-      continue;
-    }
-    const int j = t.hole.position(v);
-    const int bi = j / p.block_size, off = j - bi * p.block_size;
-    const int blk = bi < p.max_blocks_per_seq ? bt_row[bi] : -1;
-    if (blk < 0 || blk >= p.num_blocks) continue;
-    const int64_t at = (int64_t)blk * p.sk_blk + (int64_t)off * p.sk_tok + (int64_t)kvh * p.sk_head + d0;
-    float s = 0.f;
+  float o[E], m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) s = fmaf(q[i], element(p.k, at + i), s);
-    s = wave_sum(s);
-    const float mn = fmaxf(m, s);
+  for (int i = 0; i < E; ++i) o[i] = 0.f;
+  for (int v0 = 0; v0 < n; v0 += 64) {
+    if (v0 >= p.sinks && v0 + 64 <= h1) continue;   // hidden
+    const int v = v0 + lane, j = t.hole.position(min(v, n - 1));
+    const int bi = j / p.block_size, off = j - bi * p.block_size;
+    int blk = v < n && (v < p.sinks || v >= h1) && bi < p.max_blocks_per_seq ? bt_row[bi] : -1;
+    if (blk >= p.num_blocks) blk = -1;
+    const uint64_t seen = __ballot(blk >= 0);
+    const int64_t krow = (int64_t)max(blk, 0) * p.sk_blk + (int64_t)off * p.sk_tok + (int64_t)kvh * p.sk_head;
+    const int64_t vrow = (int64_t)max(blk, 0) * p.sv_blk + (int64_t)off * p.sv_tok + (int64_t)kvh * p.sv_head;
+    float s = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < D; d += 8) {
+      const u32x4 a = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.q) + q0 + d);
+      const u32x4 b = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.k) + krow + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s = fmaf(M::lo(a[i]) * p.scale_log2, M::lo(b[i]), s);
+        s = fmaf(M::hi(a[i]) * p.scale_log2, M::hi(b[i]), s);
+      }
+    }
+    if (blk < 0) s = -INFINITY;
+    const float mn = fmaxf(m, wave_max(s));
     const float alpha = mn == -INFINITY ? 0.f : exp2f(m - mn), w = mn == -INFINITY ? 0.f : exp2f(s - mn);
     m = mn;
-    l = fmaf(l, alpha, w);
-    const int64_t vt = (int64_t)blk * p.sv_blk + (int64_t)off * p.sv_tok + (int64_t)kvh * p.sv_head + d0;
+    l = fmaf(l, alpha, wave_sum(w));
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = fmaf(w, element(p.v, vt + i), alpha == 1.f ? o[i] : o[i] * alpha);
+    for (int i = 0; i < E; ++i) o[i] = alpha == 1.f ? o[i] : o[i] * alpha;
+    for (int k0 = 0; k0 < 64; k0 += 16) {   // sixteen rows' loads together
+      float x[16][E];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const uint64_t row = (uint32_t)__builtin_amdgcn_readlane((int)vrow, k0 + k) |
+                             (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(vrow >> 32), k0 + k) << 32;
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[k][i] = element(p.v, (int64_t)row + lane * E + i);
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if ((seen >> (k0 + k)) & 1ull) {
+          const float wk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), k0 + k));
+#pragma unroll
+          for (int i = 0; i < E; ++i) o[i] = fmaf(wk, x[k][i], o[i]);
+        }
+    }
   }
 #pragma unroll
   for (int i = 0; i < E; ++i)
-    store_one<T>(p.out, (int64_t)(t.t0 + tok) * p.so_tok + (int64_t)h * p.so_head + d0 + i, l > 0.f ? o[i] / l : 0.f);
-}
-
-// The wave's columns whose written outputs are not finite, again in float arithmetic.  An infinite or NaN value makes NaN
-// of the zero weight that a token of the tile has which does not see it, and of the two parts of one that does where
-// infinity is right.
-template <typename T, int D, int G>
-__device__ __forceinline__ void redo_columns(const PaParams& p, const PfTile& t, int kvh) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  __builtin_amdgcn_s_waitcnt(0);   // the wave's own stores are out
-  for (int c = 32 * wave; c < 32 * wave + 32 && c / G < t.nq; ++c) {
-    const uint16_t* out = reinterpret_cast<const uint16_t*>(p.out) + (int64_t)(t.t0 + c / G) * p.so_tok +
-                          (int64_t)(kvh * G + c % G) * p.so_head;
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i)
-      odd |= !(fabsf(Mma<T>::lo(__hip_atomic_load(out + lane + 64 * i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))) <
-               INFINITY);
-    if (__ballot(odd) != 0ull) plain_column<T, D>(p, t, c, G, kvh, lane);
-  }
+    store_one<T>(p.out, (int64_t)(t.t0 + tok) * p.so_tok + (int64_t)h * p.so_head + lane * E + i,
+                 quotient<true>(o[i], l));
 }
 
 template <typename T, int D, int G>
@@ -103,18 +103,14 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(D ==
   __shared__ __align__(16) unsigned char s_k[2][kPfPos * PK];
   __shared__ __align__(16) unsigned char s_v[2][kPfPos * PV];
   __shared__ int s_last;
-  __shared__ int s_odd;   // an output that is not finite was written
 
   // consecutive workgroups, which run on different XCDs, take a tile's KV heads
   const int kvh = (int)(blockIdx.x % p.hkv), tile = (int)(blockIdx.x / p.hkv % f.n_tiles);
   const int part = (int)(blockIdx.x / p.hkv / f.n_tiles);
   const PfTile t = pf_tile<true>(p, f, tile, BQ);
-  if (threadIdx.x == 0) {
-    s_odd = 0;
-    if (kvh == 0 && part == 0 && p.status) {
-      if (t.steps == 0) atomicOr(p.status, NS_PA_STATUS_BAD_TILE);
-      if (t.cut) atomicOr(p.status, NS_PA_STATUS_SEQ_TOO_LONG);
-    }
+  if (threadIdx.x == 0 && kvh == 0 && part == 0 && p.status) {
+    if (t.steps == 0) atomicOr(p.status, NS_PA_STATUS_BAD_TILE);
+    if (t.cut) atomicOr(p.status, NS_PA_STATUS_SEQ_TOO_LONG);
   }
   // steps of a part: those of a tile shared evenly, none for some parts of a tile of few steps
   auto first_step = [&](int i) -> int { return (int)((int64_t)t.steps * i / f.parts); };
@@ -123,6 +119,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(D ==
 
   const float scale = f.scale_log2;
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  uint64_t todo = 0ull;   // lanes whose columns' outputs are not finite though their sums are
   {
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c32 = lane & 31;
     const int dc0 = lane % CPP;   // every chunk of the thread has dims 8 dc0 .. + 7
@@ -340,10 +337,10 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(D ==
     l += __shfl_xor(l, 32);   // the other half's positions
 
     // O^T layout: lane, element e -> column c, dim 32 db + 8 (e / 4) + 4 h + e % 4
-    auto write_out = [&](const f32x16_t (&o)[DB], float sum) {
-      if (kvl < 0) return;
+    auto write_out = [&](const f32x16_t (&o)[DB], float sum) -> bool {
+      if (kvl < 0) return false;
       const int64_t obase = (int64_t)(t.t0 + tok) * p.so_tok + (int64_t)(kvh * G + hd) * p.so_head + 4 * h;
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;   // no visible key: zeros
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;   // no visible key: zeros; NaN scores: NaN
       float z = 0.f;   // NaN with an output that is not finite
 #pragma unroll
       for (int db = 0; db < DB; ++db)
@@ -352,7 +349,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(D ==
           float x[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x[i] = sum > 0.f ? o[db][4 * e4 + i] * inv : 0.f;
+            x[i] = sum != 0.f ? o[db][4 * e4 + i] * inv : 0.f;
             z = fmaf(o[db][4 * e4 + i], 0.f, z);
           }
           const int64_t d = obase + 32 * db + 8 * e4;
@@ -364,10 +361,10 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(D ==
             for (int i = 0; i < 4; ++i) store_one<T>(p.out, d + i, x[i]);
           }
         }
-      if (z != 0.f) s_odd = 1;
+      return z != 0.f && sum == sum;   // with a NaN among the column's scores it all is NaN
     };
     if (take == t.steps) {
-      write_out(acc, l);
+      todo = __ballot(write_out(acc, l));
     } else {
       // a tile in parts: this one's partials to its slot, in the lanes' accumulator layout (agent-scope stores: the
       // parts' workgroups run on different XCDs)
@@ -417,17 +414,20 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(D ==
             acc[e / 8][2 * (e % 8) + 1] = fmaf(wt, x[e][1], acc[e / 8][2 * (e % 8) + 1]);
           }
         }
-        write_out(acc, L);
+        todo = __ballot(write_out(acc, L));
       }
     }
   }
-  __syncthreads();
-  if (__builtin_expect(s_odd != 0, 0)) {
-    // The arguments are read anew, hidden from the compiler, which would hold them in registers throughout.
+  if (__builtin_expect(todo != 0ull, 0)) {
+    // An infinite or NaN value makes NaN of the zero weight that a token of the tile has which does not see it, and of
+    // the two parts of one that does where infinity is right: those columns again, over the outputs just written.  (The
+    // arguments are read anew, hidden from the compiler, which would hold them in registers throughout.)
+    __builtin_amdgcn_s_waitcnt(0);
     uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(args));
     const PaParams pa = *reinterpret_cast<const PaParams*>(args);
-    redo_columns<T, D, G>(pa, t, kvh);
+    for (todo = (todo | todo >> 32) & 0xffffffffull; todo != 0ull; todo &= todo - 1ull)
+      plain_column<T, D>(pa, t, 32 * wv + __ffsll((unsigned long long)todo) - 1, G, kvh, (int)threadIdx.x & 63);
   }
 }
 

@@ -384,11 +384,23 @@ template <> struct Mma<F16> {
 
 // ---- partition kernel ---------------------------------------------------------------------------
 
+// An output from its sum o and the sum of its weights l: no visible key (l = 0) gives zeros.  With a NaN among the
+// scores l is NaN, and a windowed call's outputs are NaN (the others' are zeros).
+template <bool WIN>
+__device__ __forceinline__ float quotient(float o, float l) {
+  return (WIN ? l != 0.f : l > 0.f) ? o / l : 0.f;
+}
+// A score's weight, m the largest score, -inf where there is none but NaN.
+template <bool WIN>
+__device__ __forceinline__ float weight_of(float score, float m) {
+  return m == -INFINITY && !(WIN && score != score) ? 0.f : exp2f(score - m);
+}
+
 // The end of a partition: the sum over the waves of red(wave, head, dim), s_m and s_l the partition's
 // maximum (log2 units) and sum of weights per head.  s_w: G * kMaxMerge floats of LDS, free once red
 // has been read.  s_odd (or NULL): an LDS word, 0 so far; with a sum that is NaN, infinite or large enough
 // to overflow in the merge, redo() makes red, s_m and s_l anew and they are stored again.
-template <typename T, int D, int G, typename Red, typename Redo>
+template <typename T, int D, int G, bool WIN, typename Red, typename Redo>
 __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int kvh, int part, int n_parts, Red red,
                                                  float* s_m, float* s_l, float* s_w, int* s_odd, Redo redo) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -404,7 +416,7 @@ __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int 
       const int h = kvh * G + g;
       if (direct) {
         const float l = s_l[g];
-        store_one<T>(p.out, (int64_t)qi * p.so_tok + (int64_t)h * p.so_head + d, l > 0.f ? o / l : 0.f);
+        store_one<T>(p.out, (int64_t)qi * p.so_tok + (int64_t)h * p.so_head + d, quotient<WIN>(o, l));
       } else if (p.ws_acc && part < p.max_parts) {
         const int64_t slot_idx = ((int64_t)qi * p.hq + h) * p.max_parts + part;
         st_dev(&p.ws_acc[slot_idx * D + d], o);
@@ -482,7 +494,7 @@ __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int 
       if (i + 4 <= arrivals) add(Int<4>{});
       while (i < arrivals) add(Int<1>{});
       const float l = s_l[g];
-      store_one<T>(p.out, (int64_t)qi * p.so_tok + (int64_t)h * p.so_head + d, l > 0.f ? o / l : 0.f);
+      store_one<T>(p.out, (int64_t)qi * p.so_tok + (int64_t)h * p.so_head + d, quotient<WIN>(o, l));
     }
     return;
   }
@@ -496,7 +508,7 @@ __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int 
       const float mi = ld_dev(&p.ws_ml[(base + i) * 2]);
       const float li = ld_dev(&p.ws_ml[(base + i) * 2 + 1]);
       const float ai = ld_dev(&p.ws_acc[(base + i) * D + d]);
-      if (mi == -INFINITY) continue;  // a partition whose keys were all skipped
+      if (mi == -INFINITY && !(WIN && li != li)) continue;  // a partition whose keys were all skipped
       if (mi > m) {
         const float r = m == -INFINITY ? 0.f : exp2f(m - mi);
         l *= r;
@@ -507,7 +519,7 @@ __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int 
       l = fmaf(w, li, l);
       o = fmaf(w, ai, o);
     }
-    store_one<T>(p.out, (int64_t)qi * p.so_tok + (int64_t)h * p.so_head + d, l > 0.f ? o / l : 0.f);
+    store_one<T>(p.out, (int64_t)qi * p.so_tok + (int64_t)h * p.so_head + d, quotient<WIN>(o, l));
   }
 }
 
@@ -617,7 +629,7 @@ __global__ __launch_bounds__(kThreads) void pa_partition_kernel(PaParams p) {
     m = wave_max(m);
     float l = 0.f;
     for (int j = lane; j < n; j += 64) {
-      const float e = m == -INFINITY ? 0.f : exp2f(s_score[g * kMaxPart + j] - m);
+      const float e = weight_of<WIN>(s_score[g * kMaxPart + j], m);
       s_score[g * kMaxPart + j] = e;
       l += e;
     }
@@ -662,7 +674,7 @@ __global__ __launch_bounds__(kThreads) void pa_partition_kernel(PaParams p) {
   }
   __syncthreads();
 
-  finish_partition<float, D, G>(p, qi, kvh, part, n_parts,
+  finish_partition<float, D, G, WIN>(p, qi, kvh, part, n_parts,
                             [&](int w, int g, int d) { return s_red[(w * G + g) * D + d]; }, s_m, s_l, s_score,
                             nullptr, []() {});
 }
@@ -703,7 +715,7 @@ __device__ __forceinline__ void plain_partition(const PaParams& p, int qi, int k
     for (int j = lane; j < n; j += 64) m = fmaxf(m, s_buf[g * kMaxPart + j]);
     m = wave_max(m);
     for (int j = lane; j < n; j += 64) {
-      const float w = m == -INFINITY ? 0.f : exp2f(s_buf[g * kMaxPart + j] - m);
+      const float w = weight_of<WIN>(s_buf[g * kMaxPart + j], m);
       s_buf[g * kMaxPart + j] = w;
       l += w;
     }
@@ -1045,7 +1057,7 @@ __global__ __launch_bounds__(kThreads)
     }
   }
   __syncthreads();
-  finish_partition<T, D, G>(p, qi, kvh, part, n_parts, [&](int w, int g, int d) { return s_red[(w * G + g) * D + d]; },
+  finish_partition<T, D, G, WIN>(p, qi, kvh, part, n_parts, [&](int w, int g, int d) { return s_red[(w * G + g) * D + d]; },
                             s_m, s_l, s_red, &s_odd,
                             [&]() { plain_partition<T, D, G, WIN>(p, qi, kvh, n, blocks, s_red, s_m, s_l); });
 }

@@ -140,6 +140,50 @@ def test_values_that_only_some_tokens_of_a_tile_see(device, value, dtype, hq, hk
         assert (out[hit] == value).all() and (ref[hit] == value).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_tiles_in_parts(device, dtype):
+    """One short chunk far into a context: its tile's steps are shared by several workgroups, whose partials are merged;
+    with an infinite value in the first of them, and one in a row that the second half of the chunk alone sees."""
+    n, m, window, sinks = 6000, 20, 4000, 5
+    case = make_case(1650, [n], [m], hq=8, hkv=2, dtype=dtype)
+    ref = PA.paged_attention(**oracle_args(case), terms=True, window=window, sinks=sinks)
+    a = run(case, device, window, sinks)
+    assert_close_to_oracle(a, ref, dtype)
+    assert torch.equal(a, run(case, device, window, sinks))
+    for t, dim in ((2, 9), (n - 8, 70)):
+        case["v_cache"][int(case["block_tables"][0, t // 16]), t % 16, 1, dim] = math.inf
+    got = run(case, device, window, sinks).double().cpu().numpy()
+    hit = np.zeros(got.shape, dtype=bool)
+    hit[:, 4:, 9] = True
+    hit[m - 8:, 4:, 70] = True
+    assert (got[hit] == math.inf).all() and np.isfinite(got[~hit]).all()
+    assert_close_to_oracle(torch.from_numpy(np.where(hit, 0.0, got)).to(dtype), (np.where(hit, 0.0, ref[0]), ref[1]), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_nan_keys_and_queries_give_nan(device, dtype):
+    # a NaN among the scores makes the token's whole output NaN, and no other's; in a chunk, in one partition and in many
+    lens, qlens = [300, 200, 4000, 90], [100, 1, 1, 1]
+    case = make_case(1660, lens, qlens, dtype=dtype)
+    ref, cond = PA.paged_attention(**oracle_args(case), terms=True, window=50, sinks=2)
+    wide, wide_cond = PA.paged_attention(**oracle_args(case), terms=True, window=3000, sinks=2)
+    case["k_cache"][int(case["block_tables"][0, 270 // 16]), 270 % 16, 3, 7] = math.nan    # seen from position 270 on
+    case["k_cache"][int(case["block_tables"][2, 3990 // 16]), 3990 % 16, 0, 7] = math.nan
+    case["query"][10, 5] = math.nan
+    case["query"][101, 23] = math.nan
+    case["query"][102, 8] = math.nan
+    for window, want, terms in ((50, ref, cond), (3000, wide, wide_cond)):
+        got = run(case, device, window, 2).double().cpu().numpy()
+        hit = np.zeros(got.shape, dtype=bool)
+        hit[70:100, 9:12] = True
+        hit[10, 5] = True
+        hit[101, 23] = True
+        hit[101, 0:3] = True      # sequence 2's token: its NaN key is KV head 0's
+        hit[102, 8] = True
+        assert np.isnan(got[hit]).all()
+        assert_close_to_oracle(torch.from_numpy(np.where(hit, 0.0, got)).to(dtype), (np.where(hit, 0.0, want), terms), dtype)
+
+
 def test_rows_that_are_no_tokens_are_left_alone(device):
     # a padded batch: rows behind the last sequence, and a sequence with fewer query tokens than its place holds
     case = make_case(1700, [300, 40, 500], [1, 1, 1])
