@@ -45,6 +45,13 @@ constexpr int kMinPart = 64;
 constexpr int kMaxMerge = 1024;
 // workgroups a launch aims for before splitting stops: four per CU (the 128-dim 16-bit kernels hold three at once)
 constexpr int kTargetGroups = 1024;
+// the same for calls with a window: one per CU.  Their rows are short and all of a length, so no long row waits to be
+// balanced, and every further part costs its prologue and its share of the merge.  A target of 1024 and of 256 in us (bf16, 32 / 8
+// heads of 128 dims, replayed from a graph, rows x window): 1 x 4096 18.7, 13.7; 1 x 8192 29.3, 16.7; 2 x 4096 26.4,
+// 16.2; 4 x 4096 23.6, 19.1; 8 x 1024 18.7, 14.4; 8 x 4096 35.4, 33.4; 16 x 2048 35.8, 34.2; 32 x 1024 36.5, 33.9;
+// 1 x 1024, which does not reach 256 either, 10.3 both.  64 dims, 1 x 4096: 14.5, 10.7; 4 x 1024 11.1, 9.5; 16 x 1024
+// 15.6, 13.7; 32 x 1024 20.5, 18.0.
+constexpr int kWindowGroups = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Windows and sinks are clamped to this on the host, so that sums of the two and a position's alignment fit 32 bits.
@@ -1687,11 +1694,11 @@ uint64_t pw_workspace_bytes(int32_t n_tiles, int32_t hkv, int32_t head_dim, int3
   return parts <= 1 ? 0 : (uint64_t)n_tiles * hkv * parts * kPfCols * (head_dim + 2) * sizeof(float);
 }
 
-int part_tokens_for(int32_t total_q, int32_t hkv, int32_t max_seq_len) {
+int part_tokens_for(int32_t total_q, int32_t hkv, int32_t max_seq_len, int target = kTargetGroups) {
   int part = kMaxPart;
   while (part > kMinPart) {
     const int64_t parts = ((int64_t)max_seq_len + part - 1) / part;
-    if ((int64_t)total_q * hkv * parts >= kTargetGroups) break;
+    if ((int64_t)total_q * hkv * parts >= target) break;
     part >>= 1;
   }
   return part;
@@ -1713,14 +1720,14 @@ int check_sizes(int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim, int3
 // Bytes of the per-token kernel's partials: total_q query slots (the kernel indexes them by query
 // token), the partition length sized for the n_tokens workgroups along x.
 uint64_t workspace_bytes(int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim, int32_t max_seq_len,
-                         int32_t n_tokens) {
-  const int part = part_tokens_for(n_tokens, hkv, max_seq_len);
+                         int32_t n_tokens, int target) {
+  const int part = part_tokens_for(n_tokens, hkv, max_seq_len, target);
   const int64_t max_parts = ((int64_t)max_seq_len + part - 1) / part;
   if (max_parts <= 1) return 0;
   return (uint64_t)total_q * hq * max_parts * (head_dim + 2) * sizeof(float);
 }
 uint64_t workspace_bytes(int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim, int32_t max_seq_len) {
-  return workspace_bytes(total_q, hq, hkv, head_dim, max_seq_len, total_q);
+  return workspace_bytes(total_q, hq, hkv, head_dim, max_seq_len, total_q, kTargetGroups);
 }
 
 // n_tokens decode workgroups along x (p.tokens or the first n_tokens tokens); the prefill tiles
@@ -1794,6 +1801,7 @@ struct Sizes {
   int32_t n_tokens, n_tiles;       // workgroups along x of the per-token kernel, tiles
   int32_t token_len, tile_len;     // positions that one of them can have to walk
   uint64_t token_bytes, tile_bytes;   // of workspace
+  int target;                      // workgroups that the per-token kernel's rows are split for
 };
 
 Sizes sizes_of(const ns_paged_attn_args* a, int32_t window, int32_t sinks) {
@@ -1802,7 +1810,9 @@ Sizes sizes_of(const ns_paged_attn_args* a, int32_t window, int32_t sinks) {
   z.n_tiles = a->prefill_tiles ? a->n_prefill_tiles : 0;
   z.token_len = walked(a->max_seq_len, window, sinks, 1);
   z.tile_len = walked(a->max_seq_len, window, sinks, kPfCols / (a->num_heads_q / a->num_kv_heads));
-  z.token_bytes = workspace_bytes(a->total_q, a->num_heads_q, a->num_kv_heads, a->head_dim, z.token_len, z.n_tokens);
+  z.target = window > 0 ? kWindowGroups : kTargetGroups;
+  z.token_bytes =
+      workspace_bytes(a->total_q, a->num_heads_q, a->num_kv_heads, a->head_dim, z.token_len, z.n_tokens, z.target);
   z.tile_bytes = window > 0 ? pw_workspace_bytes(z.n_tiles, a->num_kv_heads, a->head_dim, z.tile_len)
                             : pf_workspace_bytes(z.n_tiles, a->num_kv_heads, a->head_dim, z.tile_len);
   return z;
@@ -1853,7 +1863,7 @@ int attend(const ns_paged_attn_args* a, int32_t window, int32_t sinks, hipStream
   const int32_t n_tiles = z.n_tiles, n_tokens = z.n_tokens;
   const uint64_t need = z.token_bytes, pf_need = z.tile_bytes;
   if (need > 0 && !a->counters) return fail("a call with split rows needs the zero-filled counters buffer");
-  const int part = part_tokens_for(n_tokens, a->num_kv_heads, z.token_len);
+  const int part = part_tokens_for(n_tokens, a->num_kv_heads, z.token_len, z.target);
   const int64_t max_parts = ((int64_t)z.token_len + part - 1) / part;
   if (max_parts > 65535) return fail("max_seq_len too large");
   if (need + pf_need > 0 && (!a->workspace || a->workspace_bytes < need + pf_need))

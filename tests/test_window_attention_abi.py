@@ -60,11 +60,12 @@ def test_wrapper_refusals(window, sinks, word):
 def test_workspace_follows_the_window():
     built()
     floats = 4 * 24 * (128 + 2) * 4      # a partition's partials, all rows and heads
-    # 4 rows x 8 heads of 100,000 positions: partitions of 1024; of sinks and window alone: partitions of 64
+    # 4 rows x 8 heads of 100,000 positions: partitions of 1024; of sinks and window alone:
+    # partitions of 128, the longest that give 256 workgroups
     rc, whole = workspace(args(), 2 ** 31 - 1, 0)
     assert rc == 0 and whole == floats * -(-100000 // 1024)
     rc, some = workspace(args(), 1000, 4)
-    assert rc == 0 and some == floats * -(-(16 + 1000 + 15) // 64)
+    assert rc == 0 and some == floats * -(-(16 + 1000 + 15) // 128)
     rc, none = workspace(args(), 33, 0)
     assert rc == 0 and none == 0         # one partition
     # sequences shorter than the window
