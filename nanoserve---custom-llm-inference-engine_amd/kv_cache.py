@@ -197,7 +197,11 @@ class PagePool:
                 raise KvCacheError("all caches of a pool must share shape, dtype and device")
             if not c[:1].is_contiguous():
                 raise KvCacheError("a cache's pages must be contiguous")
+            if c.shape[0] > 1 and c.stride(0) < c[0].numel():
+                raise KvCacheError("a cache's pages overlap")
         pages, bs, heads, d = first.shape
+        if block_tables.dim() != 2:
+            raise KvCacheError("block_tables must be (rows, columns) with contiguous rows")
         dev, slot = first.device, heads * d * first.element_size()
         if min(pages, bs) < 1 or slot < 16 or slot % 16 != 0:
             raise KvCacheError(f"a page's slot must be a positive multiple of 16 bytes (got {slot})")
@@ -206,7 +210,7 @@ class PagePool:
             if t.dtype is not torch.int32 or t.device != dev or (shape is not None and t.shape != shape):
                 raise KvCacheError(f"{name} must be an int32 tensor on the caches' device"
                                    + (f" of shape {shape}" if shape is not None else ""))
-        if block_tables.dim() != 2 or block_tables.numel() == 0 or block_tables.stride(1) != 1 \
+        if block_tables.numel() == 0 or block_tables.stride(1) != 1 \
                 or block_tables.stride(0) < block_tables.shape[1]:
             raise KvCacheError("block_tables must be (rows, columns) with contiguous rows")
         if not seq_lens.is_contiguous() or not page_refs.is_contiguous():

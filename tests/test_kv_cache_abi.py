@@ -192,6 +192,10 @@ def test_wrapper_refusals():
     no_pool("as many", [k, k])
     no_pool("share shape", [k[:5]])
     no_pool("contiguous", [k.transpose(1, 2)], [k.transpose(1, 2)])
+    no_pool("overlap", [k[:1].expand(6, 16, 8, 64)], [k])
+    no_pool("overlap", [k], [torch.zeros(k.numel()).as_strided(k.shape, (8 * 8 * 64, 8 * 64, 64, 1))])
+    no_pool("block_tables", tables=one)
+    no_pool("block_tables", tables=torch.zeros((), dtype=torch.int32))
     no_pool("block_tables", tables=torch.zeros(2, 3))
     no_pool("block_tables", tables=torch.zeros(3, 2, dtype=torch.int32).t())
     no_pool("seq_lens", lens=one)
