@@ -45,13 +45,6 @@ constexpr int kMinPart = 64;
 constexpr int kMaxMerge = 1024;
 // workgroups a launch aims for before splitting stops: four per CU (the 128-dim 16-bit kernels hold three at once)
 constexpr int kTargetGroups = 1024;
-// the same for calls with a window: one per CU.  Their rows are short and all of a length, so no long row waits to be
-// balanced, and every further part costs its prologue and its share of the merge.  A target of 1024 and of 256 in us (bf16, 32 / 8
-// heads of 128 dims, replayed from a graph, rows x window): 1 x 4096 18.7, 13.7; 1 x 8192 29.3, 16.7; 2 x 4096 26.4,
-// 16.2; 4 x 4096 23.6, 19.1; 8 x 1024 18.7, 14.4; 8 x 4096 35.4, 33.4; 16 x 2048 35.8, 34.2; 32 x 1024 36.5, 33.9;
-// 1 x 1024, which does not reach 256 either, 10.3 both.  64 dims, 1 x 4096: 14.5, 10.7; 4 x 1024 11.1, 9.5; 16 x 1024
-// 15.6, 13.7; 32 x 1024 20.5, 18.0.
-constexpr int kWindowGroups = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Windows and sinks are clamped to this on the host, so that sums of the two and a position's alignment fit 32 bits.
@@ -411,6 +404,8 @@ template <typename T, int D, int G, bool WIN, typename Red, typename Redo>
 __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int kvh, int part, int n_parts, Red red,
                                                  float* s_m, float* s_l, float* s_w, int* s_odd, Redo redo) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  // partials by query token, with a window by workgroup along x: a chunk's tokens beside the listed ones need no room
+  const int64_t at = WIN ? (int64_t)blockIdx.x : (int64_t)qi;
   const bool direct = n_parts == 1;
   auto store = [&]() -> bool {
     bool odd = false;
@@ -425,7 +420,7 @@ __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int 
         const float l = s_l[g];
         store_one<T>(p.out, (int64_t)qi * p.so_tok + (int64_t)h * p.so_head + d, quotient<WIN>(o, l));
       } else if (p.ws_acc && part < p.max_parts) {
-        const int64_t slot_idx = ((int64_t)qi * p.hq + h) * p.max_parts + part;
+        const int64_t slot_idx = (at * p.hq + h) * p.max_parts + part;
         st_dev(&p.ws_acc[slot_idx * D + d], o);
         if (d == 0) {
           st_dev(&p.ws_ml[slot_idx * 2], s_m[g]);
@@ -462,11 +457,72 @@ __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int 
   __syncthreads();
   if (!s_last) return;
   if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (arrivals <= 64) {
+    // A lane a partition: maxima, sums and every output's first eight partials are requested together, so that a row
+    // waits for one trip to memory where the loops below wait for three and more.  The order of the sums is theirs.
+    // By those loops and so, us: 1 x 512 (32 / 8 heads of 128 dims, bf16) 10.4, 8.7; 16 x 2048 (24 / 8) 24.8, 23.2;
+    // 8 x 2048 (32 / 8) and 8 x 8192 (24 / 8) the same.
+    const int n = __builtin_amdgcn_readfirstlane(arrivals);
+    constexpr int E = (G * D + kThreads - 1) / kThreads, H = (G + kWaves - 1) / kWaves;
+    const int64_t row = at * p.hq + kvh * G;
+    float mi[H], li[H], a[E][8];
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const int g = wave + i * kWaves;
+      const bool in = g < G && lane < n;
+      const float* ml = p.ws_ml + ((row + g) * p.max_parts + lane) * 2;
+      mi[i] = in ? ld_dev(ml) : -INFINITY;
+      li[i] = in ? ld_dev(ml + 1) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const int e = threadIdx.x + k * kThreads;
+      const float* acc = p.ws_acc + (row + e / D) * p.max_parts * D + e % D;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[k][j] = e < G * D && j < n ? ld_dev(acc + j * D) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const int g = wave + i * kWaves;
+      const float m = wave_max(mi[i]);
+      const float w = m == -INFINITY || mi[i] == -INFINITY ? 0.f : exp2f(mi[i] - m);
+      const float l = wave_sum(w * li[i]);
+      if (g < G && lane < n) s_w[g * kMaxMerge + lane] = w;
+      if (g < G && lane == 0) s_l[g] = l;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const int e = threadIdx.x + k * kThreads;
+      if (e >= G * D) break;
+      const int g = e / D, d = e % D;
+      const float* acc = p.ws_acc + (row + g) * p.max_parts * D + d;
+      float o = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) o = fmaf(s_w[g * kMaxMerge + j], a[k][j], o);
+      int i = 8;
+      auto add = [&](auto count) {
+        float x[decltype(count)::value];
+#pragma unroll
+        for (int j = 0; j < decltype(count)::value; ++j) x[j] = ld_dev(acc + (i + j) * D);
+#pragma unroll
+        for (int j = 0; j < decltype(count)::value; ++j) o = fmaf(s_w[g * kMaxMerge + i + j], x[j], o);
+        i += decltype(count)::value;
+      };
+      while (i + 8 <= n) add(Int<8>{});
+      if (i + 4 <= n) add(Int<4>{});
+      if (i + 2 <= n) add(Int<2>{});
+      if (i < n) add(Int<1>{});
+      store_one<T>(p.out, (int64_t)qi * p.so_tok + (int64_t)(kvh * G + g) * p.so_head + d, quotient<WIN>(o, s_l[g]));
+    }
+    return;
+  }
   if (arrivals <= kMaxMerge) {
     // weights w_i / L of the partitions into LDS (one wave per head, lanes over partitions), then
     // every output is an independent weighted sum of the partitions' unnormalised outputs
     for (int g = wave; g < G; g += kWaves) {
-      const int64_t base = ((int64_t)qi * p.hq + kvh * G + g) * p.max_parts;
+      const int64_t base = (at * p.hq + kvh * G + g) * p.max_parts;
       float m = -INFINITY;
       for (int i = lane; i < arrivals; i += 64) m = fmaxf(m, ld_dev(&p.ws_ml[(base + i) * 2]));
       m = wave_max(m);
@@ -484,7 +540,7 @@ __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int 
     for (int e = threadIdx.x; e < G * D; e += kThreads) {
       const int g = e / D, d = e % D;
       const int h = kvh * G + g;
-      const int64_t base = ((int64_t)qi * p.hq + h) * p.max_parts;
+      const int64_t base = (at * p.hq + h) * p.max_parts;
       float o = 0.f;
       int i = 0;
       // so many partitions, their loads in flight together: 8, then 4, then one by one (1 x 65,536, 8 heads on 1
@@ -509,7 +565,7 @@ __device__ __forceinline__ void finish_partition(const PaParams& p, int qi, int 
   for (int e = threadIdx.x; e < G * D; e += kThreads) {
     const int g = e / D, d = e % D;
     const int h = kvh * G + g;
-    const int64_t base = ((int64_t)qi * p.hq + h) * p.max_parts;
+    const int64_t base = (at * p.hq + h) * p.max_parts;
     float m = -INFINITY, l = 0.f, o = 0.f;
     for (int i = 0; i < arrivals; ++i) {
       const float mi = ld_dev(&p.ws_ml[(base + i) * 2]);
@@ -1694,14 +1750,49 @@ uint64_t pw_workspace_bytes(int32_t n_tiles, int32_t hkv, int32_t head_dim, int3
   return parts <= 1 ? 0 : (uint64_t)n_tiles * hkv * parts * kPfCols * (head_dim + 2) * sizeof(float);
 }
 
-int part_tokens_for(int32_t total_q, int32_t hkv, int32_t max_seq_len, int target = kTargetGroups) {
+int part_tokens_for(int32_t total_q, int32_t hkv, int32_t max_seq_len) {
   int part = kMaxPart;
   while (part > kMinPart) {
     const int64_t parts = ((int64_t)max_seq_len + part - 1) / part;
-    if ((int64_t)total_q * hkv * parts >= target) break;
+    if ((int64_t)total_q * hkv * parts >= kTargetGroups) break;
     part >>= 1;
   }
   return part;
+}
+
+// The same with a window, where rows are short and of a length: partitions of a multiple of 64 positions, those of which
+// an estimate of the time is the least.  A workgroup of the busiest CU takes 1 us and more for a step (32 KB of key and
+// value rows), as many steps as a partition has; workgroups of one CU share its rate, and all of them the memory's;
+// splitting costs the merge, and more of it beyond the eight partitions whose sums it requests at once.  In us by the
+// rule above and by the estimate (bf16, 32 / 8 heads of 128 dims, replayed from a graph, rows x window): 1 x 240 8.8,
+// 8.3; 1 x 1024 10.2, 10.0; 1 x 4096 20.2, 14.7; 4 x 1024 13.4, 11.5; 8 x 624 15.1, 11.9; 8 x 4096 35.4, 33.0;
+// 16 x 368 16.9, 12.4; 16 x 1024 21.8, 18.5; 24 x 1024 28.9, 25.6; 40 x 1024 47.0, 43.0.  Over 135 such calls it was
+// 0.7% off the best split on average, 8% at most.
+int window_part_for(int32_t n_tokens, int32_t hkv, int32_t row_bytes, int32_t len) {
+  constexpr int kCus = 256;
+  const int64_t all = (int64_t)n_tokens * hkv, most = 1 << 20;   // (more choose as these do, within 64 bits)
+  const int64_t pairs = all < most ? all : most;
+  const int step = (1 << 14) / row_bytes;
+  int64_t best = 0;
+  int best_part = kMaxPart;
+  for (int part = kMaxPart; part > 0; part -= kMinPart) {
+    const int parts = len > part ? (int)((uint32_t)(len - 1) / (uint32_t)part) + 1 : 1;
+    const int pos = part < len ? part : len, last = len - (parts - 1) * part;
+    // workgroups, and those that keep a CU: a last partition of a few positions does not
+    const int64_t groups = pairs * parts, busy = parts > 1 && last <= part / 8 ? groups - pairs : groups;
+    const int64_t share = (busy + kCus - 1) / kCus;
+    int64_t rate = 22 * busy / kCus;   // in twentieths of a us
+    if (rate < 20) rate = 20;
+    if (share > 1 && rate < 23 * share) rate = 23 * share;
+    const int64_t walk = share > 1 ? (pos > step ? pos : step) : (int64_t)(pos + step - 1) / step * step;
+    const int64_t cost = walk * rate / step + 16 * ((groups + kCus - 1) / kCus) +
+                         (parts > 1 ? 44 + 3 * parts + (parts > 8 ? 2 * (parts - 8) : 0) : 0);
+    if (best == 0 || cost < best) {
+      best = cost;
+      best_part = part;
+    }
+  }
+  return best_part;
 }
 
 int check_sizes(int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim, int32_t max_seq_len) {
@@ -1717,17 +1808,11 @@ int check_sizes(int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim, int3
   return 0;
 }
 
-// Bytes of the per-token kernel's partials: total_q query slots (the kernel indexes them by query
-// token), the partition length sized for the n_tokens workgroups along x.
-uint64_t workspace_bytes(int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim, int32_t max_seq_len,
-                         int32_t n_tokens, int target) {
-  const int part = part_tokens_for(n_tokens, hkv, max_seq_len, target);
+// Bytes of the per-token kernel's partials: of so many query tokens' partitions.
+uint64_t workspace_bytes(int32_t tokens, int32_t hq, int32_t head_dim, int32_t max_seq_len, int part) {
   const int64_t max_parts = ((int64_t)max_seq_len + part - 1) / part;
   if (max_parts <= 1) return 0;
-  return (uint64_t)total_q * hq * max_parts * (head_dim + 2) * sizeof(float);
-}
-uint64_t workspace_bytes(int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim, int32_t max_seq_len) {
-  return workspace_bytes(total_q, hq, hkv, head_dim, max_seq_len, total_q, kTargetGroups);
+  return (uint64_t)tokens * hq * max_parts * (head_dim + 2) * sizeof(float);
 }
 
 // n_tokens decode workgroups along x (p.tokens or the first n_tokens tokens); the prefill tiles
@@ -1801,7 +1886,7 @@ struct Sizes {
   int32_t n_tokens, n_tiles;       // workgroups along x of the per-token kernel, tiles
   int32_t token_len, tile_len;     // positions that one of them can have to walk
   uint64_t token_bytes, tile_bytes;   // of workspace
-  int target;                      // workgroups that the per-token kernel's rows are split for
+  int32_t part, rows;              // positions of the per-token kernel's partitions, tokens with room for theirs
 };
 
 Sizes sizes_of(const ns_paged_attn_args* a, int32_t window, int32_t sinks) {
@@ -1810,9 +1895,10 @@ Sizes sizes_of(const ns_paged_attn_args* a, int32_t window, int32_t sinks) {
   z.n_tiles = a->prefill_tiles ? a->n_prefill_tiles : 0;
   z.token_len = walked(a->max_seq_len, window, sinks, 1);
   z.tile_len = walked(a->max_seq_len, window, sinks, kPfCols / (a->num_heads_q / a->num_kv_heads));
-  z.target = window > 0 ? kWindowGroups : kTargetGroups;
-  z.token_bytes =
-      workspace_bytes(a->total_q, a->num_heads_q, a->num_kv_heads, a->head_dim, z.token_len, z.n_tokens, z.target);
+  z.rows = window > 0 ? z.n_tokens : a->total_q;
+  z.part = window > 0 ? window_part_for(z.n_tokens, a->num_kv_heads, a->head_dim * (a->dtype == NS_PA_DTYPE_F32 ? 4 : 2), z.token_len)
+                      : part_tokens_for(z.n_tokens, a->num_kv_heads, z.token_len);
+  z.token_bytes = workspace_bytes(z.rows, a->num_heads_q, a->head_dim, z.token_len, z.part);
   z.tile_bytes = window > 0 ? pw_workspace_bytes(z.n_tiles, a->num_kv_heads, a->head_dim, z.tile_len)
                             : pf_workspace_bytes(z.n_tiles, a->num_kv_heads, a->head_dim, z.tile_len);
   return z;
@@ -1863,7 +1949,7 @@ int attend(const ns_paged_attn_args* a, int32_t window, int32_t sinks, hipStream
   const int32_t n_tiles = z.n_tiles, n_tokens = z.n_tokens;
   const uint64_t need = z.token_bytes, pf_need = z.tile_bytes;
   if (need > 0 && !a->counters) return fail("a call with split rows needs the zero-filled counters buffer");
-  const int part = part_tokens_for(n_tokens, a->num_kv_heads, z.token_len, z.target);
+  const int part = z.part;
   const int64_t max_parts = ((int64_t)z.token_len + part - 1) / part;
   if (max_parts > 65535) return fail("max_seq_len too large");
   if (need + pf_need > 0 && (!a->workspace || a->workspace_bytes < need + pf_need))
@@ -1887,7 +1973,7 @@ int attend(const ns_paged_attn_args* a, int32_t window, int32_t sinks, hipStream
   // no room of its own (the workspace may still be there for the tiles): a row longer than max_seq_len
   // allows is flagged and leaves no partials
   p.ws_acc = need ? reinterpret_cast<float*>(a->workspace) : nullptr;
-  p.ws_ml = need ? p.ws_acc + (uint64_t)a->total_q * a->num_heads_q * max_parts * a->head_dim : nullptr;
+  p.ws_ml = need ? p.ws_acc + (uint64_t)z.rows * a->num_heads_q * max_parts * a->head_dim : nullptr;
   p.counters = a->counters;
   p.sq_tok = a->stride_q_token;
   p.sq_head = a->stride_q_head;
@@ -1956,7 +2042,8 @@ int ns_paged_attention_workspace_bytes(int32_t total_q, int32_t num_heads_q, int
                                        int32_t head_dim, int32_t max_seq_len, uint64_t* bytes) {
   if (!bytes) return fail("bytes is NULL");
   if (check_sizes(total_q, num_heads_q, num_kv_heads, head_dim, max_seq_len)) return 1;
-  *bytes = workspace_bytes(total_q, num_heads_q, num_kv_heads, head_dim, max_seq_len);
+  *bytes = workspace_bytes(total_q, num_heads_q, head_dim, max_seq_len,
+                           part_tokens_for(total_q, num_kv_heads, max_seq_len));
   return 0;
 }
 
