@@ -1,4 +1,4 @@
-// The host side of the attention's and the cache store's calls: argument checks, the packing of the C ABI's structs and
+// The host side of the attention's, the cache store's and the page pool's calls: argument checks, the packing of the C ABI's structs and
 // the call, which in Python took 8 to 12 us of a call whose kernel takes 4.  The modules paged_attention.py and
 // kv_cache.py hold the interfaces and say what the arguments mean; the kernels stay behind their C ABI, whose functions
 // come in as addresses.
@@ -331,6 +331,38 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// pages(kind, the library's function, ns_kv_last_error, ns_kv_pool address, device index, list, other list or None, window,
+//       sinks, stream handle) -> None, or False where a list is not a contiguous int32 tensor of one dimension on the
+// device, for the caller to make it one.  kind 0: ns_kv_free; 1: ns_kv_extend or ns_kv_fork; 2: ns_kv_release.
+PyObject* pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!arguments(n, 10)) return nullptr;
+  return guarded(g_store_error, [&]() -> PyObject* {
+    const int64_t kind = number(a[0]), index = number(a[4]);
+    const ns_kv_pool* pool = function<const ns_kv_pool*>(a[3]);
+    const at::Tensor* list[2] = {nullptr, nullptr};
+    for (int i = 0; i < (kind == 1 ? 2 : 1); ++i) {
+      if (!THPVariable_Check(a[5 + i])) Py_RETURN_FALSE;
+      list[i] = &THPVariable_Unpack(a[5 + i]);
+      if (list[i]->scalar_type() != at::kInt || list[i]->dim() != 1 || !list[i]->is_cuda() ||
+          list[i]->get_device() != index || !list[i]->is_contiguous())
+        Py_RETURN_FALSE;
+    }
+    if (kind == 1 && list[0]->numel() != list[1]->numel())
+      throw Refused{"the two lists must be as many (got " + std::to_string(list[0]->numel()) + " and " +
+                    std::to_string(list[1]->numel()) + ")"};
+    if (list[0]->numel() > INT32_MAX) throw Refused{"the list is too long"};
+    const int32_t count = (int32_t)list[0]->numel();
+    const int64_t window = number(a[7]), sinks = number(a[8]);
+    const hipStream_t stream = reinterpret_cast<hipStream_t>(number(a[9]));
+    const int rc = kind == 0   ? function<decltype(&ns_kv_free)>(a[1])(pool, words(list[0]), count, stream)
+                   : kind == 1 ? function<decltype(&ns_kv_extend)>(a[1])(pool, words(list[0]), words(list[1]), count, stream)
+                               : function<decltype(&ns_kv_release)>(a[1])(pool, words(list[0]), count, (int32_t)window,
+                                                                          (int32_t)sinks, stream);
+    if (rc != 0) throw Refused{function<decltype(&ns_kv_last_error)>(a[2])()};
+    Py_RETURN_NONE;
+  });
+}
+
 PyObject* set_errors(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arguments(n, 2)) return nullptr;
   PyObject** to[] = {&g_attention_error, &g_store_error};
@@ -346,6 +378,7 @@ PyObject* set_errors(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef g_methods[] = {
     {"store", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(store)), METH_FASTCALL, nullptr},
     {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend)), METH_FASTCALL, nullptr},
+    {"pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pages)), METH_FASTCALL, nullptr},
     {"set_errors", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(set_errors)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_ns_host", nullptr, -1, g_methods};

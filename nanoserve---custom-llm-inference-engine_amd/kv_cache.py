@@ -74,11 +74,12 @@ class NsKvPool(ctypes.Structure):
 
 _LIB: Optional[ctypes.CDLL] = None
 _STORE = None    # the host module's function, and the addresses of the library's that it calls
+_PAGES = None    # the same for the pool's: the function, ns_kv_last_error, and the others by name
 
 
 def load(path: str = LIB_PATH) -> ctypes.CDLL:
     """Load the HIP library (raises when it is not built: there is no fallback)."""
-    global _LIB, _STORE
+    global _LIB, _STORE, _PAGES
     if _LIB is not None:
         return _LIB
     if not os.path.exists(path):
@@ -99,6 +100,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     host = host_module(KvCacheError)
     host.set_errors(None, KvCacheError)
     _STORE = (host.store, *(ctypes.cast(f, p).value for f in (lib.ns_kv_store, lib.ns_kv_last_error)))
+    _PAGES = (host.pages, _STORE[2], {n: ctypes.cast(getattr(lib, "ns_kv_" + n), p).value
+                                      for n in ("free", "extend", "fork", "release")})
     _LIB = lib
     return lib
 
@@ -234,7 +237,7 @@ class PagePool:
                               self._tensors.data_ptr(), self._scratch.data_ptr(), int(need.value),
                               block_tables.stride(0), slot, block_tables.shape[0], block_tables.shape[1], pages,
                               len(caches), bs)
-        self._ref = ctypes.byref(self._pool)
+        self._ref, self._at = ctypes.byref(self._pool), ctypes.addressof(self._pool)
 
     @classmethod
     def empty(cls, k_caches, v_caches, max_seqs: int, max_pages_per_seq: int, reserved: int = 1):
@@ -262,30 +265,38 @@ class PagePool:
             raise KvCacheError(f"{names[0]} and {names[1]} must be as many (got {a.numel()} and {b.numel()})")
         return a, b
 
+    def _change(self, kind, name, a, b, names, window, sinks, stream):
+        """One of the calls that change the tables."""
+        pages, why, entries = _PAGES
+        dev = self._dev
+        if stream is None and dev == torch.cuda.current_device():
+            if pages(kind, entries[name], why, self._at, dev, a, b, window, sinks,
+                     torch._C._cuda_getCurrentRawStream(dev)) is None:
+                return
+        handle, on = _on(dev, stream)
+        with on:   # the lists are made on the call's stream
+            if b is None:
+                a = self._list(a, names[0])
+            else:
+                a, b = self._two(a, b, names)
+            if pages(kind, entries[name], why, self._at, dev, a, b, window, sinks, handle) is not None:
+                raise KvCacheError(f"{' and '.join(names)} must be lists of rows")
+
     def extend(self, rows, lens, stream=None) -> None:
         """Row ``rows[i]`` grows to ``lens[i]`` tokens (its length grows with it) and gets the pages for them, the
         lowest free ones first.  A row is served if the pages that it and the rows listed before it ask for are all
         there; else it is left as it was (NO_PAGES).  At most MAX_ROWS rows a call."""
-        handle, on = _on(self._dev, stream)
-        with on:
-            rows, lens = self._two(rows, lens, ("rows", "lens"))
-            _check(self._lib.ns_kv_extend(self._ref, rows.data_ptr(), lens.data_ptr(), rows.numel(), handle))
+        self._change(1, "extend", rows, lens, ("rows", "lens"), 0, 0, stream)
 
     def fork(self, parents, children, stream=None) -> None:
         """Row ``children[i]``, an empty one, becomes a copy of row ``parents[i]``: full pages are shared, the tokens
         of a last page that is not full are copied, in every layer, to a page of the child's own.  A child for which
         no page is left stays empty (NO_PAGES).  At most MAX_ROWS pairs a call."""
-        handle, on = _on(self._dev, stream)
-        with on:
-            parents, children = self._two(parents, children, ("parents", "children"))
-            _check(self._lib.ns_kv_fork(self._ref, parents.data_ptr(), children.data_ptr(), parents.numel(), handle))
+        self._change(1, "fork", parents, children, ("parents", "children"), 0, 0, stream)
 
     def free(self, rows, stream=None) -> None:
         """The rows give up their pages and become empty; a page that no row names any more is free."""
-        handle, on = _on(self._dev, stream)
-        with on:
-            rows = self._list(rows, "rows")
-            _check(self._lib.ns_kv_free(self._ref, rows.data_ptr(), rows.numel(), handle))
+        self._change(0, "free", rows, None, ("rows",), 0, 0, stream)
 
     def release(self, rows, window: int, sinks: int = 0, stream=None) -> None:
         """The rows give up the pages that no later token sees through ``window`` and ``sinks`` (those of
@@ -294,10 +305,7 @@ class PagePool:
             raise KvCacheError(f"window must be at least 1 and below 2^31 (got {window})")
         if not 0 <= sinks < 2 ** 31:
             raise KvCacheError(f"sinks must lie in [0, 2^31) (got {sinks})")
-        handle, on = _on(self._dev, stream)
-        with on:
-            rows = self._list(rows, "rows")
-            _check(self._lib.ns_kv_release(self._ref, rows.data_ptr(), rows.numel(), window, sinks, handle))
+        self._change(2, "release", rows, None, ("rows",), window, sinks, stream)
 
     def copy(self, src, dst, into: Optional["PagePool"] = None, stream=None) -> None:
         """Pages ``src[i]`` to pages ``dst[i]``, in every layer, of this pool or of ``into``, a pool of pages alike.
