@@ -113,6 +113,8 @@ __device__ __forceinline__ int find_seq(const int32_t* qsl, int num_seqs, int i)
 // and, a lane per frequency, forms the angles: p * inv_freq / (2 pi) in 64 bits less its nearest whole number, so that
 // positions of millions keep their angle to 2^-26 of a turn.  Then all threads take items: 16 bytes of a head's
 // lower half and the 16 bytes half a head above, which the rotation pairs; a value head's two pieces are only copied.
+// Bound: memory.  8192 tokens of 24 / 8 heads of 128 dims (bf16, rotated; 168 MB read and written) take 30 us, 5.6 TB/s;
+// 64 tokens 3.8 us, which a launch and three loads after one another (place, table entry, row) are.
 template <typename T, int D, int TOK>
 __global__ __launch_bounds__(kStoreThreads) void store_kernel(ns_kv_store_args a) {
   using E = Elem<T>;
@@ -476,7 +478,8 @@ __global__ __launch_bounds__(kCopy) void extend_kernel(ns_kv_pool p, int n) {
   }
 }
 
-// A fork's first launch, as extending's.
+// A fork's first launch, as extending's.  Both: 3.8 us and 4.9 for one pair of 32 tensors (latency); 96 pairs of 56
+// tensors, up to 15 slots of 2 KB each, 29 us (5.6 TB/s of reads and writes, pages shared by siblings read once).
 __global__ __launch_bounds__(kPlan) void fork_plan_kernel(ns_kv_pool p, const int32_t* parents, const int32_t* children, int n) {
   __shared__ Rows s;
   const Plan plan(p);
@@ -594,7 +597,8 @@ __global__ __launch_bounds__(kCopy) void fork_kernel(ns_kv_pool p, const int32_t
 }
 
 // A workgroup a listed row: its entries in [first, last) of its columns become -1, their pages' counts fall.  An entry
-// is taken out by an exchange, so that a row listed twice gives its pages up once.
+// is taken out by an exchange, so that a row listed twice gives its pages up once.  2.4 us for one row, 3.5 for 40 of 8192
+// tokens: a launch, then reads, exchanges and counts one after the other.
 template <bool ALL>
 __global__ __launch_bounds__(kCopy) void drop_kernel(ns_kv_pool p, const int32_t* rows, int window, int sinks) {
   const int row = rows[blockIdx.x];
@@ -697,7 +701,8 @@ __global__ __launch_bounds__(kPlan) void compact_plan_kernel(ns_kv_pool p, int32
   }
 }
 
-// The first num_rows workgroups rewrite a table row each; the others take (page, tensor) pieces in turn.
+// The first num_rows workgroups rewrite a table row each; the others take (page, tensor) pieces in turn.  Bound: memory.
+// 1.7 GB of pages moved take 682 us, 4.98 TB/s of reads and writes; a large copy reaches 4.95.
 __global__ __launch_bounds__(kCopy) void compact_kernel(ns_kv_pool p, ns_kv_pool to, const int32_t* map, int into) {
   const int32_t* head = p.scratch;
   const int32_t* list = head + 4;

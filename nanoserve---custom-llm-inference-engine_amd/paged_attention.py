@@ -243,7 +243,8 @@ class PagedAttentionPlan:
 def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens,
                         scale: float, block_size: int, *, max_seq_len: Optional[int] = None,
                         max_query_len: Optional[int] = None, plan: Optional[PagedAttentionPlan] = None,
-                        window: Optional[int] = None, sinks: int = 0, out=None, workspace=None, counters=None, status=None, stream=None):
+                        window: Optional[int] = None, sinks: int = 0, out=None, workspace=None, counters=None,
+                        status=None, stream=None):
     """Attention of every query token over its sequence's paged KV (the reference's
     ``paged_attention_triton``; same arguments, same result up to float32 rounding order).
 
@@ -264,6 +265,9 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
     its own, t > p - window, and the sequence's first ``sinks`` positions.  Block-table entries of blocks that no
     token of the call sees are not read, so they may hold anything (a released block's -1).  Query rows that are
     none of a sequence's ``query_lens`` tokens (a padded batch's) are left as they were.
+
+    A call captured into a graph keeps the workspace and counters that it was captured with: graphs captured on one
+    stream share this module's counters, so they are replayed one after another, or given ``counters`` of their own.
     """
     import torch
 
