@@ -1,6 +1,6 @@
 """CPU oracle of the paged KV cache: new rows into their pages, and the pages' bookkeeping.
 
-TEST INFRASTRUCTURE ONLY: imported by ``tests/`` as the checker of the HIP kernels, never by the product.
+TEST INFRASTRUCTURE ONLY: imported by ``tests/`` as the oracle of the HIP kernels, never by the product.
 
 ``store`` follows nanoserve/model/rope.py:78-91 (rotate-half) and nanoserve/model/attention.py:55-72 (the write) in
 float64, one token after the other; a token's position is the one of oracle/paged_attention_oracle.py.  ``Pool``
