@@ -174,7 +174,8 @@ def counters_for(device, n: int, stream=None):
     """A zero-filled int32 buffer of at least ``n`` arrival counters kept per device and stream
     (calls on one stream run one after another; calls on two streams may overlap, so they never
     share counters).  Every call leaves its counters at zero whatever its shape, so the buffer
-    stays valid for all calls of its stream; it only grows, zero-filled on ``stream``."""
+    stays valid for all calls of its stream; it only grows, zero-filled on ``stream``.  One made while
+    ``stream`` is captured is filled by the graph alone, so it is that call's own and not kept."""
     import torch
 
     dev = torch.device(device)
@@ -183,6 +184,8 @@ def counters_for(device, n: int, stream=None):
     buf = _COUNTERS.get(key)
     if buf is None or buf.numel() < n:
         with torch.cuda.stream(s):
+            if torch.cuda.is_current_stream_capturing():
+                return torch.zeros(n, dtype=torch.int32, device=dev)
             buf = torch.zeros(max(n, 1 << 16), dtype=torch.int32, device=dev)
         _COUNTERS[key] = buf
     return buf
@@ -266,8 +269,9 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
     token of the call sees are not read, so they may hold anything (a released block's -1).  Query rows that are
     none of a sequence's ``query_lens`` tokens (a padded batch's) are left as they were.
 
-    A call captured into a graph keeps the workspace and counters that it was captured with: graphs captured on one
-    stream share this module's counters, so they are replayed one after another, or given ``counters`` of their own.
+    A call captured into a graph keeps the workspace and counters that it was captured with.  On a stream that made
+    such a call before, these are the stream's counters: its graphs are then replayed one after another, or given
+    ``counters`` of their own.  On another the graph zero-fills counters for each call that splits rows or tiles.
     """
     import torch
 

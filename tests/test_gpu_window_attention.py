@@ -1,5 +1,6 @@
 """GPU parity of windowed paged attention (sliding window and sinks) against the CPU oracle, with the
 tolerances of the unwindowed kernels' suite (tests/pa_cases.py): half an ulp of the output type + K * u * cond."""
+import ctypes
 import math
 
 import numpy as np
@@ -342,3 +343,81 @@ def test_captured_calls_and_side_streams(device):
     raw = call(dev[1], stream=side.cuda_stream)
     side.synchronize()
     assert torch.equal(got, want[1]) and torch.equal(raw, want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("window", [200, 420, 600, 1100, 1500, 2100, 3300, 4100, 7000])
+def test_a_row_of_few_and_many_partitions(device, window, dtype):
+    # one row: from one partition to more than two rounds of eight, with every remainder of the merge's loads
+    case = make_case(2300 + window, [7300], [1], hq=8, hkv=2, d=64, dtype=dtype)
+    check(release_hidden(case, window, 4), device, window, 4, max_query_len=1, max_seq_len=7300)
+
+
+@pytest.mark.parametrize("window", [65000, 69000])
+def test_more_partitions_than_a_wave_has_lanes(device, window):
+    case = make_case(2400, [69500], [1], hq=4, hkv=1, d=64)
+    check(release_hidden(case, window, 4), device, window, 4, max_query_len=1, max_seq_len=69500)
+
+
+def needed(case, window, sinks, plan=None):
+    """Bytes of workspace that a call is said to need."""
+    a = A.NsPagedAttnArgs()
+    a.total_q, a.num_heads_q, a.head_dim = case["query"].shape
+    a.num_seqs, a.num_kv_heads, a.max_seq_len = len(case["seq_lens"]), case["k_cache"].shape[2], int(case["seq_lens"].max())
+    a.dtype = A.NS_PA_DTYPE_BF16
+    if plan is not None:
+        a.decode_tokens, a.n_decode_tokens = plan.tokens
+        a.prefill_tiles, a.n_prefill_tiles = plan.tiles
+    n, counters = ctypes.c_uint64(), ctypes.c_uint64()
+    assert A.load().ns_paged_attention_windowed_workspace(ctypes.byref(a), window, sinks, ctypes.byref(n),
+                                                          ctypes.byref(counters)) == 0
+    return int(n.value)
+
+
+@pytest.mark.parametrize("lens,qlens", [([9000, 700, 5000], [1, 1, 1]), ([700, 9000, 4000, 3000], [300, 1, 17, 1]),
+                                        ([2000, 2000], [600, 600])])
+def test_a_workspace_of_the_size_asked_for(device, lens, qlens):
+    """Split rows and tiles stay within it, and a listed row's place in the batch does not size it."""
+    case = make_case(2500 + len(lens), lens, qlens)
+    c = to_device(case, device)
+    plan = A.PagedAttentionPlan(c["seq_lens"], c["query_start_loc"], c["query_lens"], 24, 8, c["query"].device)
+    n = needed(case, 2500, 4, plan if plan.tiles is not None else None)
+    assert n < 64 << 20
+    room = torch.full((n + 4096,), 0x5A, dtype=torch.uint8, device=device)
+    check(case, device, 2500, 4, plan=plan, workspace=room[:n])
+    assert (room[n:] == 0x5A).all()
+    if n > 0:
+        with pytest.raises(A.PagedAttentionError, match="workspace"):
+            run(case, device, 2500, 4, plan=plan, workspace=room[:n - 4])
+
+
+@pytest.mark.parametrize("window", [None, 2500])
+def test_graphs_of_a_new_stream_are_independent(device, window):
+    """Counters first needed within a capture are the graph's: the second graph runs without the first."""
+    cases = [make_case(2600, [3000, 2900], [1, 1]), make_case(2601, [2800, 3100], [1, 1])]
+    dev = [to_device(c, device) for c in cases]
+    kw = dict(max_query_len=1, max_seq_len=3100, window=window, sinks=0 if window is None else 4)
+
+    def call(c, **more):
+        return A.paged_attention_hip(c["query"], c["k_cache"], c["v_cache"], c["block_tables"], c["seq_lens"],
+                                     c["query_start_loc"], c["query_lens"], c["scale"], c["block_size"], **kw, **more)
+
+    want = [call(c) for c in dev]
+    stream = torch.cuda.Stream(device=device)
+    torch.cuda.synchronize()
+    A._COUNTERS.pop((stream.device.index or 0, stream.cuda_stream), None)   # handles come from a pool of streams
+    graphs, outs = [], [torch.zeros_like(c["query"]) for c in dev]
+    for c, out in zip(dev, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            call(c, out=out)
+        graphs.append(g)
+    assert (stream.device.index or 0, stream.cuda_stream) not in A._COUNTERS
+    for order in ((1, 0), (0, 1), (1, 1, 0)):
+        for out in outs:
+            out.zero_()
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        assert torch.equal(call(dev[0]), want[0])
