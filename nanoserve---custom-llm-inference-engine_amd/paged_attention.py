@@ -168,6 +168,17 @@ def workspace_bytes(total_q: int, num_heads_q: int, num_kv_heads: int, head_dim:
 
 
 _COUNTERS = {}
+_CAPTURED = {}    # by device and stream: a capture's id, and its counters
+
+
+def _capture_id(handle):
+    """The id of the capture that the stream of ``handle`` is in, or None."""
+    state, number = ctypes.c_int(0), ctypes.c_ulonglong(0)
+    info = load().hipStreamGetCaptureInfo   # of the HIP runtime that the library is linked with
+    info.restype = ctypes.c_int
+    info.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_ulonglong)]
+    ok = info(handle, ctypes.byref(state), ctypes.byref(number)) == 0
+    return int(number.value) if ok and state.value == 1 else None   # hipStreamCaptureStatusActive
 
 
 def counters_for(device, n: int, stream=None):
@@ -175,7 +186,7 @@ def counters_for(device, n: int, stream=None):
     (calls on one stream run one after another; calls on two streams may overlap, so they never
     share counters).  Every call leaves its counters at zero whatever its shape, so the buffer
     stays valid for all calls of its stream; it only grows, zero-filled on ``stream``.  One made while
-    ``stream`` is captured is filled by the graph alone, so it is that call's own and not kept."""
+    ``stream`` is captured is filled by the graph, when it runs, so it serves the calls of that capture alone."""
     import torch
 
     dev = torch.device(device)
@@ -185,7 +196,11 @@ def counters_for(device, n: int, stream=None):
     if buf is None or buf.numel() < n:
         with torch.cuda.stream(s):
             if torch.cuda.is_current_stream_capturing():
-                return torch.zeros(n, dtype=torch.int32, device=dev)
+                number = _capture_id(int(s.cuda_stream))
+                held = _CAPTURED.get(key)
+                if held is None or held[0] != number or number is None or held[1].numel() < n:
+                    held = _CAPTURED[key] = (number, torch.zeros(max(n, 1 << 12), dtype=torch.int32, device=dev))
+                return held[1]
             buf = torch.zeros(max(n, 1 << 16), dtype=torch.int32, device=dev)
         _COUNTERS[key] = buf
     return buf
@@ -271,7 +286,7 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
 
     A call captured into a graph keeps the workspace and counters that it was captured with.  On a stream that made
     such a call before, these are the stream's counters: its graphs are then replayed one after another, or given
-    ``counters`` of their own.  On another the graph zero-fills counters for each call that splits rows or tiles.
+    ``counters`` of their own.  On another each graph zero-fills counters of its own, once, for its calls.
     """
     import torch
 

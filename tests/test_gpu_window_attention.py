@@ -405,14 +405,20 @@ def test_graphs_of_a_new_stream_are_independent(device, window):
     want = [call(c) for c in dev]
     stream = torch.cuda.Stream(device=device)
     torch.cuda.synchronize()
-    A._COUNTERS.pop((stream.device.index or 0, stream.cuda_stream), None)   # handles come from a pool of streams
+    key = (stream.device.index or 0, stream.cuda_stream)
+    A._COUNTERS.pop(key, None)   # handles come from a pool of streams
     graphs, outs = [], [torch.zeros_like(c["query"]) for c in dev]
     for c, out in zip(dev, outs):
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=stream):
             call(c, out=out)
+            held = A._CAPTURED[key]
+            out.zero_()
+            call(c, out=out)     # the capture's second call takes the same counters
+            assert A._CAPTURED[key] is held and (not graphs or held[1].data_ptr() != before)
+        before = held[1].data_ptr()
         graphs.append(g)
-    assert (stream.device.index or 0, stream.cuda_stream) not in A._COUNTERS
+    assert key not in A._COUNTERS
     for order in ((1, 0), (0, 1), (1, 1, 0)):
         for out in outs:
             out.zero_()
