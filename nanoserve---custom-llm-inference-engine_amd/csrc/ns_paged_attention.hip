@@ -190,7 +190,7 @@ struct Hole {
   int sa, gap, h1;
   __device__ __forceinline__ int position(int v) const { return v + (v >= sa ? gap : 0); }
 };
-__device__ __forceinline__ Hole hole_of(const PaParams& p, int kv_pos) {   // kv_pos >= -1
+__device__ __forceinline__ Hole hole_of(const PaParams& p, int kv_pos) {   // kv_pos >= -kMaxWindow; below 0: no gap
   const int first = kv_pos - p.window + 1;   // the window's first position
   const int sa = (p.sinks + kAlign - 1) & -kAlign;
   const int gap = (first & -kAlign) - sa;
@@ -1225,8 +1225,10 @@ __device__ __forceinline__ PfTile pf_tile(const PaParams& p, const PfParams& f, 
   r.kv_pos0 = seq_len - ql + (r.t0 - q0);
   int lt = r.kv_pos0 + r.nq < seq_len ? r.kv_pos0 + r.nq : seq_len;
   if (lt < 0) lt = 0;
-  if constexpr (WIN) {   // the tile's first window begins first: what it leaves out, all of them do
-    r.hole = hole_of(p, r.kv_pos0 > -1 ? r.kv_pos0 : -1);
+  if constexpr (WIN) {
+    // The tile's first window begins first: what it leaves out, all of them do.  Token tok's begins at h1 + tok, so a
+    // first position below 0 (more query tokens than positions) counts as it is.
+    r.hole = hole_of(p, r.kv_pos0 > -kMaxWindow ? r.kv_pos0 : -kMaxWindow);
     lt -= r.hole.gap;
   }
   r.cut = lt > f.cap;
