@@ -168,6 +168,7 @@ def workspace_bytes(total_q: int, num_heads_q: int, num_kv_heads: int, head_dim:
 
 
 _COUNTERS = {}
+_OUTGROWN = []    # counters that larger ones replaced: graphs captured on their stream before hold their addresses
 _CAPTURED = {}    # by device and stream: a capture's id, and its counters
 
 
@@ -185,8 +186,9 @@ def counters_for(device, n: int, stream=None):
     """A zero-filled int32 buffer of at least ``n`` arrival counters kept per device and stream
     (calls on one stream run one after another; calls on two streams may overlap, so they never
     share counters).  Every call leaves its counters at zero whatever its shape, so the buffer
-    stays valid for all calls of its stream; it only grows, zero-filled on ``stream``.  One made while
-    ``stream`` is captured is filled by the graph, when it runs, so it serves the calls of that capture alone."""
+    stays valid for all calls of its stream; it only grows, zero-filled on ``stream``, to at least twice its size,
+    and what it replaces is kept for the graphs that hold it.  One made while ``stream`` is captured is filled by
+    the graph, when it runs, so it serves the calls of that capture alone."""
     import torch
 
     dev = torch.device(device)
@@ -201,6 +203,9 @@ def counters_for(device, n: int, stream=None):
                 if held is None or held[0] != number or number is None or held[1].numel() < n:
                     held = _CAPTURED[key] = (number, torch.zeros(max(n, 1 << 12), dtype=torch.int32, device=dev))
                 return held[1]
+            if buf is not None:
+                _OUTGROWN.append(buf)
+                n = max(n, 2 * buf.numel())
             buf = torch.zeros(max(n, 1 << 16), dtype=torch.int32, device=dev)
         _COUNTERS[key] = buf
     return buf
@@ -285,8 +290,9 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
     none of a sequence's ``query_lens`` tokens (a padded batch's) are left as they were.
 
     A call captured into a graph keeps the workspace and counters that it was captured with.  On a stream that made
-    such a call before, these are the stream's counters: its graphs are then replayed one after another, or given
-    ``counters`` of their own.  On another each graph zero-fills counters of its own, once, for its calls.
+    such a call before, these are the stream's counters: its graphs are then replayed one after another and not
+    beside the stream's own calls, or given ``counters`` of their own.  On another each graph zero-fills counters of
+    its own, once, for its calls.
     """
     import torch
 

@@ -62,3 +62,42 @@ def test_infinite_values_there(device, dtype, hq, n, m, window, t, value):
     assert np.isfinite(got).all()
     assert_close_to_oracle(torch.from_numpy(got).to(dtype), (np.where(hit, 0.0, ref), cond), dtype)
     assert (np.isnan(out[hit]) if math.isnan(value) else out[hit] == value).all()
+
+
+@pytest.mark.parametrize("window", [None, 2500])
+def test_a_graph_keeps_its_counters_when_the_stream_needs_more(device, window):
+    """Captured on a stream that made an eager call before; then a call on that stream outgrows its counters."""
+    case = make_case(3200, [3000, 2900], [1, 1])
+    c = to_device(case, device)
+
+    def call(out=None):
+        return A.paged_attention_hip(c["query"], c["k_cache"], c["v_cache"], c["block_tables"], c["seq_lens"],
+                                     c["query_start_loc"], c["query_lens"], c["scale"], c["block_size"], window=window,
+                                     sinks=0 if window is None else 4, max_query_len=1, max_seq_len=3000, out=out)
+
+    stream = torch.cuda.Stream(device=device)
+    key = (stream.device.index or 0, stream.cuda_stream)
+    A._COUNTERS.pop(key, None)   # handles come from a pool of streams
+    with torch.cuda.stream(stream):
+        want = call()
+        held = A._COUNTERS[key]
+        out = torch.zeros_like(c["query"])
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=stream):
+            call(out=out)
+        assert A._COUNTERS[key] is held
+        address, size = held.data_ptr(), held.numel()
+        del held
+        more = A.counters_for(device, size + 1, stream)
+        assert more.numel() >= 2 * size and A._COUNTERS[key] is more
+        # what is made now does not come to lie where the graph counts
+        filled = [torch.full((size,), 7, dtype=torch.int32, device=device) for _ in range(8)]
+        assert all(f.data_ptr() != address for f in filled)
+        for _ in range(3):
+            out.zero_()
+            g.replay()
+            assert torch.equal(call(), want)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        assert all((f == 7).all() for f in filled) and not more.any()
