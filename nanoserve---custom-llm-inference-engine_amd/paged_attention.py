@@ -338,12 +338,14 @@ def _paged_attention_on(index, handle, query, k_cache, v_cache, block_tables, se
                                                                   or max_query_len >= PREFILL_MIN_QUERY)
     if made or plan is None and max_seq_len is None:
         # the batch layout is read on the host, once the call is known to be in order
-        attend(*entries, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens, scale, block_size,
-               0, 0, 0, 0, 0, 0, 0, out, workspace, counters, status, False, -1)
-        if query.shape[0] > 0 and made:
+        empty = attend(*entries, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens, scale,
+                       block_size, 0, 0, 0, 0, 0, 0, 0, out, workspace, counters, status, False, -1)
+        if query.shape[0] == 0:
+            return empty
+        if made:
             plan = PagedAttentionPlan(seq_lens, query_start_loc, query_lens, query.shape[1], k_cache.shape[2],
                                       query.device)
-        elif max_seq_len is None:
+        else:
             max_seq_len = int(seq_lens.max().item()) if seq_lens.numel() else 0
     if plan is not None:
         # (a padded batch's rows behind the plan's are left alone with a window)

@@ -39,3 +39,35 @@ def test_counters_that_a_graph_may_hold_are_kept(host_stream):
         del now
     assert all(ref() is not None for ref in alive)
     assert total < 2 * n      # what is kept stays below what is in use
+
+
+class Unread(torch.Tensor):
+    """A tensor whose values the host does not ask for."""
+
+    def max(self, *args, **kw):
+        raise AssertionError("read on the host")
+
+    item = tolist = cpu = numpy = max
+
+
+@pytest.mark.parametrize("kw", [{}, {"max_query_len": 1}, {"max_seq_len": 8}, {"window": 5}])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_an_empty_query_reads_nothing_on_the_host(dtype, kw):
+    PA.load_host()
+    lens = torch.tensor([3, 4], dtype=torch.int32).as_subclass(Unread)
+    zero = torch.zeros(2, dtype=torch.int32).as_subclass(Unread)
+    starts = torch.zeros(3, dtype=torch.int32).as_subclass(Unread)
+    q, cache = torch.empty(0, 8, 64, dtype=dtype), torch.empty(4, 16, 8, 64, dtype=dtype)
+    out = torch.empty_like(q)
+    args = dict(max_seq_len=None, max_query_len=None, plan=None, window=None, sinks=0, out=None, workspace=None,
+                counters=None, status=None)
+    args.update(kw)
+
+    def call():
+        return PA._paged_attention_on(0, 0, q, cache, cache, torch.zeros(2, 1, dtype=torch.int32), lens, starts, zero, 1.0,
+                                      16, *args.values())
+
+    got = call()
+    assert got.shape == q.shape and got.dtype == dtype
+    args["out"] = out
+    assert call() is out
