@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 
 #include <exception>
+#include <optional>
 #include <string>
 #include <utility>
 
@@ -75,6 +76,15 @@ PyObject* guarded(PyObject* error, Body body) {
   return nullptr;
 }
 
+// Other Python threads run meanwhile: around what may wait for the device or its queue (copies, allocations, launches).
+// Nothing there touches Python's objects.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 bool arguments(Py_ssize_t got, Py_ssize_t want) {
   if (got == want) return true;
   PyErr_Format(PyExc_TypeError, "%zd arguments expected, %zd given", want, got);
@@ -137,7 +147,10 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
       throw Refused{"seq_lens/query_lens need num_seqs entries and query_start_loc num_seqs + 1"};
     if (!dev.is_cuda()) throw Refused{"store_kv_hip needs device tensors"};
     if (handle == -1) Py_RETURN_NONE;
+    const auto call = function<decltype(&ns_kv_store)>(a[0]);
+    const auto why = function<decltype(&ns_kv_last_error)>(a[1]);
     at::Tensor made, h[4];
+    std::optional<Unlocked> meanwhile(std::in_place);
     if (query != nullptr && out == nullptr) {
       made = at::empty_like(*query);
       if (made.stride(-1) != 1) made = at::empty(query->sizes(), query->options());
@@ -187,9 +200,9 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
       s.num_blocks = (int32_t)kc.size(0);
       s.max_blocks_per_seq = (int32_t)bt.size(1);
       s.dtype = dtype;
-      if (function<decltype(&ns_kv_store)>(a[0])(&s, reinterpret_cast<hipStream_t>(handle)) != 0)
-        throw Refused{function<decltype(&ns_kv_last_error)>(a[1])()};
+      if (call(&s, reinterpret_cast<hipStream_t>(handle)) != 0) throw Refused{why()};
     }
+    meanwhile.reset();
     if (query == nullptr) Py_RETURN_NONE;
     if (!made.defined()) {
       Py_INCREF(a[13]);
@@ -254,13 +267,25 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       : type == at::kFloat ? NS_PA_DTYPE_F32 : -1;
     if (dtype < 0) throw Refused{std::string("unsupported dtype ") + c10::toString(type) + " (float32, bfloat16, float16)"};
     if (handle == -1) Py_RETURN_NONE;
+    ns_paged_attn_args s = {};
+    s.max_seq_len = (int32_t)number(a[14]);
+    s.decode_tokens = reinterpret_cast<const int32_t*>(number(a[15]));
+    s.n_decode_tokens = (int32_t)number(a[16]);
+    s.prefill_tiles = reinterpret_cast<const int32_t*>(number(a[17]));
+    s.n_prefill_tiles = (int32_t)number(a[18]);
+    const int64_t window = number(a[19]), sinks = number(a[20]);
+    const auto sizes = function<decltype(&ns_paged_attention_call_workspace)>(a[0]);
+    const auto call = function<decltype(&ns_paged_attention)>(a[1]);
+    const auto window_sizes = function<decltype(&ns_paged_attention_windowed_workspace)>(a[2]);
+    const auto window_call = function<decltype(&ns_paged_attention_windowed)>(a[3]);
+    const auto why = function<decltype(&ns_pa_last_error)>(a[4]);
+    std::optional<Unlocked> meanwhile(std::in_place);
     const at::Tensor &bt = int32_on(bt0, dev, nullptr, held[0]), &sl = int32_on(sl0, dev, nullptr, held[1]),
                      &qsl = int32_on(qsl0, dev, nullptr, held[2]), &ql = int32_on(ql0, dev, nullptr, held[3]);
     if (out == nullptr) {
       made = at::empty_like(q);
       out = &made;
     }
-    ns_paged_attn_args s = {};
     s.query = q.data_ptr();
     s.k_cache = kc.data_ptr();
     s.v_cache = vc.data_ptr();
@@ -289,21 +314,13 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     s.head_dim = (int32_t)d;
     s.block_size = (int32_t)block_size;
     s.num_blocks = (int32_t)kc.size(0);
-    s.max_seq_len = (int32_t)number(a[14]);
     s.dtype = dtype;
     s.scale = (float)scale;
-    s.decode_tokens = reinterpret_cast<const int32_t*>(number(a[15]));
-    s.n_decode_tokens = (int32_t)number(a[16]);
-    s.prefill_tiles = reinterpret_cast<const int32_t*>(number(a[17]));
-    s.n_prefill_tiles = (int32_t)number(a[18]);
-    const int64_t window = number(a[19]), sinks = number(a[20]);
     auto checked = [&](int rc) {
-      if (rc != 0) throw Refused{function<decltype(&ns_pa_last_error)>(a[4])()};
+      if (rc != 0) throw Refused{why()};
     };
     uint64_t need = 0, count = 0;
-    checked(window == 0 ? function<decltype(&ns_paged_attention_call_workspace)>(a[0])(&s, &need, &count)
-                        : function<decltype(&ns_paged_attention_windowed_workspace)>(a[2])(&s, (int32_t)window, (int32_t)sinks,
-                                                                                          &need, &count));
+    checked(window == 0 ? sizes(&s, &need, &count) : window_sizes(&s, (int32_t)window, (int32_t)sinks, &need, &count));
     at::Tensor room;
     if (need > 0) {
       if (ws != nullptr && (uint64_t)ws->numel() * ws->element_size() < need)
@@ -313,7 +330,10 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       std::to_string(s.prefill_tiles != nullptr ? s.n_decode_tokens : s.total_q) + " per-token queries, " +
                       std::to_string(s.n_prefill_tiles) + " prefill tiles)"};
       const bool enough = counters != nullptr && (uint64_t)counters->numel() >= count;
-      if (!enough && (counters == nullptr || counters_grow)) return PyLong_FromUnsignedLongLong(count);
+      if (!enough && (counters == nullptr || counters_grow)) {
+        meanwhile.reset();
+        return PyLong_FromUnsignedLongLong(count);
+      }
       if (!enough || counters->scalar_type() != at::kInt || counters->device() != dev)
         throw Refused{"counters must be an int32 device tensor of at least " + std::to_string(count) + " entries"};
       if (ws == nullptr) {
@@ -325,8 +345,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       s.counters = words(counters);
     }
     const hipStream_t stream = reinterpret_cast<hipStream_t>(handle);
-    checked(window == 0 ? function<decltype(&ns_paged_attention)>(a[1])(&s, stream)
-                        : function<decltype(&ns_paged_attention_windowed)>(a[3])(&s, (int32_t)window, (int32_t)sinks, stream));
+    checked(window == 0 ? call(&s, stream) : window_call(&s, (int32_t)window, (int32_t)sinks, stream));
+    meanwhile.reset();
     return answer();
   });
 }
@@ -354,11 +374,15 @@ PyObject* pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t count = (int32_t)list[0]->numel();
     const int64_t window = number(a[7]), sinks = number(a[8]);
     const hipStream_t stream = reinterpret_cast<hipStream_t>(number(a[9]));
-    const int rc = kind == 0   ? function<decltype(&ns_kv_free)>(a[1])(pool, words(list[0]), count, stream)
-                   : kind == 1 ? function<decltype(&ns_kv_extend)>(a[1])(pool, words(list[0]), words(list[1]), count, stream)
-                               : function<decltype(&ns_kv_release)>(a[1])(pool, words(list[0]), count, (int32_t)window,
-                                                                          (int32_t)sinks, stream);
-    if (rc != 0) throw Refused{function<decltype(&ns_kv_last_error)>(a[2])()};
+    void* const call = PyLong_AsVoidPtr(a[1]);
+    const auto why = function<decltype(&ns_kv_last_error)>(a[2]);
+    std::optional<Unlocked> meanwhile(std::in_place);
+    const int rc = kind == 0   ? reinterpret_cast<decltype(&ns_kv_free)>(call)(pool, words(list[0]), count, stream)
+                   : kind == 1 ? reinterpret_cast<decltype(&ns_kv_extend)>(call)(pool, words(list[0]), words(list[1]), count, stream)
+                               : reinterpret_cast<decltype(&ns_kv_release)>(call)(pool, words(list[0]), count, (int32_t)window,
+                                                                                  (int32_t)sinks, stream);
+    if (rc != 0) throw Refused{why()};
+    meanwhile.reset();
     Py_RETURN_NONE;
   });
 }

@@ -1,14 +1,20 @@
-"""CPU checks of the host side of the attention's and the cache's calls (paged_attention.py, kv_cache.py,
+"""Checks of the host side of the attention's and the cache's calls (paged_attention.py, kv_cache.py,
 csrc/ns_host.cpp): what it keeps, reads and holds around a launch."""
 import contextlib
+import ctypes
+import os
+import subprocess
+import threading
+import time
 import types
 import weakref
 
 import pytest
 import torch
 
-from conftest import pkg
+from conftest import ROOT, pkg
 
+KV = pkg("kv_cache")
 PA = pkg("paged_attention")
 
 
@@ -71,3 +77,58 @@ def test_an_empty_query_reads_nothing_on_the_host(dtype, kw):
     assert got.shape == q.shape and got.dtype == dtype
     args["out"] = out
     assert call() is out
+
+
+@pytest.fixture
+def waiting(tmp_path):
+    """Calls a function in a C library that returns once another Python thread has run meanwhile."""
+    so = str(tmp_path / "wait_for_flag.so")
+    subprocess.run(["gcc", "-O1", "-shared", "-fPIC", os.path.join(ROOT, "tests", "native", "wait_for_flag.c"), "-o", so],
+                   check=True)
+    lib = ctypes.CDLL(so)
+    entered, flag = (ctypes.c_int.in_dll(lib, n) for n in ("entered", "flag"))
+    stop = threading.Event()
+
+    def other():
+        while not entered.value and not stop.is_set():
+            time.sleep(0.001)
+        flag.value = 1
+
+    thread = threading.Thread(target=other)
+    thread.start()
+    yield tuple(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.wait_for_flag, lib.no_flag))
+    stop.set()
+    thread.join()
+    assert entered.value
+
+
+def test_other_threads_run_during_an_attention_call(waiting):
+    PA.load_host()
+    attend, workspace = PA._ATTEND[:2]
+    launch, why = waiting
+    q, cache = torch.zeros(1, 8, 64, dtype=torch.bfloat16), torch.zeros(4, 16, 8, 64, dtype=torch.bfloat16)
+    one = torch.ones(1, dtype=torch.int32)
+    out = attend(workspace, launch, workspace, launch, why, q, cache, cache, torch.zeros(1, 1, dtype=torch.int32), one,
+                 torch.tensor([0, 1], dtype=torch.int32), one, 1.0, 16, 1, 0, 0, 0, 0, 0, 0, None, None, None, None, True, 0)
+    assert out.shape == q.shape
+
+
+@pytest.mark.gpu
+def test_other_threads_run_during_a_store(device, waiting):
+    KV.load()
+    x = torch.zeros(1, 8, 64, dtype=torch.bfloat16, device=device)
+    cache = torch.zeros(4, 16, 8, 64, dtype=torch.bfloat16, device=device)
+    one = torch.ones(1, dtype=torch.int32, device=device)
+    starts = torch.tensor([0, 1], dtype=torch.int32, device=device)
+    freq = torch.ones(32, device=device)
+    out = KV._STORE[0](*waiting, x, x, cache, cache, one[None], one, starts, one, 16, x, freq, None, None, 0)
+    assert out.shape == x.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_other_threads_run_during_a_pool_call(device, waiting, kind):
+    KV.load()
+    rows = torch.zeros(1, dtype=torch.int32, device=device)
+    launch, why = waiting
+    assert KV._PAGES[0](kind, launch, why, 0, rows.get_device(), rows, rows, 8, 0, 0) is None
