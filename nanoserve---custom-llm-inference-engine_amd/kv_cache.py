@@ -185,7 +185,9 @@ class PagePool:
     there).  What a call cannot do is left undone and marked in ``status``, an int32 device tensor of STATUS_* bits
     that the caller reads (and clears) when it wants: NO_PAGES, BAD_ROW (no such row, listed twice, or not empty),
     BAD_LENGTH, BAD_PAGE.  Results do not depend on timing: pages are handed out lowest first, in the order of
-    the list.  One pool's calls run one after another; ``stream`` as in ``store_kv_hip``.
+    the list.  One pool's calls run one after another; ``stream`` as in ``store_kv_hip``.  A pool may be dropped while
+    calls on torch's streams run: its tensors stay allocated until these have ended.  It is kept until calls on a
+    stream given as a raw handle have ended, and as long as graphs that hold its calls are replayed.
     """
 
     def __init__(self, k_caches, v_caches, block_tables, seq_lens, page_refs):
@@ -231,6 +233,7 @@ class PagePool:
         self._dev = first.get_device()
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._scratch = torch.empty(int(need.value), dtype=torch.uint8, device=dev)
+        # (a copy from pageable memory: once it returns, the tensors made before it can be used on any stream)
         self._tensors = torch.tensor([[c.data_ptr(), c.stride(0) * c.element_size()] for c in caches],
                                      dtype=torch.int64, device=dev)
         self._pool = NsKvPool(block_tables.data_ptr(), seq_lens.data_ptr(), page_refs.data_ptr(), self.status.data_ptr(),
@@ -238,6 +241,7 @@ class PagePool:
                               block_tables.stride(0), slot, block_tables.shape[0], block_tables.shape[1], pages,
                               len(caches), bs)
         self._ref, self._at = ctypes.byref(self._pool), ctypes.addressof(self._pool)
+        self._streams = set()    # handles of the torch streams that the tensors are recorded on
 
     @classmethod
     def empty(cls, k_caches, v_caches, max_seqs: int, max_pages_per_seq: int, reserved: int = 1):
@@ -248,6 +252,19 @@ class PagePool:
         refs[:reserved] = 1
         return cls(k_caches, v_caches, torch.full((max_seqs, max_pages_per_seq), -1, dtype=torch.int32, device=dev),
                    torch.zeros(max_seqs, dtype=torch.int32, device=dev), refs)
+
+    def _on(self, stream):
+        """``_on`` of a call of this pool, whose tensors are recorded on the call's stream."""
+        handle, on = _on(self._dev, stream)
+        if handle not in self._streams and (stream is None or isinstance(stream, torch.cuda.Stream)):
+            self._record(handle, torch.cuda.current_stream(self.device) if stream is None else stream)
+        return handle, on
+
+    def _record(self, handle, stream):
+        for t in (*self.k_caches, *self.v_caches, self.block_tables, self.seq_lens, self.page_refs, self.status,
+                  self._scratch, self._tensors):
+            t.record_stream(stream)
+        self._streams.add(handle)
 
     def _list(self, x, name):
         if isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.dim() == 1 and x.get_device() == self._dev \
@@ -270,10 +287,11 @@ class PagePool:
         pages, why, entries = _PAGES
         dev = self._dev
         if stream is None and dev == torch.cuda.current_device():
-            if pages(kind, entries[name], why, self._at, dev, a, b, window, sinks,
-                     torch._C._cuda_getCurrentRawStream(dev)) is None:
+            handle = torch._C._cuda_getCurrentRawStream(dev)
+            if handle in self._streams and pages(kind, entries[name], why, self._at, dev, a, b, window, sinks,
+                                                 handle) is None:
                 return
-        handle, on = _on(dev, stream)
+        handle, on = self._on(stream)
         with on:   # the lists are made on the call's stream
             if b is None:
                 a = self._list(a, names[0])
@@ -317,7 +335,9 @@ class PagePool:
             src, dst = list(src), list(dst)
             if len(set(dst)) != len(dst) or set(src) & set(dst):
                 raise KvCacheError("a page is named twice by dst, or by src and dst")
-        handle, on = _on(self._dev, stream)
+        handle, on = self._on(stream)
+        if to is not self:
+            to._on(stream)
         with on:
             src, dst = self._two(src, dst, ("src", "dst"))
             _check(self._lib.ns_kv_copy(self._ref, to._ref, src.data_ptr(), dst.data_ptr(), src.numel(), handle))
@@ -351,7 +371,9 @@ class PagePool:
             raise KvCacheError("the pools' caches differ in layers, page shape, dtype or device")
 
     def _compact(self, to, stream):
-        handle, on = _on(self._dev, stream)
+        handle, on = self._on(stream)
+        if to is not None:
+            to._on(stream)
         with on:
             page_map = torch.empty(self.num_pages, dtype=torch.int32, device=self.device)
             _check(self._lib.ns_kv_compact(self._ref, to._ref if to is not None else None, page_map.data_ptr(), handle))

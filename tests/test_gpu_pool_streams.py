@@ -1,0 +1,86 @@
+"""The page pool's tensors and the streams that its calls run on."""
+import pytest
+import torch
+
+from conftest import pkg
+
+pytestmark = pytest.mark.gpu
+KV = pkg("kv_cache")
+
+
+def busy(stream):
+    """Some milliseconds of work on ``stream``."""
+    with torch.cuda.stream(stream):
+        x = torch.randn(4096, 4096, device="cuda")
+        for _ in range(40):
+            x = x @ x * 0.01
+    assert not stream.query()
+
+
+def caches(device, n=1, pages=64):
+    return [[torch.zeros(pages, 16, 2, 64, dtype=torch.bfloat16, device=device) for _ in range(n)] for _ in range(2)]
+
+
+def test_a_new_pool_is_ready_on_any_stream(device):
+    # made on a busy stream, used on another one at once: what its making fills is filled by then
+    made, used = torch.cuda.Stream(device=device), torch.cuda.Stream(device=device)
+    k, v = caches(device)
+    torch.cuda.synchronize()
+    busy(made)
+    with torch.cuda.stream(made):
+        pool = KV.PagePool.empty(k, v, 4, 8)
+    assert made.query()
+    with torch.cuda.stream(used):
+        pool.extend([1, 9], [40, 1])
+    torch.cuda.synchronize()
+    assert pool.status.item() == KV.STATUS_BAD_ROW
+    assert pool.seq_lens.tolist() == [0, 40, 0, 0] and pool.block_tables[1, :4].tolist() == [1, 2, 3, -1]
+
+
+@pytest.mark.parametrize("way", ["current", "stream"])
+@pytest.mark.parametrize("call", ["extend", "free", "copy", "compact", "into"])
+def test_a_pool_dropped_while_a_stream_works_keeps_its_memory(device, call, way):
+    side = torch.cuda.Stream(device=device)
+    k, v = caches(device)
+    pool = KV.PagePool.empty(k, v, 4, 8)
+    other = KV.PagePool.empty(*caches(device), 4, 8)
+    pool.extend([0, 1], [40, 17])
+    rows, lens = (torch.tensor(x, dtype=torch.int32, device=device) for x in ([0, 1], [70, 33]))
+    torch.cuda.synchronize()
+    busy(side)
+    with torch.cuda.stream(side if way == "current" else torch.cuda.current_stream()):
+        kw = {} if way == "current" else {"stream": side}
+        if call == "extend":
+            pool.extend(rows, lens, **kw)
+        elif call == "free":
+            pool.free(rows, **kw)
+        elif call == "copy":
+            pool.copy(rows, lens, into=other, **kw)
+        elif call == "compact":
+            pool.compact(**kw)
+        else:
+            pool.compact_into(other, **kw)
+    held = []
+    for p in (pool, other) if call in ("copy", "into") else (pool,):
+        held += [p.status, p._scratch, p._tensors, p.block_tables, p.seq_lens, p.page_refs, *p.k_caches, *p.v_caches]
+    at = {t.data_ptr() for t in held}
+    sizes = [t.numel() * t.element_size() for t in held]
+    del pool, other, held, k, v, p
+    assert not side.query()
+    new = [torch.empty(n, dtype=torch.uint8, device=device) for n in sizes for _ in range(3)]
+    assert not side.query()
+    assert not at & {t.data_ptr() for t in new}
+    side.synchronize()
+
+
+def test_raw_handles_and_repeated_calls(device):
+    side = torch.cuda.Stream(device=device)
+    pool = KV.PagePool.empty(*caches(device), 4, 8)
+    torch.cuda.synchronize()
+    pool.extend([0], [20], stream=side.cuda_stream)
+    assert side.cuda_stream not in pool._streams      # nothing is known of such a stream's life
+    for n in (40, 41, 60):
+        pool.extend([0], [n], stream=side)
+    assert side.cuda_stream in pool._streams
+    side.synchronize()
+    assert pool.seq_lens.tolist() == [60, 0, 0, 0] and pool.status.item() == 0
