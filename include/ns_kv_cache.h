@@ -135,7 +135,8 @@ int ns_kv_copy(const ns_kv_pool* pool, const ns_kv_pool* to, const int32_t* src,
 /* The m pages in use become pages 0 .. m-1: those numbered m or higher move, in ascending order, to the free
  * ones below m.  page_map[p] (num_pages) receives page p's new number, -1 for a free page.  With `to` NULL the
  * pages move within the pool and its tables and counts follow; else the pool stays as it is and `to`, a pool of
- * as many rows, columns and tensors and of at least m pages, receives its pages, tables, lengths and counts. */
+ * as many rows, columns and tensors and of at least m pages, receives its pages, tables, lengths and counts (its memory
+ * is none of the pool's). */
 int ns_kv_compact(const ns_kv_pool* pool, const ns_kv_pool* to, int32_t* page_map, hipStream_t stream);
 
 #ifdef __cplusplus

@@ -21,6 +21,7 @@ import ctypes
 import os
 from typing import Optional
 
+import numpy as np
 import torch
 
 from .paged_attention import host_module
@@ -136,6 +137,32 @@ def _i32(t, dev, name):
     if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
         raise KvCacheError(f"{name} must be an integer tensor")
     return t.to(device=dev, dtype=torch.int32).contiguous()
+
+
+def _pieces(t):
+    """(address, bytes from piece to piece, pieces, bytes of a piece) of a tensor whose entries t[i] are contiguous."""
+    size, n = t.element_size(), t.shape[0]
+    if n and t.is_contiguous():
+        return t.data_ptr(), t.numel() * size, 1, t.numel() * size
+    return t.data_ptr(), t.stride(0) * size, n, t[0].numel() * size if n else 0
+
+
+def _overlap(a, b):
+    """Whether two tensors as ``_pieces`` takes them have a byte in common (slices of one tensor may lie between each
+    other and have none)."""
+    (a0, step_a, na, la), (b0, step_b, nb, lb) = _pieces(a), _pieces(b)
+    if min(na, nb, la, lb) < 1 or a0 + (na - 1) * step_a + la <= b0 or b0 + (nb - 1) * step_b + lb <= a0:
+        return False
+    if na == 1 or nb == 1 or step_a != step_b:
+        if na < nb:
+            a0, step_a, na, la, b0, step_b, nb, lb = b0, step_b, nb, lb, a0, step_a, na, la
+        # for each piece of b: the last of a that begins below its end
+        b = b0 + step_b * np.arange(nb, dtype=np.int64)
+        i = np.minimum((b + lb - 1 - a0) // step_a, na - 1)
+        return bool(((i >= 0) & (a0 + i * step_a + la > b)).any())
+    # of one step: piece i of a meets piece i + k of b for the k that bring them nearest
+    near = (a0 - b0) // step_a
+    return any(-na < k < nb and a0 < b0 + k * step_a + lb and b0 + k * step_a < a0 + la for k in (near, near + 1))
 
 
 def store_kv_hip(key, value, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens, block_size: int, *,
@@ -357,9 +384,10 @@ class PagePool:
         self._alike(to)
         if to.block_tables.shape != self.block_tables.shape:
             raise KvCacheError("the pools' block tables differ in shape")
-        mine = {c.data_ptr() for c in self.k_caches + self.v_caches}
-        if any(c.data_ptr() in mine for c in to.k_caches + to.v_caches):
+        if any(_overlap(a, b) for a in self.k_caches + self.v_caches for b in to.k_caches + to.v_caches):
             raise KvCacheError("the pools share a cache")
+        if any(_overlap(getattr(self, n), getattr(to, n)) for n in ("block_tables", "seq_lens", "page_refs")):
+            raise KvCacheError("the pools share a table")
         return self._compact(to, stream)
 
     def _alike(self, to):

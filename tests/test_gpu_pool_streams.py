@@ -84,3 +84,37 @@ def test_raw_handles_and_repeated_calls(device):
     assert side.cuda_stream in pool._streams
     side.synchronize()
     assert pool.seq_lens.tolist() == [60, 0, 0, 0] and pool.status.item() == 0
+
+
+def pool_over(k, v, device, tables=None, refs=None):
+    pages = k.shape[0]
+    tables = torch.full((4, 8), -1, dtype=torch.int32, device=device) if tables is None else tables
+    refs = torch.zeros(pages, dtype=torch.int32, device=device) if refs is None else refs
+    return KV.PagePool([k], [v], tables, torch.zeros(4, dtype=torch.int32, device=device), refs)
+
+
+def test_compaction_into_memory_that_the_pools_share_is_refused(device):
+    kv = torch.randn(100, 2, 16, 2, 64, device=device).to(torch.bfloat16)
+    k, v = kv[:, 0], kv[:, 1]                      # interleaved: neighbours, but no byte in common
+    whole = pool_over(k[:60], v[:60], device)
+    for other in (pool_over(k[59:], v[59:], device), pool_over(k[40:61], v[70:91], device), pool_over(v[:60], k[:60], device)):
+        with pytest.raises(KV.KvCacheError, match="share a cache"):
+            whole.compact_into(other)
+    tables = torch.full((7, 8), -1, dtype=torch.int32, device=device)
+    refs = torch.zeros(100, dtype=torch.int32, device=device)
+    low = pool_over(k[:60], v[:60], device, tables[:4], refs[:60])
+    with pytest.raises(KV.KvCacheError, match="share a table"):
+        low.compact_into(pool_over(k[60:], v[60:], device, tables[3:]))
+    with pytest.raises(KV.KvCacheError, match="share a table"):
+        low.compact_into(pool_over(k[60:], v[60:], device, refs=refs[56:96]))
+    # the rest of the same tensors is another pool's to take
+    want = kv.clone()
+    low.extend([2, 0], [33, 20])                   # pages 0 .. 2 and 3, 4
+    low.free([2])
+    high = pool_over(k[60:], v[60:], device)
+    page_map = low.compact_into(high)
+    torch.cuda.synchronize()
+    assert page_map[:6].tolist() == [-1, -1, -1, 0, 1, -1] and high.seq_lens.tolist() == [20, 0, 0, 0]
+    assert high.block_tables[0, :3].tolist() == [0, 1, -1] and high.page_refs[:3].tolist() == [1, 1, 0]
+    want[60:62] = want[3:5]
+    assert torch.equal(kv, want)

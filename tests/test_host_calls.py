@@ -3,6 +3,7 @@ csrc/ns_host.cpp): what it keeps, reads and holds around a launch."""
 import contextlib
 import ctypes
 import os
+import random
 import subprocess
 import threading
 import time
@@ -132,3 +133,33 @@ def test_other_threads_run_during_a_pool_call(device, waiting, kind):
     rows = torch.zeros(1, dtype=torch.int32, device=device)
     launch, why = waiting
     assert KV._PAGES[0](kind, launch, why, 0, rows.get_device(), rows, rows, 8, 0, 0) is None
+
+
+def bytes_of(t):
+    """The addresses of a tensor's bytes."""
+    at = torch.zeros(1, dtype=torch.int64)
+    for n, s in zip(t.shape, t.stride()):
+        at = (at[:, None] + torch.arange(n)[None, :] * s).reshape(-1)
+    return {t.data_ptr() + int(i) * t.element_size() + j for i in at for j in range(t.element_size())}
+
+
+def test_overlap_of_pages_and_tables():
+    """Against the sets of bytes themselves: slices, interleaved and strided pages, tables of one larger table."""
+    rng = random.Random(5)
+    room = torch.zeros(160, dtype=torch.int16)
+    met = 0
+    for _ in range(3000):
+        pair = []
+        for _ in range(2):
+            n, page = rng.randint(1, 6), rng.choice((1, 2, 4, 7, 8))
+            step = page + rng.choice((0, 0, 1, 4, 8, 9))
+            last = (n - 1) * step + page
+            pair.append(room[rng.randint(0, 159 - last):].as_strided((n, page), (step, 1), rng.randint(0, 159 - last)))
+        want = bool(bytes_of(pair[0]) & bytes_of(pair[1]))
+        met += want
+        assert KV._overlap(*pair) == KV._overlap(*pair[::-1]) == want, [(t.data_ptr(), t.shape, t.stride()) for t in pair]
+    assert 500 < met < 2500
+    kv = torch.zeros(12, 2, 16, 2, 8)
+    assert not KV._overlap(kv[:, 0], kv[:, 1]) and not KV._overlap(kv[:6, 0], kv[6:, 0])
+    assert KV._overlap(kv[:7, 0], kv[6:, 0]) and KV._overlap(kv[:, 0], kv[3:4, 0]) and KV._overlap(kv[:, 0], kv)
+    assert not KV._overlap(room[:0], room)
