@@ -128,7 +128,7 @@ int ns_kv_release(const ns_kv_pool* pool, const int32_t* rows, int32_t n, int32_
                   hipStream_t stream);
 
 /* Pages src[0 .. n-1] of `pool` copied to pages dst[0 .. n-1] of `to` (the same pool or one of equal tensors), in
- * every tensor.  Within one pool no page is to be named twice by dst, or by both. */
+ * every tensor.  No page is to be named twice by dst or, within one pool, by both. */
 int ns_kv_copy(const ns_kv_pool* pool, const ns_kv_pool* to, const int32_t* src, const int32_t* dst, int32_t n,
                hipStream_t stream);
 

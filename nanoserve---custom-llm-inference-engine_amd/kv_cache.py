@@ -354,13 +354,16 @@ class PagePool:
 
     def copy(self, src, dst, into: Optional["PagePool"] = None, stream=None) -> None:
         """Pages ``src[i]`` to pages ``dst[i]``, in every layer, of this pool or of ``into``, a pool of pages alike.
-        Within one pool no page is to be in ``dst`` twice or in both lists (checked for lists, not for tensors).
+        No page is to be in ``dst`` twice or, within one pool, in both lists (checked for lists, not for tensors).
         Tables and counts stay as they are."""
         to = self if into is None else into
         self._alike(to)
-        if to is self and not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
-            src, dst = list(src), list(dst)
-            if len(set(dst)) != len(dst) or set(src) & set(dst):
+        if not isinstance(dst, torch.Tensor):
+            dst = list(dst)
+            other = []
+            if to is self and not isinstance(src, torch.Tensor):
+                other = src = list(src)
+            if len(set(dst)) != len(dst) or set(other) & set(dst):
                 raise KvCacheError("a page is named twice by dst, or by src and dst")
         handle, on = self._on(stream)
         if to is not self:

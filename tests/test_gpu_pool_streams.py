@@ -118,3 +118,17 @@ def test_compaction_into_memory_that_the_pools_share_is_refused(device):
     assert high.block_tables[0, :3].tolist() == [0, 1, -1] and high.page_refs[:3].tolist() == [1, 1, 0]
     want[60:62] = want[3:5]
     assert torch.equal(kv, want)
+
+
+def test_a_copy_into_another_pool_names_no_page_twice(device):
+    pool, other = (pool_over(*(c[0] for c in caches(device)), device) for _ in range(2))
+    pool.k_caches[0].normal_()
+    for src in ([1, 2], torch.tensor([1, 2], dtype=torch.int32, device=device)):
+        with pytest.raises(KV.KvCacheError, match="named twice"):
+            pool.copy(src, [5, 5], into=other)
+    pool.copy([1, 1], [5, 6], into=other)          # one page to two places
+    pool.copy(iter([2, 3]), (3, 2), into=other)    # the numbers of two pools have nothing to do with each other
+    torch.cuda.synchronize()
+    at = [5, 6, 3, 2]
+    assert torch.equal(other.k_caches[0][at], pool.k_caches[0][[1, 1, 2, 3]])
+    assert torch.count_nonzero(other.k_caches[0]) == torch.count_nonzero(other.k_caches[0][at])
