@@ -123,6 +123,8 @@ def _on(dev: int, stream):
             return torch._C._cuda_getCurrentRawStream(dev), _NO_SWITCH
         s = torch.cuda.current_stream(dev)
     elif isinstance(stream, torch.cuda.Stream):
+        if stream.device_index != dev:
+            raise KvCacheError(f"the stream is one of device {stream.device_index}, the tensors are on device {dev}")
         s = stream
     elif int(stream) == 0:
         s = torch.cuda.default_stream(dev)

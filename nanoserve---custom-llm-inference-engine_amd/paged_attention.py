@@ -312,6 +312,9 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
                                        max_seq_len, max_query_len, plan, window, sinks, out, workspace, counters, status)
         s = torch.cuda.current_stream(query.device)
     elif isinstance(stream, torch.cuda.Stream):
+        if stream.device_index != index:
+            raise PagedAttentionError(f"the stream is one of device {stream.device_index}, the tensors are on device "
+                                      f"{index}")
         s = stream
     elif int(stream) == 0:
         # the null stream is torch's default stream (an ExternalStream of handle 0 is not it)

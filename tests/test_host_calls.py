@@ -163,3 +163,27 @@ def test_overlap_of_pages_and_tables():
     assert not KV._overlap(kv[:, 0], kv[:, 1]) and not KV._overlap(kv[:6, 0], kv[6:, 0])
     assert KV._overlap(kv[:7, 0], kv[6:, 0]) and KV._overlap(kv[:, 0], kv[3:4, 0]) and KV._overlap(kv[:, 0], kv)
     assert not KV._overlap(room[:0], room)
+
+
+class OnDevice(torch.Tensor):
+    def get_device(self):
+        return 0
+
+
+def test_a_stream_of_another_device_is_refused(monkeypatch):
+    class Stream:
+        device_index, cuda_stream = 1, 4096
+
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(PA, "_paged_attention_on", lambda *a: pytest.fail("called"))
+    x = torch.zeros(1, 8, 64).as_subclass(OnDevice)
+    cache = torch.zeros(4, 16, 8, 64).as_subclass(OnDevice)
+    n = torch.ones(1, dtype=torch.int32)
+    with pytest.raises(PA.PagedAttentionError, match="device 1"):
+        PA.paged_attention_hip(x, cache, cache, n[None], n, n, n, 1.0, 16, stream=Stream())
+    with pytest.raises(KV.KvCacheError, match="device 1"):
+        KV.store_kv_hip(x, x, cache, cache, n[None], n, n, n, 16, stream=Stream())
+    with pytest.raises(KV.KvCacheError, match="device 1"):
+        KV._on(0, Stream())
