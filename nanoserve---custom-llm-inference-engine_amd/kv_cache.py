@@ -150,9 +150,9 @@ def _pieces(t):
 
 
 def _overlap(a, b):
-    """Whether two tensors as ``_pieces`` takes them have a byte in common (slices of one tensor may lie between each
-    other and have none)."""
-    (a0, step_a, na, la), (b0, step_b, nb, lb) = _pieces(a), _pieces(b)
+    """Whether two tensors, given by their ``_pieces``, have a byte in common (slices of one tensor may lie between
+    each other and have none)."""
+    (a0, step_a, na, la), (b0, step_b, nb, lb) = a, b
     if min(na, nb, la, lb) < 1 or a0 + (na - 1) * step_a + la <= b0 or b0 + (nb - 1) * step_b + lb <= a0:
         return False
     if na == 1 or nb == 1 or step_a != step_b:
@@ -165,6 +165,25 @@ def _overlap(a, b):
     # of one step: piece i of a meets piece i + k of b for the k that bring them nearest
     near = (a0 - b0) // step_a
     return any(-na < k < nb and a0 < b0 + k * step_a + lb and b0 + k * step_a < a0 + la for k in (near, near + 1))
+
+
+class _Memory:
+    """What a pool's caches and tables occupy."""
+
+    def __init__(self, caches, tables):
+        self.caches, self.tables = [_pieces(t) for t in caches], [_pieces(t) for t in tables]
+        self.low = np.array([at for at, _, _, _ in self.caches])
+        self.high = np.array([at + step * (n - 1) + size for at, step, n, size in self.caches])
+        self.lows, self.highs = np.sort(self.low), np.sort(self.high)
+
+    def shared_cache(self, other):
+        # of each cache here, how many there begin before its end and do not end before its beginning: mostly none,
+        # which takes 5 us for 56 caches each, where looking at all pairs takes 3 ms
+        near = np.searchsorted(other.lows, self.high) - np.searchsorted(other.highs, self.low, "right")
+        return near.any() and any(_overlap(a, b) for a, n in zip(self.caches, near) if n for b in other.caches)
+
+    def shared_table(self, other):
+        return any(map(_overlap, self.tables, other.tables))
 
 
 def store_kv_hip(key, value, k_cache, v_cache, block_tables, seq_lens, query_start_loc, query_lens, block_size: int, *,
@@ -270,6 +289,7 @@ class PagePool:
                               block_tables.stride(0), slot, block_tables.shape[0], block_tables.shape[1], pages,
                               len(caches), bs)
         self._ref, self._at = ctypes.byref(self._pool), ctypes.addressof(self._pool)
+        self._memory = _Memory(caches, (block_tables, seq_lens, page_refs))
         self._streams = set()    # handles of the torch streams that the tensors are recorded on
 
     @classmethod
@@ -389,9 +409,9 @@ class PagePool:
         self._alike(to)
         if to.block_tables.shape != self.block_tables.shape:
             raise KvCacheError("the pools' block tables differ in shape")
-        if any(_overlap(a, b) for a in self.k_caches + self.v_caches for b in to.k_caches + to.v_caches):
+        if self._memory.shared_cache(to._memory):
             raise KvCacheError("the pools share a cache")
-        if any(_overlap(getattr(self, n), getattr(to, n)) for n in ("block_tables", "seq_lens", "page_refs")):
+        if self._memory.shared_table(to._memory):
             raise KvCacheError("the pools share a table")
         return self._compact(to, stream)
 

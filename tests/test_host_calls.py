@@ -143,6 +143,10 @@ def bytes_of(t):
     return {t.data_ptr() + int(i) * t.element_size() + j for i in at for j in range(t.element_size())}
 
 
+def overlap(a, b):
+    return KV._overlap(KV._pieces(a), KV._pieces(b))
+
+
 def test_overlap_of_pages_and_tables():
     """Against the sets of bytes themselves: slices, interleaved and strided pages, tables of one larger table."""
     rng = random.Random(5)
@@ -157,12 +161,35 @@ def test_overlap_of_pages_and_tables():
             pair.append(room[rng.randint(0, 159 - last):].as_strided((n, page), (step, 1), rng.randint(0, 159 - last)))
         want = bool(bytes_of(pair[0]) & bytes_of(pair[1]))
         met += want
-        assert KV._overlap(*pair) == KV._overlap(*pair[::-1]) == want, [(t.data_ptr(), t.shape, t.stride()) for t in pair]
+        assert overlap(*pair) == overlap(*pair[::-1]) == want, [(t.data_ptr(), t.shape, t.stride()) for t in pair]
     assert 500 < met < 2500
     kv = torch.zeros(12, 2, 16, 2, 8)
-    assert not KV._overlap(kv[:, 0], kv[:, 1]) and not KV._overlap(kv[:6, 0], kv[6:, 0])
-    assert KV._overlap(kv[:7, 0], kv[6:, 0]) and KV._overlap(kv[:, 0], kv[3:4, 0]) and KV._overlap(kv[:, 0], kv)
-    assert not KV._overlap(room[:0], room)
+    assert not overlap(kv[:, 0], kv[:, 1]) and not overlap(kv[:6, 0], kv[6:, 0])
+    assert overlap(kv[:7, 0], kv[6:, 0]) and overlap(kv[:, 0], kv[3:4, 0]) and overlap(kv[:, 0], kv)
+    assert not overlap(room[:0], room)
+
+
+def test_overlap_of_pools_memory():
+    rng = random.Random(6)
+    room = torch.zeros(4096, dtype=torch.int16)
+    met = 0
+    for _ in range(400):
+        caches, at = [], rng.randint(0, 3)
+        for _ in range(8):     # beside each other, with gaps that the other pool's may fall into
+            n, page = rng.randint(1, 4), rng.choice((8, 16))
+            step = page + rng.choice((0, 8, 40))
+            caches.append(room.as_strided((n, page), (step, 1), at))
+            at += (n - 1) * step + page + rng.randint(0, 300)
+        rng.shuffle(caches)
+        a, b = KV._Memory(caches[:4], caches[:1]), KV._Memory([c[:, :8] for c in caches[4:]], caches[1:2])
+        assert not a.shared_cache(b) and not b.shared_cache(a) and not a.shared_table(b)
+        other = [room.as_strided((2, 8), (rng.choice((8, 16, 200)), 1), rng.randint(0, 3800)) for _ in range(3)]
+        want = bool(set().union(*map(bytes_of, caches)) & set().union(*map(bytes_of, other)))
+        met += want
+        whole, part = KV._Memory(caches, caches), KV._Memory(other, other)
+        assert whole.shared_cache(part) == part.shared_cache(whole) == want
+        assert whole.shared_table(part) == any(overlap(x, y) for x, y in zip(caches, other))
+    assert 40 < met < 360
 
 
 class OnDevice(torch.Tensor):
