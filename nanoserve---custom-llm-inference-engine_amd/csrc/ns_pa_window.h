@@ -298,10 +298,11 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(D ==
         // per 16-position k-step s: P as the hi / lo B operands, then O^T += V^T P^T; the weights of k-step s + 1 are
         // made between the products of s
         u32x4 wh[2], wl[2];
+        float ls = 0.f;   // a step's sum by itself: added to l one by one, equal weights err to one side in their thousands
         auto weigh = [&](int s, int i2) {
           const float p0 = __builtin_amdgcn_exp2f(fmaf(st[s >> 1][8 * (s & 1) + 2 * i2], scale, -msub));
           const float p1 = __builtin_amdgcn_exp2f(fmaf(st[s >> 1][8 * (s & 1) + 2 * i2 + 1], scale, -msub));
-          l += p0 + p1;
+          ls += p0 + p1;
           const uint32_t x = M::pack2(p0, p1);
           wh[s & 1][i2] = x;
           wl[s & 1][i2] = M::pack2(p0 - M::lo(x), p1 - M::hi(x));
@@ -334,6 +335,7 @@ __global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(D ==
           }
           __builtin_amdgcn_sched_barrier(0);
         }
+        l += ls;
       }
       if (more) store_rows(jt + kPfPos, buf ^ 1);
       __syncthreads();   // the next step staged, this one read

@@ -101,3 +101,29 @@ def test_a_graph_keeps_its_counters_when_the_stream_needs_more(device, window):
             torch.cuda.synchronize()
             assert torch.equal(out, want)
         assert all((f == 7).all() for f in filled) and not more.any()
+
+
+@pytest.mark.parametrize("sink", [0.515625, 0.625])
+@pytest.mark.parametrize("d", [64, 128])
+def test_long_sums_of_equal_weights(device, d, sink):
+    """2^20 keys alike but for sixteen sinks, whose values alone are not zero: equal weights, no power of two, are added
+    one after another.  Rounding then errs to one side, an addition by at most 2^-24 of the sum so far, half of that on
+    average over the additions of one whole sum: with one for each step of 64 positions 2^14 * 2^-25 = 2^-11 of the
+    sum, besides the output's own 2^-11 and some 2^-20 for the weights.  (One for each pair of a lane's positions, 2^18,
+    is off by 1.5 to 3.5 thousandths here.)"""
+    bs, hkv, window, m = 16, 8, 2 ** 20, 8192
+    n = window + m
+    k = torch.full((2, bs, hkv, d), 0.5, dtype=torch.float16, device=device)
+    k[1] = sink
+    v = torch.zeros_like(k)
+    v[1] = 32768.0
+    q = torch.ones((m, hkv, d), dtype=torch.float16, device=device)
+    tables = torch.zeros((1, n // bs), dtype=torch.int32, device=device)
+    tables[0, 0] = 1
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)   # noqa: E731
+    out = A.paged_attention_hip(q, k, v, tables, i32(n), i32(0, m), i32(m), d ** -0.5, bs, window=window, sinks=bs)
+    w = bs * math.exp(d ** 0.5 * (sink - 0.5))
+    want = 32768.0 * w / (w + window)
+    off = (out.double().cpu() / want - 1.0).abs().max().item()
+    print(f"d {d} sink {sink}: off by {off:.2e} of {want}", flush=True)
+    assert off <= 2.0 ** -10 + 2.0 ** -20
