@@ -110,7 +110,7 @@ int ns_kv_scratch_bytes(int32_t num_pages, uint64_t* bytes);
 
 /* Rows rows[0 .. n-1] grow to lens[0 .. n-1] tokens and get the pages that these need, the lowest free pages
  * first, in the order of the list.  A row is served if the pages that it and the rows listed before it ask for
- * are all there. */
+ * are all there, or if it asks for none. */
 int ns_kv_extend(const ns_kv_pool* pool, const int32_t* rows, const int32_t* lens, int32_t n, hipStream_t stream);
 
 /* children[i], an empty row, becomes a copy of row parents[i]: the full pages are shared, the filled slots of a

@@ -114,7 +114,8 @@ __device__ __forceinline__ int find_seq(const int32_t* qsl, int num_seqs, int i)
 // positions of millions keep their angle to 2^-26 of a turn.  Then all threads take items: 16 bytes of a head's
 // lower half and the 16 bytes half a head above, which the rotation pairs; a value head's two pieces are only copied.
 // Bound: memory.  8192 tokens of 24 / 8 heads of 128 dims (bf16, rotated; 168 MB read and written) take 30 us, 5.6 TB/s;
-// 64 tokens 3.8 us, which a launch and three loads after one another (place, table entry, row) are.
+// 64 tokens 3.6 us: a launch and four trips to memory after one another (the starts that are searched, the sequence's
+// length, the table entry, the rows, which wait at the barrier although their own addresses do not need the place).
 template <typename T, int D, int TOK>
 __global__ __launch_bounds__(kStoreThreads) void store_kernel(ns_kv_store_args a) {
   using E = Elem<T>;
@@ -751,6 +752,11 @@ __global__ __launch_bounds__(kCopy) void compact_kernel(ns_kv_pool p, ns_kv_pool
 
 // ---- host side ----------------------------------------------------------------------------------------------
 
+// Four tokens a workgroup, a wave a token to place, from 4096 on; below, one, so that few tokens spread over more CUs.  In
+// us, one and four (from a graph): 24 / 8 heads of 128 dims, rotated, bf16: 64 tokens 3.6, 5.3; 512 4.4, 6.0; 2048 9.4,
+// 9.8; 4096 16.0, 15.5; 8192 31.4, 30.4.  32 / 8 of 64, f16: 512 3.6, 4.6; 2048 6.5, 7.3; 4096 11.6, 10.9; 8192 18.8, 18.1;
+// keys and values alone 512 3.0, 3.2; 2048 3.8, 3.7; 4096 6.0, 5.2; 8192 9.7, 8.3.  4 / 1 of 64: 512 3.4, 3.5; 2048 3.9,
+// 3.8; 4096 5.9, 4.2.
 template <typename T, int D>
 void launch_store(const ns_kv_store_args& a, hipStream_t stream) {
   if (a.total >= 4096)

@@ -7,8 +7,9 @@
 //   * A step's rows are placed a lane a position: each lane maps its position, reads its block-table entry and checks
 //     it, and the lanes that load the row take block and offset from it by a lane exchange: 116 us.  Placed by scalar
 //     instructions, a load's four rows at a time, a step took some 700 of them a wave, more than its products.
-//   * The window makes the tiles alike, so a workgroup takes a (tile, KV head): 113.6 us; or one of f.parts even parts of
-//     its steps where there are few of them (pw_parts_for has the figures): 105.8 us.
+//   * The window makes the tiles alike, so a workgroup takes a (tile, KV head): 113.6 us, with what follows and on a warm
+//     GPU 105 to 107; or one of f.parts even parts of its steps where there are few of them: one chunk alone 73 us, 47 in
+//     two parts (pw_parts_for has more).
 //   * LDS reads run a few ahead of their products, and the weights of the next 16 positions are made between the
 //     products of these, in an order that the compiler is held to: by itself it waits for each read before its product.
 //     On the first walk that order changed nothing (119); it stays for its registers, which are known.

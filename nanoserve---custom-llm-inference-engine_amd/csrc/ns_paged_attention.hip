@@ -1738,10 +1738,17 @@ uint64_t pf_workspace_bytes(int32_t n_tiles, int32_t hkv, int32_t head_dim, int3
 // The workgroups that share a (tile, KV head) of a windowed call, so that few tiles still fill the GPU.  The cost of a
 // count is estimated for the busiest CU, in tenths of a microsecond at 128 dims: its workgroups run two at a time, 2.8 us
 // for a step of both, 1.8 for one alone; each has some 2.5 us around its steps, and parts cost 4 and more to merge.  More
-// parts have to gain a twentieth.  Measured (24 / 8 heads of 128 dims, bf16; 1, 2, 3, 4 parts): one 512-token chunk at
-// window 2048 74, 48, 52, 44 us (4 are taken), two of them 74, 66, 74, 73 (2), three 103, 95, 89, 91 (3), four
-// 112, 116, 112, 119 (1), ten at window 1024 138, 163, 180, 206 (1); one of 17 tokens at window 4096 121 by itself, 35 in
-// eight parts.
+// parts have to gain a twentieth.  At 64 dims, where three workgroups run at a time and a step costs less, the same
+// estimate is used: its count is off the best by a sixth at most here, at 128 by a tenth.  Measured, us in 1, 2, 3, 4, 6,
+// 8 parts (from a graph; in brackets the count that is taken), at window 2048 unless stated:
+//   24 / 8 heads of 128 dims, bf16: one 512-token chunk 73, 47, 51, 43, 51, 59 (2); two 74, 64, 73, 73, 72, 85 (2); three
+//   103, 94, 88, 91, 106, 122 (3); four 105, 114, 110, 121, 135, 154 (1); three of 125 to 417 tokens at window 1000 42, 41,
+//   47, 49, 54, 63 (1); ten of 512 at window 1024 125, 153, 168, 196, 251, 329 (1); one of 17 tokens at window 4096 122,
+//   69, 51, 44, 36, 35 (11: 33); one of 128 at window 1024 39, 29, 25, 25, 26, 30 (6).
+//   32 / 8 heads of 64 dims, f16: 52, 36, 35, 32, 33, 37 (2); 53, 46, 45, 50, 52, 58 (2); 70, 61, 65, 65, 70, 79 (2); 75, 80,
+//   79, 85, 95, 107 (1); 31, 30, 30, 34, 37, 41 (1); 89, 107, 118, 131, 165, 207 (1); 93, 52, 39, 33, 27, 26 (11: 25); 30,
+//   22, 19, 18, 17, 19 (6).
+//   16 / 8 heads of 64 dims, bf16, the ten chunks: 57, 60, 62, 68, 86, 107 (2).
 int pw_parts_for(int32_t n_tiles, int32_t hkv, int32_t tile_len) {
   const int64_t pairs = (int64_t)n_tiles * hkv, steps = ((int64_t)tile_len + kPfPos - 1) / kPfPos;
   int64_t best = 0;
@@ -1781,6 +1788,10 @@ int part_tokens_for(int32_t total_q, int32_t hkv, int32_t max_seq_len) {
 // 8.3; 1 x 1024 10.2, 10.0; 1 x 4096 20.2, 14.7; 4 x 1024 13.4, 11.5; 8 x 624 15.1, 11.9; 8 x 4096 35.4, 33.0;
 // 16 x 368 16.9, 12.4; 16 x 1024 21.8, 18.5; 24 x 1024 28.9, 25.6; 40 x 1024 47.0, 43.0.  Over 135 such calls it was
 // 0.7% off the best split on average, 8% at most.
+// With sinks a row walks up to 31 positions more than the window, so a window that is a multiple of the partitions leaves
+// a last one of those few.  It is called free, and nearly is (24 / 8 heads, 1024 and so a fifth partition, 960 with one
+// of 287 positions, 832 even: 64 x 4096 198, 195, 199; 8 x 4096 28.2, 30.4, 31.5); nor does a ninth partition show, which
+// the merge requests by itself (1 x 1024 in nine 9.5, in six 9.7).
 int window_part_for(int32_t n_tokens, int32_t hkv, int32_t row_bytes, int32_t len) {
   constexpr int kCus = 256;
   const int64_t all = (int64_t)n_tokens * hkv, most = 1 << 20;   // (more choose as these do, within 64 bits)

@@ -352,7 +352,7 @@ class PagePool:
     def extend(self, rows, lens, stream=None) -> None:
         """Row ``rows[i]`` grows to ``lens[i]`` tokens (its length grows with it) and gets the pages for them, the
         lowest free ones first.  A row is served if the pages that it and the rows listed before it ask for are all
-        there; else it is left as it was (NO_PAGES).  At most MAX_ROWS rows a call."""
+        there, or if it asks for none; else it is left as it was (NO_PAGES).  At most MAX_ROWS rows a call."""
         self._change(1, "extend", rows, lens, ("rows", "lens"), 0, 0, stream)
 
     def fork(self, parents, children, stream=None) -> None:

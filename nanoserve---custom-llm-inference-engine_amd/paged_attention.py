@@ -278,7 +278,7 @@ def paged_attention_hip(query, k_cache, v_cache, block_tables, seq_lens, query_s
     than ``max_seq_len``): a caller that wants the check reads it after the call. ``workspace``
     (uint8, any contents) and ``counters`` (int32, zero-filled once; every call leaves it so) are
     allocated per call, resp. taken from this module's per-device, per-stream buffer, when not
-    given.  ``max_query_len``: an upper bound of ``query_lens`` (1 for a decode step, which then
+    given.  ``out`` lies apart from the inputs.  ``max_query_len``: an upper bound of ``query_lens`` (1 for a decode step, which then
     takes the per-token kernel without reading the batch layout on the host).  ``plan``: a
     ``PagedAttentionPlan`` of this batch layout (then nothing is read on the host).  ``stream``: a
     ``torch.cuda.Stream`` or a raw HIP stream handle, default the current stream; the call's own temporaries
