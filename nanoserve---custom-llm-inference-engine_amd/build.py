@@ -24,7 +24,10 @@ PA_OUT = os.path.join(HERE, "libns_paged_attention.so")
 # the paged KV cache: the store of new rows and the pages (include/ns_kv_cache.h)
 KV_SRC = os.path.join(HERE, "csrc", "ns_kv_cache.hip")
 KV_OUT = os.path.join(HERE, "libns_kv_cache.so")
-# the host side of the attention's and the cache's calls, a Python module over torch's C++ interface
+# the layer operators: norms, the gated activation, products of MX rows (include/ns_mx.h)
+MX_SRC = os.path.join(HERE, "csrc", "ns_mx.hip")
+MX_OUT = os.path.join(HERE, "libns_mx.so")
+# the host side of the attention's, the cache's and the layer operators' calls, a Python module over torch's C++ interface
 HOST_SRC = os.path.join(HERE, "csrc", "ns_host.cpp")
 HOST_OUT = os.path.join(HERE, "_ns_host.so")
 # the benchmark's bandwidth reference (not part of the sampler's ABI)
@@ -73,7 +76,7 @@ def _host_command(src: str, out: str) -> list:
 def build(verbose: bool = False) -> str:
     """Compile every library, the compilers side by side."""
     jobs = [(out, _command(src, out, defines)) for src, out, defines in
-            ((SRC, OUT, ()), (PA_SRC, PA_OUT, ()), (KV_SRC, KV_OUT, ()), (PROBE_SRC, PROBE_OUT, ()),
+            ((SRC, OUT, ()), (PA_SRC, PA_OUT, ()), (KV_SRC, KV_OUT, ()), (MX_SRC, MX_OUT, ()), (PROBE_SRC, PROBE_OUT, ()),
              (SRC, STAMPS_OUT, ("NS_PHASE_STAMPS",)))]
     jobs.append((HOST_OUT, _host_command(HOST_SRC, HOST_OUT)))
     procs = []
