@@ -56,33 +56,6 @@ template <typename T> __device__ __forceinline__ void load8(const void* base, in
   }
 }
 
-template <typename T> __device__ __forceinline__ void store8(void* base, int64_t at, int left, const float (&v)[8]) {
-  T* p = static_cast<T*>(base) + at;
-  if (left >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      typedef uint32_t words __attribute__((ext_vector_type(4), aligned(4)));
-      words a, b;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = __float_as_uint(v[i]);
-        b[i] = __float_as_uint(v[4 + i]);
-      }
-      *reinterpret_cast<words*>(p) = a;
-      *reinterpret_cast<words*>(p + 4) = b;
-    } else {
-      typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
-      words a;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = narrow2<T>(v[2 * i], v[2 * i + 1]);
-      *reinterpret_cast<words*>(p) = a;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) p[i] = narrow<T>(v[i]);
-  }
-}
-
 // ---- MX codes -------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t quad_max(uint32_t x) {   // over the four lanes of a quad
@@ -443,6 +416,10 @@ int ns_mx_linear(const ns_mx_linear_args* a, hipStream_t stream) {
   if (a->k < NS_MX_ROW_ALIGN || a->k % NS_MX_ROW_ALIGN != 0) return fail("k must be a positive multiple of %d (got %d)", NS_MX_ROW_ALIGN, a->k);
   if (a->m == 0 || a->n == 0) return 0;
   if (check_mx(a->x, "x", a->m, a->k) || check_mx(a->weight, "weight", a->n, a->k)) return 1;
+  // a workgroup's 256 rows are addressed by 32 bits
+  if ((a->m > 1 && (a->x.stride_codes >= 1 << 23 || a->x.stride_scales >= 1 << 23)) ||
+      (a->n > 1 && (a->weight.stride_codes >= 1 << 23 || a->weight.stride_scales >= 1 << 23)))
+    return fail("strides must be below 2^23 bytes");
   if (a->weight.format != NS_MX_FP4) return fail("weight: format must be NS_MX_FP4");
   if (!a->out) return fail("out is NULL");
   if (a->m > 1 && a->stride_out < a->n) return fail("stride_out must be at least n");

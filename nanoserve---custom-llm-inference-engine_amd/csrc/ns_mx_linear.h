@@ -56,6 +56,33 @@ template <typename T> __device__ __forceinline__ T narrow(float a) {
 }
 template <typename T> __device__ __forceinline__ float rounded(float a) { return widen<T>(narrow<T>(a)); }
 
+template <typename T> __device__ __forceinline__ void store8(void* base, int64_t at, int left, const float (&v)[8]) {
+  T* p = static_cast<T*>(base) + at;
+  if (left >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      typedef uint32_t words __attribute__((ext_vector_type(4), aligned(4)));
+      words a, b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        a[i] = __float_as_uint(v[i]);
+        b[i] = __float_as_uint(v[4 + i]);
+      }
+      *reinterpret_cast<words*>(p) = a;
+      *reinterpret_cast<words*>(p + 4) = b;
+    } else {
+      typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
+      words a;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = narrow2<T>(v[2 * i], v[2 * i + 1]);
+      *reinterpret_cast<words*>(p) = a;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) p[i] = narrow<T>(v[i]);
+  }
+}
+
 // ---- one 16 x 16 tile a wave ------------------------------------------------------------------------------------
 
 template <int XF> __device__ __forceinline__ f32x4 products(u32x4 w, const u32x4 (&x)[2], int sw, int sx, f32x4 c) {
@@ -98,8 +125,170 @@ template <typename T, int XF> __global__ __launch_bounds__(256) void linear_kern
     if (n0 + 4 * g + e < a.n) out[e] = narrow<T>(acc[e]);
 }
 
+// ---- tiles through LDS ------------------------------------------------------------------------------------------
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+}
+
+// One direct load: 16 (4) bytes a lane from the buffer at voff + soff, to LDS at dst + 16 (4) lane (dst the same for the wave).
+__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, unsigned char* dst, uint32_t voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 16, voff, soff, 0, 0);
+}
+__device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, unsigned char* dst, uint32_t voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 4, voff, soff, 0, 0);
+}
+
+// `rows` rows from row `first` on
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* base, int64_t first, int64_t stride, int rows, int width) {
+  return rsrc(static_cast<const unsigned char*>(base) + first * stride, (uint32_t)((rows - 1) * stride + width));
+}
+
+// A workgroup computes BM rows of x by BN rows of the weight, its WM x WN waves 16 TI by 16 TJ each.  Stages of 128
+// columns go to LDS by direct loads, two stages ahead, in a ring of three: at stage t a wave waits for its own share of
+// stage t, the barrier makes everyone's visible and says that everyone is past stage t - 1, whose place stage t + 2 takes.
+// The three places are three arrays and the loop is unrolled by three: the compiler sees that a stage's reads touch none
+// that a direct load is filling, and waits for none of those.
+//
+// LDS rows are the stage's codes of a matrix row: 8 (8-bit) or 4 pieces of 16 bytes.  Piece c of row r lies at c ^ f(r), so
+// that 16 lanes that read one piece of 16 rows, and either 8 of them, meet every bank once: f = (r & 7) ^ (r >> 3 & 1) for
+// 8 pieces, and for the weight's 4 f = (r >> 3 & 3) ^ (r & 2).  The weight's rows go to the instruction in an order that leaves
+// a lane with 8 consecutive outputs: of a pair of its 16-row operands, row 8 a + 4 p + e is row 4 a + e of operand p.
+template <typename T, int XF, int BM, int BN, int WM, int WN>
+struct Tile {
+  static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int TI = BM / WM / 16, TJ = BN / WN / 16;
+  static constexpr int XP = XF == NS_MX_FP8 ? 8 : 4;            // pieces of an x row in a stage
+  static constexpr int XB = BM * XP * 16, WB = BN * 4 * 16;     // bytes of a stage
+  static constexpr int XL = XB / 1024 / WAVES, WL = WB / 1024 / WAVES, SL = (BM + BN + THREADS - 1) / THREADS;
+  static constexpr int SB = SL * THREADS * 4;                   // scales: 4 bytes of every row
+  static constexpr int BYTES = XB + WB + SB;
+  static_assert(XL * 1024 * WAVES == XB && WL * 1024 * WAVES == WB && TJ % 2 == 0 && BM % 64 == 0 && BN % 64 == 0, "tiling");
+};
+
+template <typename T, int XF, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linear_args a) {
+  using C = Tile<T, XF, BM, BN, WM, WN>;
+  constexpr int TI = C::TI, TJ = C::TJ, XP = C::XP;
+  __shared__ __attribute__((aligned(16))) unsigned char s0[C::BYTES], s1[C::BYTES], s2[C::BYTES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int nx = (int)((a.m + BM - 1) / BM);
+  const int64_t m0 = (int64_t)(blockIdx.x % nx) * BM, n0 = (int64_t)(blockIdx.x / nx) * BN;
+  const int mrows = (int)min((int64_t)BM, a.m - m0), nrows = (int)min((int64_t)BN, a.n - n0);
+  // rows past the ends lie behind the buffers' ends and read as zeros
+  const __amdgpu_buffer_rsrc_t xr = rows_buffer(a.x.codes, m0, a.x.stride_codes, mrows, XF == NS_MX_FP8 ? a.k : a.k / 2);
+  const __amdgpu_buffer_rsrc_t wr = rows_buffer(a.weight.codes, n0, a.weight.stride_codes, nrows, a.k / 2);
+  const __amdgpu_buffer_rsrc_t xsr = rows_buffer(a.x.scales, m0, a.x.stride_scales, mrows, a.k / 32);
+  const __amdgpu_buffer_rsrc_t wsr = rows_buffer(a.weight.scales, n0, a.weight.stride_scales, nrows, a.k / 32);
+  uint32_t xo[C::XL], wo[C::WL], so[C::SL];
+#pragma unroll
+  for (int j = 0; j < C::XL; ++j) {
+    const int at = j * C::THREADS + tid, row = at / XP, c = at % XP;
+    const int f = XP == 8 ? (row & 7) ^ (row >> 3 & 1) : (row >> 1 & 3) ^ (row >> 3 & 1);
+    xo[j] = (uint32_t)(row * a.x.stride_codes + 16 * (c ^ f));
+  }
+#pragma unroll
+  for (int j = 0; j < C::WL; ++j) {
+    const int at = j * C::THREADS + tid, row = at / 4, c = at % 4;
+    wo[j] = (uint32_t)(row * a.weight.stride_codes + 16 * (c ^ ((row >> 3 & 3) ^ (row & 2))));
+  }
+#pragma unroll
+  for (int j = 0; j < C::SL; ++j) {
+    const int row = j * C::THREADS + tid;
+    so[j] = (uint32_t)(row < BM ? row * a.x.stride_scales : row < BM + BN ? (row - BM) * a.weight.stride_scales : 0);
+  }
+  const int nst = a.k / 128;
+  const auto load = [&](int stage, unsigned char* to) {   // stages past the last are it again
+    const int st = stage < nst ? stage : nst - 1;
+#pragma unroll
+    for (int j = 0; j < C::XL; ++j)
+      load_lds16(xr, to + (j * C::WAVES + wave) * 1024, xo[j], st * XP * 16);
+#pragma unroll
+    for (int j = 0; j < C::WL; ++j)
+      load_lds16(wr, to + C::XB + (j * C::WAVES + wave) * 1024, wo[j], st * 64);
+#pragma unroll
+    for (int j = 0; j < C::SL; ++j)
+      load_lds4((j * C::WAVES + wave) * 64 < BM ? xsr : wsr, to + C::XB + C::WB + (j * C::WAVES + wave) * 256, so[j], st * 4);
+  };
+  const int wm = wave % WM, wn = wave / WM;
+  const int x_row = wm * (16 * TI) + r;                              // of operand 0; operand i: 16 i more
+  const int w_row = wn * (16 * TJ) + 8 * (r >> 2) + (r & 3);         // of operand 0; operand 2 q + p: 32 q + 4 p more
+  const int xf = XP == 8 ? (x_row & 7) ^ (x_row >> 3 & 1) : (x_row >> 1 & 3) ^ (x_row >> 3 & 1);
+  const int wf = (w_row >> 3 & 3) ^ (w_row & 2);
+  const int x_at = x_row * (XP * 16) + 16 * (g ^ xf), x_at2 = x_row * (XP * 16) + 16 * ((4 + g) ^ xf);
+  const int w_at = C::XB + w_row * 64 + 16 * (g ^ wf);
+  const int sx_at = C::XB + C::WB + x_row * 4 + g, sw_at = C::XB + C::WB + (BM + w_row) * 4 + g;
+  f32x4 acc[TI][TJ];
+#pragma unroll
+  for (int i = 0; i < TI; ++i)
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int LOADS = C::XL + C::WL + C::SL;
+  constexpr int WAIT = (LOADS & 15) | (7 << 4) | (15 << 8) | ((LOADS >> 4) << 14);   // vmcnt(LOADS) alone
+  const auto stage = [&](int st, const unsigned char* from, unsigned char* to) {
+    __builtin_amdgcn_s_waitcnt(WAIT);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    load(st + 2, to);
+    __builtin_amdgcn_sched_barrier(0);
+    const unsigned char *xs = from + x_at, *xs2 = from + x_at2, *ws = from + w_at, *sx0 = from + sx_at, *sw0 = from + sw_at;
+    u32x4 w[TJ];
+    int sw[TJ];
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {   // f is the same for all: 32 and 4 leave its bits alone
+      const int row = 32 * (j >> 1) + 4 * (j & 1);
+      w[j] = *reinterpret_cast<const u32x4*>(ws + row * 64);
+      sw[j] = sw0[row * 4];
+    }
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      u32x4 x[2];
+      x[0] = *reinterpret_cast<const u32x4*>(xs + i * (XP * 256));
+      if constexpr (XP == 8) x[1] = *reinterpret_cast<const u32x4*>(xs2 + i * (XP * 256));
+      const int sx = sx0[i * 64];
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[i][j] = products<XF>(w[j], x, sw[j], sx, acc[i][j]);
+    }
+  };
+  load(0, s0);
+  load(1, s1);
+  int st = 0;
+  for (; st + 3 <= nst; st += 3) {
+    stage(st, s0, s2);
+    stage(st + 1, s1, s0);
+    stage(st + 2, s2, s1);
+  }
+  if (st < nst) stage(st, s0, s2);
+  if (st + 1 < nst) stage(st + 1, s1, s0);
+  __builtin_amdgcn_s_waitcnt(0);   // nothing may land in LDS after the workgroup ends
+  // operand pair q, token r: outputs 32 q + 8 g .. + 7
+#pragma unroll
+  for (int i = 0; i < TI; ++i) {
+    const int64_t row = m0 + x_row + 16 * i;
+    if (row >= a.m) continue;
+#pragma unroll
+    for (int q = 0; q < TJ / 2; ++q) {
+      const int64_t col = n0 + wn * (16 * TJ) + 32 * q + 8 * g;
+      const float v[8] = {acc[i][2 * q][0], acc[i][2 * q][1], acc[i][2 * q][2], acc[i][2 * q][3],
+                          acc[i][2 * q + 1][0], acc[i][2 * q + 1][1], acc[i][2 * q + 1][2], acc[i][2 * q + 1][3]};
+      const int64_t left = a.n - col;
+      if (left > 0) store8<T>(a.out, row * a.stride_out + col, left < 8 ? (int)left : 8, v);
+    }
+  }
+}
+
+template <typename T, int XF, int BM, int BN, int WM, int WN> const char* launch_tile(const ns_mx_linear_args& a, hipStream_t stream) {
+  const int64_t blocks = ((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN);
+  if (blocks >= (int64_t)1 << 31) return "too many rows";
+  hipLaunchKernelGGL((tile_kernel<T, XF, BM, BN, WM, WN>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  return nullptr;
+}
+
 template <typename T, int XF> const char* launch_linear_t(const ns_mx_linear_args& a, hipStream_t stream) {
-  if (a.m > 16 * 65535) return "m must be at most 1048560";
+  if (a.m > 64) return launch_tile<T, XF, 256, 256, 4, 2>(a, stream);
   hipLaunchKernelGGL((linear_kernel<T, XF>), dim3((unsigned)((a.n + 63) / 64), (unsigned)((a.m + 15) / 16)), dim3(256), 0, stream, a);
   return nullptr;
 }

@@ -134,7 +134,8 @@ def test_quantize_refusals(kw, word):
     (dict(x=rows(stride_codes=128)), "wide"), (dict(x=rows(stride_scales=4)), "wide"),
     (dict(weight=rows()), "NS_MX_FP4"), (dict(weight=rows(format=MX.NS_MX_FP4, scales=None)), "NULL"),
     (dict(weight=rows(format=MX.NS_MX_FP4, stride_codes=112)), "wide"), (dict(out=None), "out"),
-    (dict(stride_out=15), "stride_out")])
+    (dict(stride_out=15), "stride_out"), (dict(x=rows(stride_codes=1 << 23)), "2^23"),
+    (dict(weight=rows(format=MX.NS_MX_FP4, stride_scales=1 << 23)), "2^23")])
 def test_linear_refusals(kw, word):
     refused("ns_mx_linear", linear_args(**kw), word)
 
