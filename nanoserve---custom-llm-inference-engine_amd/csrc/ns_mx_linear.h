@@ -83,7 +83,7 @@ template <typename T> __device__ __forceinline__ void store8(void* base, int64_t
   }
 }
 
-// ---- one 16 x 16 tile a wave ------------------------------------------------------------------------------------
+// ---- operands ---------------------------------------------------------------------------------------------------
 
 template <int XF> __device__ __forceinline__ f32x4 products(u32x4 w, const u32x4 (&x)[2], int sw, int sx, f32x4 c) {
   const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
@@ -96,43 +96,21 @@ template <int XF> __device__ __forceinline__ f32x4 products(u32x4 w, const u32x4
   }
 }
 
-template <typename T, int XF> __global__ __launch_bounds__(256) void linear_kernel(ns_mx_linear_args a) {
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int64_t n0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16, m0 = (int64_t)blockIdx.y * 16;
-  if (n0 >= a.n) return;
-  // rows past the ends read the last one; nothing of theirs is stored
-  const int64_t wr = min(n0 + r, a.n - 1), xr = min(m0 + r, a.m - 1);
-  const unsigned char* wc = static_cast<const unsigned char*>(a.weight.codes) + wr * a.weight.stride_codes + 16 * g;
-  const uint8_t* ws = a.weight.scales + wr * a.weight.stride_scales + g;
-  const unsigned char* xc = static_cast<const unsigned char*>(a.x.codes) + xr * a.x.stride_codes + 16 * g;
-  const uint8_t* xs = a.x.scales + xr * a.x.stride_scales + g;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int k = 0; k < a.k; k += 128) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(wc + k / 2);
-    u32x4 x[2];
-    if constexpr (XF == NS_MX_FP8) {
-      x[0] = *reinterpret_cast<const u32x4*>(xc + k);
-      x[1] = *reinterpret_cast<const u32x4*>(xc + k + 64);
-    } else {
-      x[0] = *reinterpret_cast<const u32x4*>(xc + k / 2);
-    }
-    acc = products<XF>(w, x, ws[k / 32], xs[k / 32], acc);
-  }
-  if (m0 + r >= a.m) return;
-  T* out = static_cast<T*>(a.out) + (m0 + r) * a.stride_out + n0 + 4 * g;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (n0 + 4 * g + e < a.n) out[e] = narrow<T>(acc[e]);
-}
-
-// ---- tiles through LDS ------------------------------------------------------------------------------------------
-
 typedef __attribute__((address_space(3))) void lds_void;
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
 }
-
+// `rows` rows from row `first` on
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* base, int64_t first, int64_t stride, int rows, int width) {
+  return rsrc(static_cast<const unsigned char*>(base) + first * stride, (uint32_t)((rows - 1) * stride + width));
+}
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t voff, int soff) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, soff, 0));
+}
+__device__ __forceinline__ int load1(__amdgpu_buffer_rsrc_t r, uint32_t voff, int soff) {
+  return (int)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)voff, soff, 0);
+}
 // One direct load: 16 (4) bytes a lane from the buffer at voff + soff, to LDS at dst + 16 (4) lane (dst the same for the wave).
 __device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, unsigned char* dst, uint32_t voff, int soff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 16, voff, soff, 0, 0);
@@ -141,10 +119,208 @@ __device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, unsigned cha
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 4, voff, soff, 0, 0);
 }
 
-// `rows` rows from row `first` on
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* base, int64_t first, int64_t stride, int rows, int width) {
-  return rsrc(static_cast<const unsigned char*>(base) + first * stride, (uint32_t)((rows - 1) * stride + width));
+// ---- few rows: the weight streamed through registers ------------------------------------------------------------
+
+// vmcnt(n) alone
+#define NS_MX_VMCNT(n) (((n) & 15) | (7 << 4) | (15 << 8) | (((n) >> 4) << 14))
+
+// A workgroup of eight waves computes 16 TM rows of x by 32 outputs for each of its 8 / KW waves side by side, and goes on
+// to further outputs; KW waves share one set of outputs, their columns dealt out in groups of 512 (four stages of 128).
+// The weight goes from memory into the operand registers of the one wave that uses it: a stage's registers are refilled
+// with the wave's next group as soon as its products are issued, whatever output it is of, so that 8 KB stay in flight per
+// wave.  x lies in LDS, in two halves of KS stages: where its columns fit they stay there and the waves run on their own;
+// else the halves take turns, one filled by direct loads while the other is used, with a barrier for each.  Sums of KW
+// waves meet in LDS and are added in the waves' order.
+//
+// LDS rows are the stage's codes of a row of x: 8 (8-bit) or 4 pieces of 16 bytes, piece c of row r at c ^ f(r), so that 16
+// lanes that read one piece of 16 rows, and either 8 of them, meet every bank once: f = (r & 7) ^ (r >> 3 & 1) for 8
+// pieces, (r >> 1 & 3) ^ (r >> 3 & 1) for 4.  The weight's rows go to the instruction in an order that leaves a lane with 8
+// consecutive outputs: of a pair of its 16-row operands, row 8 a + 4 p + e is row 4 a + e of operand p.
+template <int PIECES> __device__ __forceinline__ int x_swizzle(int row) {
+  return PIECES == 8 ? (row & 7) ^ (row >> 3 & 1) : (row >> 1 & 3) ^ (row >> 3 & 1);
 }
+
+template <int XF, int TM, int KS> struct Stream {
+  static constexpr int XP = XF == NS_MX_FP8 ? 8 : 4;
+  static constexpr int XSTEP = 16 * TM * XP * 16;                  // bytes of a stage's codes
+  static constexpr int XB = KS * XSTEP, SB = KS * 16 * TM * 4;     // of a half's codes and scales
+  static constexpr int FILLS = XB / 1024 / 8;                      // 16-byte direct loads of a thread
+  static_assert(FILLS * 8192 == XB, "tiling");
+};
+
+template <typename T, int XF, int TM, int KW, int KS>
+__global__ __launch_bounds__(512, TM < 4 ? 4 : 2) void stream_kernel(const ns_mx_linear_args a, int blocks_n) {
+  using C = Stream<XF, TM, KS>;
+  constexpr int XP = C::XP, NW = 8 / KW, GROUPS = KS / 4;
+  static_assert(GROUPS % KW == 0, "tiling");
+  __shared__ __attribute__((aligned(16))) unsigned char s0[C::XB + C::SB], s1[C::XB + C::SB];
+  __shared__ float sums[KW > 1 ? 8 * TM * 8 * 64 : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
+  const int kw = wave % KW, nw = wave / KW;
+  const int64_t m0 = (int64_t)(blockIdx.x / blocks_n) * (16 * TM);
+  const int mrows = (int)min((int64_t)(16 * TM), a.m - m0), xw = XF == NS_MX_FP8 ? a.k : a.k / 2;
+  const __amdgpu_buffer_rsrc_t xr = rows_buffer(a.x.codes, m0, a.x.stride_codes, mrows, xw);
+  const __amdgpu_buffer_rsrc_t xsr = rows_buffer(a.x.scales, m0, a.x.stride_scales, mrows, a.k / 32);
+  const int nst = a.k / 128, ng = (nst + 3) / 4, nc = (nst + KS - 1) / KS;
+  const bool resident = nc <= 2;
+
+  const auto fill = [&](int c, unsigned char* to) {
+    const int base = c * KS;
+#pragma unroll
+    for (int j = 0; j < C::FILLS; ++j) {
+      const int at = (j * 8 + wave) * 64 + lane, step = at / (16 * TM * XP), row = at / XP % (16 * TM), p = at % XP;
+      const int st = min(base + step, nst - 1);
+      load_lds16(xr, to + (j * 8 + wave) * 1024,
+                 (uint32_t)(row * a.x.stride_codes + st * (XP * 16) + 16 * (p ^ x_swizzle<XP>(row))), 0);
+    }
+    for (int j = wave; j < KS * TM / 4; j += 8) {
+      const int at = j * 64 + lane, step = at / (16 * TM), row = at % (16 * TM), st = min(base + step, nst - 1);
+      load_lds4(xsr, to + C::XB + j * 256, (uint32_t)(row * a.x.stride_scales + st * 4), 0);
+    }
+  };
+
+  const int tiles = (int)((a.n + 31) / 32), step_tiles = blocks_n * NW;
+  int tile = (int)(blockIdx.x % blocks_n) * NW + nw;
+  uint32_t wo[2], wso[2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    const int row = 8 * (r >> 2) + 4 * p + (r & 3);
+    wo[p] = (uint32_t)(row * a.weight.stride_codes + 16 * g);
+    wso[p] = (uint32_t)(row * a.weight.stride_scales);
+  }
+  u32x4 w[4][2], scale[2], next[2];
+  __amdgpu_buffer_rsrc_t wr, wsr;
+  const auto aim = [&](int t) {   // at a set of outputs; past the last: at nothing, which reads as zeros
+    const int64_t n0 = (int64_t)t * 32;
+    const int rows = t < tiles ? (int)min((int64_t)32, a.n - n0) : 0;
+    wr = rsrc(static_cast<const unsigned char*>(a.weight.codes) + (rows ? n0 : 0) * a.weight.stride_codes,
+              rows ? (uint32_t)((rows - 1) * a.weight.stride_codes + a.k / 2) : 0u);
+    wsr = rsrc(a.weight.scales + (rows ? n0 : 0) * a.weight.stride_scales,
+               rows ? (uint32_t)((rows - 1) * a.weight.stride_scales + a.k / 32) : 0u);
+  };
+  const auto load_stage = [&](int s, int q) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) w[s][p] = load16(wr, wo[p] + 64 * s, q * 256);
+  };
+  f32x4 acc[TM][2];
+  const int xf = x_swizzle<XP>(r);
+  const int x_at = r * (XP * 16) + 16 * (g ^ xf), x_at2 = r * (XP * 16) + 16 * ((4 + g) ^ xf);
+  const int sx_at = C::XB + r * 4 + g;
+
+  // the products of group q, and the loads of the group that this wave takes next
+  const auto group = [&](int q, const unsigned char* from) {
+    const bool here = q + KW < ng;
+    const int then = here ? q + KW : kw;
+    if (!here) aim(tile + step_tiles);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) next[p] = load16(wsr, wso[p], then * 16);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if (4 * q + s < nst) {
+        const int st = (4 * q + s) % KS;
+        const unsigned char *xs = from + st * C::XSTEP + x_at, *xs2 = from + st * C::XSTEP + x_at2, *sx = from + st * (16 * TM * 4) + sx_at;
+        const int sw[2] = {(int)(scale[0][s] >> (8 * g)), (int)(scale[1][s] >> (8 * g))};
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          u32x4 x[2];
+          x[0] = *reinterpret_cast<const u32x4*>(xs + i * (XP * 256));
+          if constexpr (XP == 8) x[1] = *reinterpret_cast<const u32x4*>(xs2 + i * (XP * 256));
+          const int f = sx[i * 64];
+#pragma unroll
+          for (int p = 0; p < 2; ++p) acc[i][p] = products<XF>(w[s][p], x, sw[p], f, acc[i][p]);
+        }
+      }
+      load_stage(s, then);
+    }
+    scale[0] = next[0];
+    scale[1] = next[1];
+  };
+
+  fill(0, s0);
+  if (resident && nc > 1) fill(1, s1);
+  aim(kw < ng ? tile : tiles);
+  scale[0] = load16(wsr, wso[0], kw * 16);
+  scale[1] = load16(wsr, wso[1], kw * 16);
+#pragma unroll
+  for (int s = 0; s < 4; ++s) load_stage(s, kw);
+  bool started = true;    // whether a group's ten loads are newer than the last fill's
+  int half = 0;
+  const auto chunk = [&](int c, unsigned char* from, unsigned char* other, bool wait, bool more) {
+    if (wait) {
+      if (started) __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(10));
+      else __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(0));
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+      if (more) {
+        fill(c + 1 < nc ? c + 1 : 0, other);
+        started = false;
+      }
+    }
+#pragma unroll 1
+    for (int j = 0; j < GROUPS / KW; ++j) {
+      const int q = c * GROUPS + kw + KW * j;
+      if (q < ng) {
+        group(q, from);
+        started = true;
+      }
+    }
+  };
+  const int rounds = (tiles - (tile - nw) + step_tiles - 1) / step_tiles;   // the same for every wave
+  for (int round = 0; round < rounds; ++round, tile += step_tiles) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) acc[i][0] = acc[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < nc; ++c) {
+      const bool wait = !resident || (round == 0 && c == 0), more = !resident && (c + 1 < nc || round + 1 < rounds);
+      if (half == 0) chunk(c, s0, s1, wait, more);
+      else chunk(c, s1, s0, wait, more);
+      half = nc > 1 ? half ^ 1 : 0;
+    }
+    if (resident) half = 0;
+    const int64_t col = (int64_t)tile * 32 + 8 * g, left = a.n - col;
+    if constexpr (KW == 1) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int64_t row = m0 + 16 * i + r;
+        const float v[8] = {acc[i][0][0], acc[i][0][1], acc[i][0][2], acc[i][0][3], acc[i][1][0], acc[i][1][1], acc[i][1][2], acc[i][1][3]};
+        if (row < a.m && left > 0) store8<T>(a.out, row * a.stride_out + col, left < 8 ? (int)left : 8, v);
+      }
+    } else {
+      float* mine = sums + wave * (TM * 8 * 64) + lane;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mine[(i * 8 + e) * 64] = acc[i][e >> 2][e & 3];
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+      for (int i = kw; i < TM; i += KW) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = 0.0f;
+#pragma unroll
+          for (int z = 0; z < KW; ++z) v[e] += sums[(nw * KW + z) * (TM * 8 * 64) + (i * 8 + e) * 64 + lane];
+        }
+        const int64_t row = m0 + 16 * i + r;
+        if (row < a.m && left > 0) store8<T>(a.out, row * a.stride_out + col, left < 8 ? (int)left : 8, v);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+      __builtin_amdgcn_s_barrier();   // before the next round's sums
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0);   // nothing may land in LDS after the workgroup ends
+}
+
+template <typename T, int XF, int TM, int KW, int KS>
+const char* launch_stream(const ns_mx_linear_args& a, int per_cu, hipStream_t stream) {
+  constexpr int NW = 8 / KW;
+  const int64_t wanted = ((a.n + 31) / 32 + NW - 1) / NW, along = (a.m + 16 * TM - 1) / (16 * TM);
+  const int64_t blocks_n = wanted < 256 * per_cu ? wanted : 256 * per_cu;
+  hipLaunchKernelGGL((stream_kernel<T, XF, TM, KW, KS>), dim3((unsigned)(blocks_n * along)), dim3(512), 0, stream, a, (int)blocks_n);
+  return nullptr;
+}
+
+// ---- tiles through LDS ------------------------------------------------------------------------------------------
 
 // A workgroup computes BM rows of x by BN rows of the weight, its WM x WN waves 16 TI by 16 TJ each.  Stages of 128
 // columns go to LDS by direct loads, two stages ahead, in a ring of three: at stage t a wave waits for its own share of
@@ -289,8 +465,15 @@ template <typename T, int XF, int BM, int BN, int WM, int WN> const char* launch
 
 template <typename T, int XF> const char* launch_linear_t(const ns_mx_linear_args& a, hipStream_t stream) {
   if (a.m > 64) return launch_tile<T, XF, 256, 256, 4, 2>(a, stream);
-  hipLaunchKernelGGL((linear_kernel<T, XF>), dim3((unsigned)((a.n + 63) / 64), (unsigned)((a.m + 15) / 16)), dim3(256), 0, stream, a);
-  return nullptr;
+  const int64_t tiles = (a.n + 31) / 32;
+  if (tiles >= 2048) {
+    if (a.m <= 16) return launch_stream<T, XF, 1, 1, 16>(a, 2, stream);
+    if (a.m <= 32) return launch_stream<T, XF, 2, 1, 8>(a, 2, stream);
+    return launch_stream<T, XF, 4, 1, 8>(a, 1, stream);
+  }
+  if (tiles >= 1024) return launch_stream<T, XF, 1, 2, 16>(a, 1, stream);
+  if (tiles >= 512) return launch_stream<T, XF, 1, 4, 16>(a, 1, stream);
+  return launch_stream<T, XF, 1, 8, 32>(a, 1, stream);
 }
 template <typename T> const char* launch_linear_x(const ns_mx_linear_args& a, hipStream_t stream) {
   return a.x.format == NS_MX_FP8 ? launch_linear_t<T, NS_MX_FP8>(a, stream) : launch_linear_t<T, NS_MX_FP4>(a, stream);
