@@ -11,9 +11,20 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+#include <utility>
+
 #include "ns_mx.h"
 
 namespace ns_mx {
+
+template <typename F, int... I> __device__ __forceinline__ void unrolled_over(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+// f(0), f(1) .. f(N - 1) with the number known to the compiler
+template <int N, typename F> __device__ __forceinline__ void unrolled(F&& f) {
+  unrolled_over(f, std::make_integer_sequence<int, N>{});
+}
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -119,68 +130,52 @@ __device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, unsigned cha
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)dst, 4, voff, soff, 0, 0);
 }
 
-// ---- few rows: the weight streamed through registers ------------------------------------------------------------
+// ---- few rows, few outputs: columns split over the waves ---------------------------------------------------------
 
 // vmcnt(n) alone
 #define NS_MX_VMCNT(n) (((n) & 15) | (7 << 4) | (15 << 8) | (((n) >> 4) << 14))
 
-// A workgroup of eight waves computes 16 TM rows of x by 32 outputs for each of its 8 / KW waves side by side, and goes on
-// to further outputs; KW waves share one set of outputs, their columns dealt out in groups of 512 (four stages of 128).
-// The weight goes from memory into the operand registers of the one wave that uses it: a stage's registers are refilled
-// with the wave's next group as soon as its products are issued, whatever output it is of, so that 8 KB stay in flight per
-// wave.  x lies in LDS, in two halves of KS stages: where its columns fit they stay there and the waves run on their own;
-// else the halves take turns, one filled by direct loads while the other is used, with a barrier for each.  Sums of KW
-// waves meet in LDS and are added in the waves' order.
+// The weight's rows go to the instruction in an order that leaves a lane with 8 consecutive outputs: of a pair of its
+// 16-row operands, row 8 a + 4 p + e is row 4 a + e of operand p.
 //
-// LDS rows are the stage's codes of a row of x: 8 (8-bit) or 4 pieces of 16 bytes, piece c of row r at c ^ f(r), so that 16
-// lanes that read one piece of 16 rows, and either 8 of them, meet every bank once: f = (r & 7) ^ (r >> 3 & 1) for 8
-// pieces, (r >> 1 & 3) ^ (r >> 3 & 1) for 4.  The weight's rows go to the instruction in an order that leaves a lane with 8
-// consecutive outputs: of a pair of its 16-row operands, row 8 a + 4 p + e is row 4 a + e of operand p.
+// LDS rows are a stage's codes of a matrix row, pieces of 16 bytes.  Piece c of x's row r lies at c ^ f(r), so that the lanes of
+// a read that the banks serve together meet each bank once.
 template <int PIECES> __device__ __forceinline__ int x_swizzle(int row) {
-  return PIECES == 8 ? (row & 7) ^ (row >> 3 & 1) : (row >> 1 & 3) ^ (row >> 3 & 1);
+  return PIECES == 16 ? row & 15 : PIECES == 8 ? (row & 7) ^ (row >> 3 & 1) : (row >> 1 & 3) ^ (row >> 3 & 1);
 }
 
-template <int XF, int TM, int KS> struct Stream {
-  static constexpr int XP = XF == NS_MX_FP8 ? 8 : 4;
-  static constexpr int XSTEP = 16 * TM * XP * 16;                  // bytes of a stage's codes
-  static constexpr int XB = KS * XSTEP, SB = KS * 16 * TM * 4;     // of a half's codes and scales
-  static constexpr int FILLS = XB / 1024 / 8;                      // 16-byte direct loads of a thread
-  static_assert(FILLS * 8192 == XB, "tiling");
-};
+// A workgroup of eight waves computes 16 rows of x by 32 outputs.  The columns are dealt out to the waves in groups of U stages
+// of 128; x's of KS stages at a time lie in LDS, the weight goes from memory into the operand registers of the one wave
+// that uses it, a stage's registers refilled with the wave's next group as soon as its products are issued.  The waves' sums
+// meet in LDS and are added in their order.
+constexpr int kFew = 8;
 
-template <typename T, int XF, int TM, int KW, int KS>
-__global__ __launch_bounds__(512, TM < 4 ? 4 : 2) void stream_kernel(const ns_mx_linear_args a, int blocks_n) {
-  using C = Stream<XF, TM, KS>;
-  constexpr int XP = C::XP, NW = 8 / KW, GROUPS = KS / 4;
-  static_assert(GROUPS % KW == 0, "tiling");
-  __shared__ __attribute__((aligned(16))) unsigned char s0[C::XB + C::SB], s1[C::XB + C::SB];
-  __shared__ float sums[KW > 1 ? 8 * TM * 8 * 64 : 1];
+template <typename T, int XF, int U, int KS>
+__global__ __launch_bounds__(64 * kFew) void few_kernel(const ns_mx_linear_args a) {
+  constexpr int XP = XF == NS_MX_FP8 ? 8 : 4, STEP = 16 * XP * 16, FILLS = KS * STEP / 1024 / kFew;
+  static_assert(FILLS * 1024 * kFew == KS * STEP && KS % (U * kFew) == 0, "tiling");
+  __shared__ __attribute__((aligned(16))) unsigned char xs[KS * STEP], sc[KS * 64];
+  __shared__ float sums[kFew * 8 * 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
-  const int kw = wave % KW, nw = wave / KW;
-  const int64_t m0 = (int64_t)(blockIdx.x / blocks_n) * (16 * TM);
-  const int mrows = (int)min((int64_t)(16 * TM), a.m - m0), xw = XF == NS_MX_FP8 ? a.k : a.k / 2;
-  const __amdgpu_buffer_rsrc_t xr = rows_buffer(a.x.codes, m0, a.x.stride_codes, mrows, xw);
-  const __amdgpu_buffer_rsrc_t xsr = rows_buffer(a.x.scales, m0, a.x.stride_scales, mrows, a.k / 32);
-  const int nst = a.k / 128, ng = (nst + 3) / 4, nc = (nst + KS - 1) / KS;
-  const bool resident = nc <= 2;
-
-  const auto fill = [&](int c, unsigned char* to) {
-    const int base = c * KS;
+  const int64_t n0 = (int64_t)blockIdx.x * 32;
+  const int nrows = (int)min((int64_t)32, a.n - n0), xw = XF == NS_MX_FP8 ? a.k : a.k / 2;
+  const __amdgpu_buffer_rsrc_t xr = rows_buffer(a.x.codes, 0, a.x.stride_codes, (int)a.m, xw);
+  const __amdgpu_buffer_rsrc_t xsr = rows_buffer(a.x.scales, 0, a.x.stride_scales, (int)a.m, a.k / 32);
+  const __amdgpu_buffer_rsrc_t wr = rows_buffer(a.weight.codes, n0, a.weight.stride_codes, nrows, a.k / 2);
+  const __amdgpu_buffer_rsrc_t wsr = rows_buffer(a.weight.scales, n0, a.weight.stride_scales, nrows, a.k / 32);
+  const int nst = a.k / 128, ng = (nst + U - 1) / U;
+  const auto fill = [&](int base) {   // stages past the last are it again
 #pragma unroll
-    for (int j = 0; j < C::FILLS; ++j) {
-      const int at = (j * 8 + wave) * 64 + lane, step = at / (16 * TM * XP), row = at / XP % (16 * TM), p = at % XP;
-      const int st = min(base + step, nst - 1);
-      load_lds16(xr, to + (j * 8 + wave) * 1024,
+    for (int j = 0; j < FILLS; ++j) {
+      const int at = (j * kFew + wave) * 64 + lane, row = at / XP % 16, p = at % XP, st = min(base + at / (16 * XP), nst - 1);
+      load_lds16(xr, xs + (j * kFew + wave) * 1024,
                  (uint32_t)(row * a.x.stride_codes + st * (XP * 16) + 16 * (p ^ x_swizzle<XP>(row))), 0);
     }
-    for (int j = wave; j < KS * TM / 4; j += 8) {
-      const int at = j * 64 + lane, step = at / (16 * TM), row = at % (16 * TM), st = min(base + step, nst - 1);
-      load_lds4(xsr, to + C::XB + j * 256, (uint32_t)(row * a.x.stride_scales + st * 4), 0);
+    for (int j = wave; j < KS / 4; j += kFew) {
+      const int at = j * 64 + lane, st = min(base + at / 16, nst - 1);
+      load_lds4(xsr, sc + j * 256, (uint32_t)(at % 16 * a.x.stride_scales + st * 4), 0);
     }
   };
-
-  const int tiles = (int)((a.n + 31) / 32), step_tiles = blocks_n * NW;
-  int tile = (int)(blockIdx.x % blocks_n) * NW + nw;
   uint32_t wo[2], wso[2];
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
@@ -188,257 +183,242 @@ __global__ __launch_bounds__(512, TM < 4 ? 4 : 2) void stream_kernel(const ns_mx
     wo[p] = (uint32_t)(row * a.weight.stride_codes + 16 * g);
     wso[p] = (uint32_t)(row * a.weight.stride_scales);
   }
-  u32x4 w[4][2], scale[2], next[2];
-  __amdgpu_buffer_rsrc_t wr, wsr;
-  const auto aim = [&](int t) {   // at a set of outputs; past the last: at nothing, which reads as zeros
-    const int64_t n0 = (int64_t)t * 32;
-    const int rows = t < tiles ? (int)min((int64_t)32, a.n - n0) : 0;
-    wr = rsrc(static_cast<const unsigned char*>(a.weight.codes) + (rows ? n0 : 0) * a.weight.stride_codes,
-              rows ? (uint32_t)((rows - 1) * a.weight.stride_codes + a.k / 2) : 0u);
-    wsr = rsrc(a.weight.scales + (rows ? n0 : 0) * a.weight.stride_scales,
-               rows ? (uint32_t)((rows - 1) * a.weight.stride_scales + a.k / 32) : 0u);
+  // a row's scales of a group are 4 U bytes; a group past the last is read behind the buffers' ends, where nothing is
+  u32x4 w[U][2], scale[2], next[2];
+  const auto load_scale = [&](u32x4 (&to)[2], int q) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) to[p] = load16(wsr, wso[p] | (q < ng ? 0u : 1u << 31), q * (4 * U));
   };
   const auto load_stage = [&](int s, int q) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) w[s][p] = load16(wr, wo[p] + 64 * s, q * 256);
+    for (int p = 0; p < 2; ++p) w[s][p] = load16(wr, (wo[p] + 64 * s) | (q < ng ? 0u : 1u << 31), q * (64 * U));
   };
-  f32x4 acc[TM][2];
-  const int xf = x_swizzle<XP>(r);
-  const int x_at = r * (XP * 16) + 16 * (g ^ xf), x_at2 = r * (XP * 16) + 16 * ((4 + g) ^ xf);
-  const int sx_at = C::XB + r * 4 + g;
-
-  // the products of group q, and the loads of the group that this wave takes next
-  const auto group = [&](int q, const unsigned char* from) {
-    const bool here = q + KW < ng;
-    const int then = here ? q + KW : kw;
-    if (!here) aim(tile + step_tiles);
+  f32x4 acc[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+  const int f = x_swizzle<XP>(r), at0 = r * (XP * 16) + 16 * (g ^ f), at1 = r * (XP * 16) + 16 * ((4 + g) ^ f);
+  int q = wave;
+  for (int base = 0; base < nst; base += KS) {
+    if (base > 0) __syncthreads();
+    fill(base);
+    if (base == 0) {
+      load_scale(scale, q);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) next[p] = load16(wsr, wso[p], then * 16);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if (4 * q + s < nst) {
-        const int st = (4 * q + s) % KS;
-        const unsigned char *xs = from + st * C::XSTEP + x_at, *xs2 = from + st * C::XSTEP + x_at2, *sx = from + st * (16 * TM * 4) + sx_at;
-        const int sw[2] = {(int)(scale[0][s] >> (8 * g)), (int)(scale[1][s] >> (8 * g))};
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          u32x4 x[2];
-          x[0] = *reinterpret_cast<const u32x4*>(xs + i * (XP * 256));
-          if constexpr (XP == 8) x[1] = *reinterpret_cast<const u32x4*>(xs2 + i * (XP * 256));
-          const int f = sx[i * 64];
-#pragma unroll
-          for (int p = 0; p < 2; ++p) acc[i][p] = products<XF>(w[s][p], x, sw[p], f, acc[i][p]);
-        }
-      }
-      load_stage(s, then);
-    }
-    scale[0] = next[0];
-    scale[1] = next[1];
-  };
-
-  fill(0, s0);
-  if (resident && nc > 1) fill(1, s1);
-  aim(kw < ng ? tile : tiles);
-  scale[0] = load16(wsr, wso[0], kw * 16);
-  scale[1] = load16(wsr, wso[1], kw * 16);
-#pragma unroll
-  for (int s = 0; s < 4; ++s) load_stage(s, kw);
-  bool started = true;    // whether a group's ten loads are newer than the last fill's
-  int half = 0;
-  const auto chunk = [&](int c, unsigned char* from, unsigned char* other, bool wait, bool more) {
-    if (wait) {
-      if (started) __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(10));
-      else __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(0));
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-      if (more) {
-        fill(c + 1 < nc ? c + 1 : 0, other);
-        started = false;
-      }
-    }
-#pragma unroll 1
-    for (int j = 0; j < GROUPS / KW; ++j) {
-      const int q = c * GROUPS + kw + KW * j;
-      if (q < ng) {
-        group(q, from);
-        started = true;
-      }
-    }
-  };
-  const int rounds = (tiles - (tile - nw) + step_tiles - 1) / step_tiles;   // the same for every wave
-  for (int round = 0; round < rounds; ++round, tile += step_tiles) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i) acc[i][0] = acc[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c = 0; c < nc; ++c) {
-      const bool wait = !resident || (round == 0 && c == 0), more = !resident && (c + 1 < nc || round + 1 < rounds);
-      if (half == 0) chunk(c, s0, s1, wait, more);
-      else chunk(c, s1, s0, wait, more);
-      half = nc > 1 ? half ^ 1 : 0;
-    }
-    if (resident) half = 0;
-    const int64_t col = (int64_t)tile * 32 + 8 * g, left = a.n - col;
-    if constexpr (KW == 1) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int64_t row = m0 + 16 * i + r;
-        const float v[8] = {acc[i][0][0], acc[i][0][1], acc[i][0][2], acc[i][0][3], acc[i][1][0], acc[i][1][1], acc[i][1][2], acc[i][1][3]};
-        if (row < a.m && left > 0) store8<T>(a.out, row * a.stride_out + col, left < 8 ? (int)left : 8, v);
-      }
+      for (int s = 0; s < U; ++s) load_stage(s, q);
+      __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(2 + 2 * U));   // x is there, the weight may be on its way
     } else {
-      float* mine = sums + wave * (TM * 8 * 64) + lane;
+      __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(0));
+    }
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    for (; q < ng && q * U < base + KS; q += kFew) {
+      load_scale(next, q + kFew);
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int s = 0; s < U; ++s) {
+        if (U * q + s < nst) {
+          const int st = U * q + s - base;
+          u32x4 x[2];
+          x[0] = *reinterpret_cast<const u32x4*>(xs + st * STEP + at0);
+          if constexpr (XP == 8) x[1] = *reinterpret_cast<const u32x4*>(xs + st * STEP + at1);
+          const int sx = sc[st * 64 + r * 4 + g];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mine[(i * 8 + e) * 64] = acc[i][e >> 2][e & 3];
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-      for (int i = kw; i < TM; i += KW) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = 0.0f;
-#pragma unroll
-          for (int z = 0; z < KW; ++z) v[e] += sums[(nw * KW + z) * (TM * 8 * 64) + (i * 8 + e) * 64 + lane];
+          for (int p = 0; p < 2; ++p) acc[p] = products<XF>(w[s][p], x, (int)(scale[p][s] >> (8 * g)), sx, acc[p]);
         }
-        const int64_t row = m0 + 16 * i + r;
-        if (row < a.m && left > 0) store8<T>(a.out, row * a.stride_out + col, left < 8 ? (int)left : 8, v);
+        load_stage(s, q + kFew);
       }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-      __builtin_amdgcn_s_barrier();   // before the next round's sums
+      scale[0] = next[0];
+      scale[1] = next[1];
     }
   }
-  __builtin_amdgcn_s_waitcnt(0);   // nothing may land in LDS after the workgroup ends
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sums[(wave * 8 + e) * 64 + lane] = acc[e >> 2][e & 3];
+  __syncthreads();
+  // wave e adds the waves' e-th sums; the results change places for whole rows
+  float v = 0.0f;
+#pragma unroll
+  for (int z = 0; z < kFew; ++z) v += sums[(z * 8 + wave) * 64 + lane];
+  __syncthreads();
+  sums[(g * 8 + wave) * 16 + r] = v;   // output 8 g + e of row r
+  __syncthreads();
+  const int col = tid & 31, row = tid >> 5;
+  if (row < a.m && n0 + col < a.n) static_cast<T*>(a.out)[row * a.stride_out + n0 + col] = narrow<T>(sums[col * 16 + row]);
 }
 
-template <typename T, int XF, int TM, int KW, int KS>
-const char* launch_stream(const ns_mx_linear_args& a, int per_cu, hipStream_t stream) {
-  constexpr int NW = 8 / KW;
-  const int64_t wanted = ((a.n + 31) / 32 + NW - 1) / NW, along = (a.m + 16 * TM - 1) / (16 * TM);
-  const int64_t blocks_n = wanted < 256 * per_cu ? wanted : 256 * per_cu;
-  hipLaunchKernelGGL((stream_kernel<T, XF, TM, KW, KS>), dim3((unsigned)(blocks_n * along)), dim3(512), 0, stream, a, (int)blocks_n);
+template <typename T, int XF> const char* launch_few(const ns_mx_linear_args& a, hipStream_t stream) {
+  // groups of 256 columns give all eight waves something to do from 2048 columns on; longer rows take fewer loads in 512
+  const auto kernel = a.k <= 2048 ? few_kernel<T, XF, 2, 16> : few_kernel<T, XF, 4, 64>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((a.n + 31) / 32)), dim3(64 * kFew), 0, stream, a);
   return nullptr;
 }
 
 // ---- tiles through LDS ------------------------------------------------------------------------------------------
 
-// A workgroup computes BM rows of x by BN rows of the weight, its WM x WN waves 16 TI by 16 TJ each.  Stages of 128
-// columns go to LDS by direct loads, two stages ahead, in a ring of three: at stage t a wave waits for its own share of
-// stage t, the barrier makes everyone's visible and says that everyone is past stage t - 1, whose place stage t + 2 takes.
-// The three places are three arrays and the loop is unrolled by three: the compiler sees that a stage's reads touch none
-// that a direct load is filling, and waits for none of those.
+// A workgroup computes BM rows of x by BN rows of the weight, its WM x WN waves 16 TI by 16 TJ each.  Stages of BK columns
+// go to LDS by direct loads, P - 1 stages ahead, in a ring of P places: at stage t a wave waits for its own share of stage t,
+// the barrier makes everyone's visible and says that everyone is past stage t - 1, whose place stage t + P - 1 takes.  Scales
+// come for SP stages at once, one such group ahead, into two places of their own: a row's 4 bytes for 128 columns are a
+// sliver of a 128-byte line that is fetched again every time.  Every place is an array and the loop is unrolled until all
+// recur: the compiler sees that a stage's reads touch none that a direct load is filling, and waits for none of those.
 //
-// LDS rows are the stage's codes of a matrix row: 8 (8-bit) or 4 pieces of 16 bytes.  Piece c of row r lies at c ^ f(r), so
-// that 16 lanes that read one piece of 16 rows, and either 8 of them, meet every bank once: f = (r & 7) ^ (r >> 3 & 1) for
-// 8 pieces, and for the weight's 4 f = (r >> 3 & 3) ^ (r & 2).  The weight's rows go to the instruction in an order that leaves
-// a lane with 8 consecutive outputs: of a pair of its 16-row operands, row 8 a + 4 p + e is row 4 a + e of operand p.
-template <typename T, int XF, int BM, int BN, int WM, int WN>
-struct Tile {
+// LDS rows are the stage's codes of a matrix row, pieces of 16 bytes.  Piece c of row r lies at c ^ f(r), so that 16 lanes that
+// read one piece of 16 rows, and either 8 of them, meet every bank once; x's 16 rows follow each other, the weight's go to
+// the instruction in the order that leaves a lane with 8 consecutive outputs (see above).
+template <int PIECES> __device__ __forceinline__ int w_swizzle(int row) {
+  return PIECES == 8 ? ((row >> 3 & 3) * 2 + (row >> 1 & 1)) ^ (row & 1) * 4 : (row >> 3 & 3) ^ (row & 2);
+}
+
+constexpr int lcm(int a, int b) {
+  int x = a;
+  while (x % b != 0) x += a;
+  return x;
+}
+
+template <int XF, int BM, int BN, int WM, int WN, int BK, int P, int SP> struct Tile {
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
-  static constexpr int TI = BM / WM / 16, TJ = BN / WN / 16;
-  static constexpr int XP = XF == NS_MX_FP8 ? 8 : 4;            // pieces of an x row in a stage
-  static constexpr int XB = BM * XP * 16, WB = BN * 4 * 16;     // bytes of a stage
-  static constexpr int XL = XB / 1024 / WAVES, WL = WB / 1024 / WAVES, SL = (BM + BN + THREADS - 1) / THREADS;
-  static constexpr int SB = SL * THREADS * 4;                   // scales: 4 bytes of every row
-  static constexpr int BYTES = XB + WB + SB;
+  static constexpr int TI = BM / WM / 16, TJ = BN / WN / 16, SUB = BK / 128;
+  static constexpr int XP = SUB * (XF == NS_MX_FP8 ? 8 : 4), WP = SUB * 4;   // pieces of a row in a stage
+  static constexpr int XB = BM * XP * 16, WB = BN * WP * 16, BYTES = XB + WB;
+  static constexpr int XL = XB / 1024 / WAVES, WL = WB / 1024 / WAVES;   // direct loads of a wave
+  static constexpr int PER_ROW = SP * SUB * 4, PARTS = (PER_ROW + 15) / 16;   // scale bytes of a group, loads of 16 for them
+  static constexpr int SR = (BM + BN + THREADS - 1) / THREADS, SL = SR * PARTS;
+  static constexpr int SB = SL * THREADS * 16;
+  static constexpr int UNROLL = lcm(P, 2 * SP);
+  // loads of a wave that are newer than stage t's when stage t is waited for
+  static constexpr int newer(int t) {
+    int n = (P - 2) * (XL + WL);
+    for (int i = t - P + 1; i < t; ++i) n += ((i % SP) + SP) % SP == 0 ? SL : 0;
+    return n;
+  }
   static_assert(XL * 1024 * WAVES == XB && WL * 1024 * WAVES == WB && TJ % 2 == 0 && BM % 64 == 0 && BN % 64 == 0, "tiling");
+  static_assert(SP >= P && P >= 2 && P <= 4, "a group of scales is older than the stages in flight");
+  static_assert(P * BYTES + 2 * SB <= 160 * 1024 && newer(0) + SL < 63, "LDS, counter");
 };
 
-template <typename T, int XF, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linear_args a) {
-  using C = Tile<T, XF, BM, BN, WM, WN>;
-  constexpr int TI = C::TI, TJ = C::TJ, XP = C::XP;
-  __shared__ __attribute__((aligned(16))) unsigned char s0[C::BYTES], s1[C::BYTES], s2[C::BYTES];
+template <typename T, int XF, int BM, int BN, int WM, int WN, int BK, int P, int SP>
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linear_args a, int gm) {
+  using C = Tile<XF, BM, BN, WM, WN, BK, P, SP>;
+  constexpr int TI = C::TI, TJ = C::TJ, XP = C::XP, WP = C::WP, SUB = C::SUB;
+  __shared__ __attribute__((aligned(16))) unsigned char s0[C::BYTES], s1[C::BYTES], s2[P > 2 ? C::BYTES : 16], s3[P > 3 ? C::BYTES : 16];
+  __shared__ __attribute__((aligned(16))) unsigned char c0[C::SB], c1[C::SB];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int nx = (int)((a.m + BM - 1) / BM);
-  const int64_t m0 = (int64_t)(blockIdx.x % nx) * BM, n0 = (int64_t)(blockIdx.x / nx) * BN;
+  const int nx = (int)((a.m + BM - 1) / BM), ny = (int)((a.n + BN - 1) / BN);
+  const int eighth = gridDim.x >> 3, xcd = blockIdx.x & 7;
+  const int at0 = xcd * eighth + min(xcd, (int)(gridDim.x & 7)) + (int)(blockIdx.x >> 3);
+  const int band = at0 / (gm * ny), in = at0 - band * gm * ny, high = min(gm, nx - band * gm);
+  const int64_t m0 = (int64_t)(band * gm + in % high) * BM, n0 = (int64_t)(in / high) * BN;
   const int mrows = (int)min((int64_t)BM, a.m - m0), nrows = (int)min((int64_t)BN, a.n - n0);
   // rows past the ends lie behind the buffers' ends and read as zeros
   const __amdgpu_buffer_rsrc_t xr = rows_buffer(a.x.codes, m0, a.x.stride_codes, mrows, XF == NS_MX_FP8 ? a.k : a.k / 2);
   const __amdgpu_buffer_rsrc_t wr = rows_buffer(a.weight.codes, n0, a.weight.stride_codes, nrows, a.k / 2);
   const __amdgpu_buffer_rsrc_t xsr = rows_buffer(a.x.scales, m0, a.x.stride_scales, mrows, a.k / 32);
   const __amdgpu_buffer_rsrc_t wsr = rows_buffer(a.weight.scales, n0, a.weight.stride_scales, nrows, a.k / 32);
-  uint32_t xo[C::XL], wo[C::WL], so[C::SL];
+  uint32_t xo[C::XL], wo[C::WL], so[C::SR];
 #pragma unroll
   for (int j = 0; j < C::XL; ++j) {
     const int at = j * C::THREADS + tid, row = at / XP, c = at % XP;
-    const int f = XP == 8 ? (row & 7) ^ (row >> 3 & 1) : (row >> 1 & 3) ^ (row >> 3 & 1);
-    xo[j] = (uint32_t)(row * a.x.stride_codes + 16 * (c ^ f));
+    xo[j] = (uint32_t)(row * a.x.stride_codes + 16 * (c ^ x_swizzle<XP>(row)));
   }
 #pragma unroll
   for (int j = 0; j < C::WL; ++j) {
-    const int at = j * C::THREADS + tid, row = at / 4, c = at % 4;
-    wo[j] = (uint32_t)(row * a.weight.stride_codes + 16 * (c ^ ((row >> 3 & 3) ^ (row & 2))));
+    const int at = j * C::THREADS + tid, row = at / WP, c = at % WP;
+    wo[j] = (uint32_t)(row * a.weight.stride_codes + 16 * (c ^ w_swizzle<WP>(row)));
   }
 #pragma unroll
-  for (int j = 0; j < C::SL; ++j) {
+  for (int j = 0; j < C::SR; ++j) {
     const int row = j * C::THREADS + tid;
     so[j] = (uint32_t)(row < BM ? row * a.x.stride_scales : row < BM + BN ? (row - BM) * a.weight.stride_scales : 0);
   }
-  const int nst = a.k / 128;
+  const int n128 = a.k / 128, nst = (n128 + SUB - 1) / SUB;
   const auto load = [&](int stage, unsigned char* to) {   // stages past the last are it again
-    const int st = stage < nst ? stage : nst - 1;
+    const int st = min(stage, nst - 1);
 #pragma unroll
-    for (int j = 0; j < C::XL; ++j)
-      load_lds16(xr, to + (j * C::WAVES + wave) * 1024, xo[j], st * XP * 16);
+    for (int j = 0; j < C::XL; ++j) load_lds16(xr, to + (j * C::WAVES + wave) * 1024, xo[j], st * XP * 16);
 #pragma unroll
-    for (int j = 0; j < C::WL; ++j)
-      load_lds16(wr, to + C::XB + (j * C::WAVES + wave) * 1024, wo[j], st * 64);
+    for (int j = 0; j < C::WL; ++j) load_lds16(wr, to + C::XB + (j * C::WAVES + wave) * 1024, wo[j], st * WP * 16);
+  };
+  const auto load_scales = [&](int group, unsigned char* to) {   // of stages SP group .. + SP - 1
+    const int st = min(group, (nst - 1) / SP) * C::PER_ROW;
 #pragma unroll
-    for (int j = 0; j < C::SL; ++j)
-      load_lds4((j * C::WAVES + wave) * 64 < BM ? xsr : wsr, to + C::XB + C::WB + (j * C::WAVES + wave) * 256, so[j], st * 4);
+    for (int q = 0; q < C::PARTS; ++q)
+#pragma unroll
+      for (int j = 0; j < C::SR; ++j) {
+        const __amdgpu_buffer_rsrc_t from = (j * C::WAVES + wave) * 64 < BM ? xsr : wsr;
+        load_lds16(from, to + ((q * C::SR + j) * C::WAVES + wave) * 1024, so[j], st + 16 * q);
+      }
   };
   const int wm = wave % WM, wn = wave / WM;
   const int x_row = wm * (16 * TI) + r;                              // of operand 0; operand i: 16 i more
   const int w_row = wn * (16 * TJ) + 8 * (r >> 2) + (r & 3);         // of operand 0; operand 2 q + p: 32 q + 4 p more
-  const int xf = XP == 8 ? (x_row & 7) ^ (x_row >> 3 & 1) : (x_row >> 1 & 3) ^ (x_row >> 3 & 1);
-  const int wf = (w_row >> 3 & 3) ^ (w_row & 2);
-  const int x_at = x_row * (XP * 16) + 16 * (g ^ xf), x_at2 = x_row * (XP * 16) + 16 * ((4 + g) ^ xf);
-  const int w_at = C::XB + w_row * 64 + 16 * (g ^ wf);
-  const int sx_at = C::XB + C::WB + x_row * 4 + g, sw_at = C::XB + C::WB + (BM + w_row) * 4 + g;
+  const int x_at = x_row * (XP * 16) + 16 * (g ^ x_swizzle<XP>(x_row));
+  const int w_at = w_row * (WP * 16) + 16 * (g ^ w_swizzle<WP>(w_row));
+  const int sx_at = x_row * 16 + g, sw_at = (BM + w_row) * 16 + g;
   f32x4 acc[TI][TJ];
 #pragma unroll
   for (int i = 0; i < TI; ++i)
 #pragma unroll
     for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr int LOADS = C::XL + C::WL + C::SL;
-  constexpr int WAIT = (LOADS & 15) | (7 << 4) | (15 << 8) | ((LOADS >> 4) << 14);   // vmcnt(LOADS) alone
-  const auto stage = [&](int st, const unsigned char* from, unsigned char* to) {
-    __builtin_amdgcn_s_waitcnt(WAIT);
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-    load(st + 2, to);
+
+  const auto place = [&](auto at) -> unsigned char* {
+    constexpr int I = decltype(at)::value % P;
+    return I == 0 ? s0 : I == 1 ? s1 : I == 2 ? s2 : s3;
+  };
+  // issues stage st + P - 1's loads, where stage st is at position AT of the unrolled loop and no one reads stage st - 1 any more
+  const auto issue = [&](auto at, int st) {
+    constexpr int AT = decltype(at)::value;
+    load(st + P - 1, place(std::integral_constant<int, AT + P - 1>{}));
+    if constexpr (AT % SP == 0) load_scales(st / SP + 1, AT / SP % 2 == 0 ? c1 : c0);
     __builtin_amdgcn_sched_barrier(0);
-    const unsigned char *xs = from + x_at, *xs2 = from + x_at2, *ws = from + w_at, *sx0 = from + sx_at, *sw0 = from + sw_at;
+  };
+  // the products of 128 columns
+  const auto multiply = [&](auto at, auto sub) {
+    constexpr int AT = decltype(at)::value, S = decltype(sub)::value;
+    constexpr int XS = XF == NS_MX_FP8 ? 128 : 64;   // bytes of 128 columns
+    constexpr int part = (AT % SP * SUB + S) / 4, byte = (AT % SP * SUB + S) % 4 * 4;
+    const unsigned char *from = place(at), *sc = (AT / SP % 2 == 0 ? c0 : c1) + part * (C::SR * C::THREADS * 16) + byte;
+    const unsigned char *xs = from + (x_at ^ (S * XS)), *xs2 = from + (x_at ^ (S * XS + 64)), *ws = from + C::XB + (w_at ^ (S * 64));
     u32x4 w[TJ];
     int sw[TJ];
 #pragma unroll
     for (int j = 0; j < TJ; ++j) {   // f is the same for all: 32 and 4 leave its bits alone
       const int row = 32 * (j >> 1) + 4 * (j & 1);
-      w[j] = *reinterpret_cast<const u32x4*>(ws + row * 64);
-      sw[j] = sw0[row * 4];
+      w[j] = *reinterpret_cast<const u32x4*>(ws + row * (WP * 16));
+      sw[j] = sc[sw_at + row * 16];
     }
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
       u32x4 x[2];
       x[0] = *reinterpret_cast<const u32x4*>(xs + i * (XP * 256));
-      if constexpr (XP == 8) x[1] = *reinterpret_cast<const u32x4*>(xs2 + i * (XP * 256));
-      const int sx = sx0[i * 64];
+      if constexpr (XF == NS_MX_FP8) x[1] = *reinterpret_cast<const u32x4*>(xs2 + i * (XP * 256));
+      const int sx = sc[sx_at + i * 256];
 #pragma unroll
       for (int j = 0; j < TJ; ++j) acc[i][j] = products<XF>(w[j], x, sw[j], sx, acc[i][j]);
     }
   };
+  // stage st, at position AT of the unrolled loop; with TAIL the last one's columns past k are left out
+  const auto stage = [&](auto at, auto tail, int st) {
+    constexpr int AT = decltype(at)::value;
+    // the share of this stage is there, and this wave's reads of the place that is filled next are done
+    __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(C::newer(AT)) & ~(15 << 8));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    issue(at, st);
+    unrolled<SUB>([&](auto sub) {
+      constexpr int S = decltype(sub)::value;
+      if (decltype(tail)::value && S > 0 && st * SUB + S >= n128) return;
+      // the accumulators of the large tiles leave no room for the operands of two
+      if (S > 0 && TI * TJ >= 32) __builtin_amdgcn_sched_barrier(0);
+      multiply(at, sub);
+    });
+  };
+  load_scales(0, c0);
   load(0, s0);
-  load(1, s1);
+  if constexpr (P > 2) load(1, s1);
+  if constexpr (P > 3) load(2, s2);
   int st = 0;
-  for (; st + 3 <= nst; st += 3) {
-    stage(st, s0, s2);
-    stage(st + 1, s1, s0);
-    stage(st + 2, s2, s1);
-  }
-  if (st < nst) stage(st, s0, s2);
-  if (st + 1 < nst) stage(st + 1, s1, s0);
+  for (; (st + C::UNROLL) * SUB <= n128; st += C::UNROLL)
+    unrolled<C::UNROLL>([&](auto at) { stage(at, std::false_type{}, st + decltype(at)::value); });
+  unrolled<C::UNROLL>([&](auto at) {
+    if (st + decltype(at)::value < nst) stage(at, std::true_type{}, st + decltype(at)::value);
+  });
   __builtin_amdgcn_s_waitcnt(0);   // nothing may land in LDS after the workgroup ends
   // operand pair q, token r: outputs 32 q + 8 g .. + 7
 #pragma unroll
@@ -456,24 +436,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linea
   }
 }
 
-template <typename T, int XF, int BM, int BN, int WM, int WN> const char* launch_tile(const ns_mx_linear_args& a, hipStream_t stream) {
+template <typename T, int XF, int BM, int BN, int WM, int WN, int BK, int P, int SP>
+const char* launch_tile(const ns_mx_linear_args& a, hipStream_t stream) {
+  using C = Tile<XF, BM, BN, WM, WN, BK, P, SP>;
   const int64_t blocks = ((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN);
   if (blocks >= (int64_t)1 << 31) return "too many rows";
-  hipLaunchKernelGGL((tile_kernel<T, XF, BM, BN, WM, WN>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  hipLaunchKernelGGL((tile_kernel<T, XF, BM, BN, WM, WN, BK, P, SP>), dim3((unsigned)blocks), dim3(C::THREADS), 0, stream, a, 4);
   return nullptr;
 }
 
 template <typename T, int XF> const char* launch_linear_t(const ns_mx_linear_args& a, hipStream_t stream) {
-  if (a.m > 64) return launch_tile<T, XF, 256, 256, 4, 2>(a, stream);
-  const int64_t tiles = (a.n + 31) / 32;
-  if (tiles >= 2048) {
-    if (a.m <= 16) return launch_stream<T, XF, 1, 1, 16>(a, 2, stream);
-    if (a.m <= 32) return launch_stream<T, XF, 2, 1, 8>(a, 2, stream);
-    return launch_stream<T, XF, 4, 1, 8>(a, 1, stream);
+  const auto tiles = [&](int64_t bm, int64_t bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
+  constexpr int64_t kFull = 200;   // tiles that keep most of the 256 compute units busy
+  if (a.m <= 16 && a.n <= 32 * 256) return launch_few<T, XF>(a, stream);
+  if (a.m > 64) {
+    if constexpr (XF == NS_MX_FP8) {
+      if (a.m > 128 && tiles(256, 256) >= kFull) return launch_tile<T, XF, 256, 256, 4, 2, 128, 3, 3>(a, stream);
+      if (tiles(128, 256) >= kFull) return launch_tile<T, XF, 128, 256, 2, 2, 128, 2, 4>(a, stream);
+    } else {
+      if (a.m > 128 && tiles(256, 256) >= kFull) return launch_tile<T, XF, 256, 256, 4, 2, 256, 2, 2>(a, stream);
+    }
+    if (tiles(128, 128) >= kFull) return launch_tile<T, XF, 128, 128, 2, 2, 256, 2, 2>(a, stream);
   }
-  if (tiles >= 1024) return launch_stream<T, XF, 1, 2, 16>(a, 1, stream);
-  if (tiles >= 512) return launch_stream<T, XF, 1, 4, 16>(a, 1, stream);
-  return launch_stream<T, XF, 1, 8, 32>(a, 1, stream);
+  if (tiles(64, 128) >= 2 * 256) return launch_tile<T, XF, 64, 128, 2, 2, 256, 2, 2>(a, stream);
+  if (tiles(64, 128) >= kFull) return launch_tile<T, XF, 64, 128, 2, 2, 256, 3, 4>(a, stream);
+  return launch_tile<T, XF, 64, 64, 2, 2, 256, 4, 4>(a, stream);
 }
 template <typename T> const char* launch_linear_x(const ns_mx_linear_args& a, hipStream_t stream) {
   return a.x.format == NS_MX_FP8 ? launch_linear_t<T, NS_MX_FP8>(a, stream) : launch_linear_t<T, NS_MX_FP4>(a, stream);
