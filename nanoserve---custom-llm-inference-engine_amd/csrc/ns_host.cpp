@@ -7,6 +7,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
 
 #include <exception>
 #include <optional>
@@ -423,6 +424,14 @@ bool same_view(const at::Tensor& a, const at::Tensor& b) {
   return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides() && a.scalar_type() == b.scalar_type();
 }
 
+// A new tensor on the current device (which is `like`'s: the caller has made it so), of torch's allocator for it, as at::empty
+// makes it on its way through the dispatcher.
+at::Tensor fresh(const at::Tensor& like, at::IntArrayRef size, at::ScalarType type) {
+  static c10::Allocator* const allocator = at::empty({16}, like.options()).storage().allocator();
+  if (allocator == nullptr) return at::empty(size, like.options().dtype(type));
+  return at::detail::empty_generic(size, allocator, c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
+}
+
 struct Written {   // a tensor that a call writes, and one that it reads or writes
   const char* name;
   const at::Tensor* t;
@@ -506,13 +515,12 @@ struct Result {
   void make(const at::Tensor& like, int64_t n) {   // without Python's lock
     if (out != nullptr) return;
     if (format == 0) {
-      made = like.dim() == 3 ? at::empty({n, like.size(1), like.size(2)}, like.options())
-                             : at::empty({n, like.size(1)}, like.options());
+      const int64_t size[] = {n, like.size(1), like.dim() == 3 ? like.size(2) : 1};
+      made = fresh(like, at::IntArrayRef(size, like.dim()), like.scalar_type());
     } else {
-      const int64_t k = padded(like);
-      made = at::empty({n, format == NS_MX_FP4 ? k / 2 : k},
-                       like.options().dtype(format == NS_MX_FP4 ? at::kFloat4_e2m1fn_x2 : at::kFloat8_e4m3fn));
-      made_scales = at::empty({n, k / 32}, like.options().dtype(at::kFloat8_e8m0fnu));
+      const int64_t k = padded(like), codes[] = {n, format == NS_MX_FP4 ? k / 2 : k}, blocks[] = {n, k / 32};
+      made = fresh(like, codes, format == NS_MX_FP4 ? at::kFloat4_e2m1fn_x2 : at::kFloat8_e4m3fn);
+      made_scales = fresh(like, blocks, at::kFloat8_e8m0fnu);
       scales = &made_scales;
     }
     out = &made;
@@ -689,7 +697,8 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     std::optional<Unlocked> meanwhile(std::in_place);
     at::Tensor made;
     if (out == nullptr) {
-      made = at::empty({rows, cols}, codes.options().dtype(torch_type(dtype)));
+      const int64_t size[] = {rows, cols};
+      made = fresh(codes, size, torch_type(dtype));
       out = &made;
     }
     if (rows > 0 && call(&r, rows, (int32_t)cols, out->data_ptr(), out->stride(0), (int32_t)dtype,
@@ -733,7 +742,8 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     std::optional<Unlocked> meanwhile(std::in_place);
     at::Tensor made;
     if (out == nullptr) {
-      made = at::empty({s.m, s.n}, xc.options().dtype(torch_type(dtype)));
+      const int64_t size[] = {s.m, s.n};
+      made = fresh(xc, size, torch_type(dtype));
       out = &made;
     }
     if (any) {

@@ -25,7 +25,6 @@ recorded.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from typing import NamedTuple, Optional
@@ -131,18 +130,15 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     return lib
 
 
-_NO_SWITCH = contextlib.nullcontext()
-
-
 def _on(t, stream):
-    """(HIP stream handle, context) of a call on a tensor's device: its current stream, a torch stream or a raw handle (0:
-    the default stream).  Inside the context the call's results are made on that stream."""
+    """(HIP stream handle, context or None) of a call on a tensor's device: its current stream, a torch stream or a raw
+    handle (0: the default stream).  Inside the context the call's results are made on that stream."""
     dev = t.get_device() if isinstance(t, torch.Tensor) else -1
     if dev < 0:
-        return 0, _NO_SWITCH        # refused by the call
+        return 0, None        # refused by the call
     if stream is None:
-        if dev == torch.cuda.current_device():
-            return torch._C._cuda_getCurrentRawStream(dev), _NO_SWITCH
+        if dev == torch._C._cuda_getDevice():    # a CUDA tensor is there, so torch has made the device ready
+            return torch._C._cuda_getCurrentRawStream(dev), None
         s = torch.cuda.current_stream(dev)
     elif isinstance(stream, torch.cuda.Stream):
         if stream.device_index != dev:
@@ -153,6 +149,14 @@ def _on(t, stream):
     else:
         s = torch.cuda.ExternalStream(int(stream), device=dev)
     return s.cuda_stream, torch.cuda.stream(s)
+
+
+def _run(call, t, stream, *args):
+    handle, context = _on(t, stream)
+    if context is None:
+        return call(*args, handle)
+    with context:
+        return call(*args, handle)
 
 
 def _format(format):
@@ -199,9 +203,7 @@ def rms_norm_hip(x, weight, eps: float, *, residual=None, sum_out=None, rows=Non
     host, calls = _HOST
     fmt = _format(format)
     to, scales = _out(out, format)
-    handle, context = _on(x, stream)
-    with context:
-        got = host.rms_norm(*calls["rms_norm"], x, weight, eps, residual, sum_out, rows, fmt, to, scales, handle)
+    got = _run(host.rms_norm, x, stream, *calls["rms_norm"], x, weight, eps, residual, sum_out, rows, fmt, to, scales)
     return got if fmt == 0 else MxTensor(*got, x.shape[1])
 
 
@@ -215,9 +217,7 @@ def silu_mul_hip(gate, up, *, format: Optional[str] = None, out=None, stream=Non
         raise MxError("up must be a tensor")
     fmt = _format(format)
     to, scales = _out(out, format)
-    handle, context = _on(gate, stream)
-    with context:
-        got = host.gate(*calls["silu_mul"], gate, up, None, fmt, to, scales, handle)
+    got = _run(host.gate, gate, stream, *calls["silu_mul"], gate, up, None, fmt, to, scales)
     return got if fmt == 0 else MxTensor(*got, gate.shape[1])
 
 
@@ -231,9 +231,7 @@ def quantize_mx_hip(x, format: str = "mxfp4", *, rows=None, out=None, stream=Non
         raise MxError("format must be \"mxfp4\" or \"mxfp8\"")
     fmt = _format(format)
     to, scales = _out(out, format)
-    handle, context = _on(x, stream)
-    with context:
-        got = host.gate(*calls["quantize"], x, None, rows, fmt, to, scales, handle)
+    got = _run(host.gate, x, stream, *calls["quantize"], x, None, rows, fmt, to, scales)
     return MxTensor(*got, x.shape[1])
 
 
@@ -243,9 +241,8 @@ def dequantize_mx_hip(t, dtype=torch.bfloat16, *, out=None, stream=None):
         load()
     host, calls = _HOST
     codes, scales, cols = _pair(t, "t")
-    handle, context = _on(codes, stream)
-    with context:
-        return host.dequantize(*calls["dequantize"], codes, scales, -1 if cols is None else cols, _dtype(dtype), out, handle)
+    return _run(host.dequantize, codes, stream, *calls["dequantize"], codes, scales, -1 if cols is None else cols, _dtype(dtype),
+                out)
 
 
 def mx_linear_hip(x, weight, *, dtype=torch.bfloat16, out=None, stream=None):
@@ -258,9 +255,7 @@ def mx_linear_hip(x, weight, *, dtype=torch.bfloat16, out=None, stream=None):
     wc, ws, w_cols = _pair(weight, "weight")
     if x_cols is not None and w_cols is not None and x_cols != w_cols:
         raise MxError(f"x's rows of {x_cols} values do not match the weight's of {w_cols}")
-    handle, context = _on(xc, stream)
-    with context:
-        return host.linear(*calls["linear"], xc, xs, wc, ws, _dtype(dtype), out, handle)
+    return _run(host.linear, xc, stream, *calls["linear"], xc, xs, wc, ws, _dtype(dtype), out)
 
 
 def mx_tensor(codes, scales, cols: Optional[int] = None) -> MxTensor:
