@@ -65,33 +65,72 @@ template <typename T> __device__ __forceinline__ T narrow(float a) {
   if constexpr (sizeof(T) == 4) return a;
   else return T{(uint16_t)narrow2<T>(a, 0.0f)};
 }
-template <typename T> __device__ __forceinline__ float rounded(float a) { return widen<T>(narrow<T>(a)); }
+// Eight values of a row as they lie in memory.
+template <typename T> struct Words {
+  static constexpr int N = 2 * sizeof(T);
+  uint32_t w[N];
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (N == 8) v[i] = __uint_as_float(w[i]);
+      else widen2<T>(w[i], v[2 * i], v[2 * i + 1]);
+    }
+  }
+  __device__ __forceinline__ void put(const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (N == 8) w[i] = __float_as_uint(v[i]);
+      else w[i] = narrow2<T>(v[2 * i], v[2 * i + 1]);
+    }
+  }
+};
 
-template <typename T> __device__ __forceinline__ void store8(void* base, int64_t at, int left, const float (&v)[8]) {
-  T* p = static_cast<T*>(base) + at;
+// Those from p on, the ones past `left` zero.  The loads are 16 bytes wide at any alignment of the element's (the hardware takes
+// global addresses as they come), so that rows of odd widths and views cost what whole ones do.
+template <typename T> __device__ __forceinline__ Words<T> load_words(const void* base, int64_t at, int left) {
+  typedef uint32_t four __attribute__((ext_vector_type(4), aligned(2)));
+  const T* p = static_cast<const T*>(base) + at;
+  Words<T> x;
   if (left >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      typedef uint32_t words __attribute__((ext_vector_type(4), aligned(4)));
-      words a, b;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = __float_as_uint(v[i]);
-        b[i] = __float_as_uint(v[4 + i]);
-      }
-      *reinterpret_cast<words*>(p) = a;
-      *reinterpret_cast<words*>(p + 4) = b;
-    } else {
-      typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
-      words a;
+    for (int i = 0; i < Words<T>::N / 4; ++i) {
+      const four a = *(reinterpret_cast<const four*>(p + 4 * i));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = narrow2<T>(v[2 * i], v[2 * i + 1]);
-      *reinterpret_cast<words*>(p) = a;
+      for (int j = 0; j < 4; ++j) x.w[4 * i + j] = a[j];
     }
   } else {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? widen<T>(p[i]) : 0.0f;
+    x.put(v);
+  }
+  return x;
+}
+
+// With PAST the lines are marked as not read again soon: they leave the caches first.
+template <typename T, bool PAST = false> __device__ __forceinline__ void store_words(void* base, int64_t at, int left, const Words<T>& x) {
+  typedef uint32_t four __attribute__((ext_vector_type(4), aligned(2)));
+  T* p = static_cast<T*>(base) + at;
+  if (left >= 8) {
+#pragma unroll
+    for (int i = 0; i < Words<T>::N / 4; ++i) {
+      const four a = {x.w[4 * i], x.w[4 * i + 1], x.w[4 * i + 2], x.w[4 * i + 3]};
+      if constexpr (PAST) __builtin_nontemporal_store(a, reinterpret_cast<four*>(p + 4 * i));
+      else *reinterpret_cast<four*>(p + 4 * i) = a;
+    }
+  } else {
+    float v[8];
+    x.get(v);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < left) p[i] = narrow<T>(v[i]);
   }
+}
+template <typename T, bool PAST = false>
+__device__ __forceinline__ void store8(void* base, int64_t at, int left, const float (&v)[8]) {
+  Words<T> x;
+  x.put(v);
+  store_words<T, PAST>(base, at, left, x);
 }
 
 // ---- operands ---------------------------------------------------------------------------------------------------

@@ -1,10 +1,12 @@
 """Inputs and bounds of the layer operators' tests.
 
 Bounds, with u = 2^-24 (float32 rounds a result by at most u of it):
-* norm: the sum and the root are float64, the factor is rounded once (u), two products follow (2 u): 3 u of the value,
-  and 4 u leaves the float64 parts their room.
-* gated: exp within 2 u (the device library's bound is 1 ulp), 1 + e is off by at most half of that and its own u, the
-  quotient, and the two products after it: 2 + 1 + 1 + 1 + 1 + 1 = 7 u, taken as 8.  Where the exponential or a product
+* norm: the sum is float64 over values (float32) or over pairs whose sum is rounded once (16 bits: u of the sum, half of it of
+  the root), the root is float64, the factor is rounded once (u), two products follow (2 u): 3.5 u of the value, and 4 u
+  leaves the float64 parts their room.
+* gated: exp within 3 u (2^t by the instruction within 1 ulp, 2 u, and the product with what t's rounding left), 1 + e adds
+  its own u (exp's error enters the quotient e / (1 + e) less than once over), the reciprocal and its product with e u each,
+  and the two products after it: 3 + 1 + 1 + 1 + 1 + 1 = 8 u.  Where the exponential or a product
   falls below the normal numbers, 2^-149 of it is lost, times |gate up|.
 * a rounding to the type: half a unit in its last place (float32's is the last product's, counted above).
 * a result in MX rows: the value before rounding is within those bounds, so the block's exponent is one of the two ends',
