@@ -297,9 +297,14 @@ template <typename T, int XF> const char* launch_few(const ns_mx_linear_args& a,
 // sliver of a 128-byte line that is fetched again every time.  Every place is an array and the loop is unrolled until all
 // recur: the compiler sees that a stage's reads touch none that a direct load is filling, and waits for none of those.
 //
-// LDS rows are the stage's codes of a matrix row, pieces of 16 bytes.  Piece c of row r lies at c ^ f(r), so that 16 lanes that
-// read one piece of 16 rows, and either 8 of them, meet every bank once; x's 16 rows follow each other, the weight's go to
-// the instruction in the order that leaves a lane with 8 consecutive outputs (see above).
+// Eight waves (the tiles of 256 x 256) work in two halves, one wave of each on every SIMD: while one half multiplies, the
+// other reads its next operands, and a barrier changes places.  A half's loads are issued among its products, where no one
+// waits for them to be taken; the first half's of 8-bit rows, whose products take twice as long, behind its reads.
+// 4096 x 16384 x 4096 (8-bit rows): 203 us, 222 with all eight waves in step, 185 without the results' stores and 152 without
+// loads, of 112 us that the matrix units need at the rate they reach by themselves (4900 TFLOP/s).
+//
+// Pieces of 16 bytes lie in LDS as above: c ^ f(r), x's 16 rows of a read one after the other, the weight's in the order of its
+// operands.
 template <int PIECES> __device__ __forceinline__ int w_swizzle(int row) {
   return PIECES == 8 ? ((row >> 3 & 3) * 2 + (row >> 1 & 1)) ^ (row & 1) * 4 : (row >> 3 & 3) ^ (row & 2);
 }
@@ -335,6 +340,7 @@ template <typename T, int XF, int BM, int BN, int WM, int WN, int BK, int P, int
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linear_args a, int gm) {
   using C = Tile<XF, BM, BN, WM, WN, BK, P, SP>;
   constexpr int TI = C::TI, TJ = C::TJ, XP = C::XP, WP = C::WP, SUB = C::SUB;
+  constexpr bool PAIRED = C::WAVES == 8, AMONG_READS = XF == NS_MX_FP8;
   __shared__ __attribute__((aligned(16))) unsigned char s0[C::BYTES], s1[C::BYTES], s2[P > 2 ? C::BYTES : 16], s3[P > 3 ? C::BYTES : 16];
   __shared__ __attribute__((aligned(16))) unsigned char c0[C::SB], c1[C::SB];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -367,22 +373,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linea
     so[j] = (uint32_t)(row < BM ? row * a.x.stride_scales : row < BM + BN ? (row - BM) * a.weight.stride_scales : 0);
   }
   const int n128 = a.k / 128, nst = (n128 + SUB - 1) / SUB;
-  const auto load = [&](int stage, unsigned char* to) {   // stages past the last are it again
+  // direct load number I of a stage, into its place; stages past the last are it again
+  const auto load = [&](auto number, int stage, unsigned char* to) {
+    constexpr int I = decltype(number)::value;
     const int st = min(stage, nst - 1);
-#pragma unroll
-    for (int j = 0; j < C::XL; ++j) load_lds16(xr, to + (j * C::WAVES + wave) * 1024, xo[j], st * XP * 16);
-#pragma unroll
-    for (int j = 0; j < C::WL; ++j) load_lds16(wr, to + C::XB + (j * C::WAVES + wave) * 1024, wo[j], st * WP * 16);
+    if constexpr (I < C::XL) load_lds16(xr, to + (I * C::WAVES + wave) * 1024, xo[I], st * XP * 16);
+    else load_lds16(wr, to + C::XB + ((I - C::XL) * C::WAVES + wave) * 1024, wo[I - C::XL], st * WP * 16);
   };
-  const auto load_scales = [&](int group, unsigned char* to) {   // of stages SP group .. + SP - 1
-    const int st = min(group, (nst - 1) / SP) * C::PER_ROW;
-#pragma unroll
-    for (int q = 0; q < C::PARTS; ++q)
-#pragma unroll
-      for (int j = 0; j < C::SR; ++j) {
-        const __amdgpu_buffer_rsrc_t from = (j * C::WAVES + wave) * 64 < BM ? xsr : wsr;
-        load_lds16(from, to + ((q * C::SR + j) * C::WAVES + wave) * 1024, so[j], st + 16 * q);
-      }
+  // number I of the scales of stages SP group .. + SP - 1
+  const auto load_scales = [&](auto number, int group, unsigned char* to) {
+    constexpr int J = decltype(number)::value % C::SR, Q = decltype(number)::value / C::SR;
+    load_lds16((J * C::WAVES + wave) * 64 < BM ? xsr : wsr, to + ((Q * C::SR + J) * C::WAVES + wave) * 1024, so[J],
+               min(group, (nst - 1) / SP) * C::PER_ROW + 16 * Q);
   };
   const int wm = wave % WM, wn = wave / WM;
   const int x_row = wm * (16 * TI) + r;                              // of operand 0; operand i: 16 i more
@@ -400,22 +402,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linea
     constexpr int I = decltype(at)::value % P;
     return I == 0 ? s0 : I == 1 ? s1 : I == 2 ? s2 : s3;
   };
-  // issues stage st + P - 1's loads, where stage st is at position AT of the unrolled loop and no one reads stage st - 1 any more
-  const auto issue = [&](auto at, int st) {
-    constexpr int AT = decltype(at)::value;
-    load(st + P - 1, place(std::integral_constant<int, AT + P - 1>{}));
-    if constexpr (AT % SP == 0) load_scales(st / SP + 1, AT / SP % 2 == 0 ? c1 : c0);
+  // Part PART of PARTS of the loads of stage st + P - 1, where stage st is at position AT of the unrolled loop and no one reads
+  // stage st - 1 any more.
+  const auto issue = [&](auto at, auto part, auto parts, int st) {
+    constexpr int AT = decltype(at)::value, DATA = C::XL + C::WL, ALL = DATA + (AT % SP == 0 ? C::SL : 0);
+    constexpr int PER = (ALL + decltype(parts)::value - 1) / decltype(parts)::value, FIRST = decltype(part)::value * PER;
+    unrolled<PER>([&](auto i) {
+      constexpr int I = FIRST + decltype(i)::value;
+      if constexpr (I < DATA) load(std::integral_constant<int, I>{}, st + P - 1, place(std::integral_constant<int, AT + P - 1>{}));
+      else if constexpr (I < ALL) load_scales(std::integral_constant<int, I - DATA>{}, st / SP + 1, AT / SP % 2 == 0 ? c1 : c0);
+    });
     __builtin_amdgcn_sched_barrier(0);
   };
-  // the products of 128 columns
-  const auto multiply = [&](auto at, auto sub) {
+  constexpr std::integral_constant<int, 0> all{};
+  constexpr std::integral_constant<int, 1> at_once{};
+  u32x4 w[TJ], x[TI][2];
+  int sw[TJ], sx[TI];
+  // the operands of 128 columns
+  const auto read = [&](auto at, auto sub) {
     constexpr int AT = decltype(at)::value, S = decltype(sub)::value;
     constexpr int XS = XF == NS_MX_FP8 ? 128 : 64;   // bytes of 128 columns
     constexpr int part = (AT % SP * SUB + S) / 4, byte = (AT % SP * SUB + S) % 4 * 4;
     const unsigned char *from = place(at), *sc = (AT / SP % 2 == 0 ? c0 : c1) + part * (C::SR * C::THREADS * 16) + byte;
     const unsigned char *xs = from + (x_at ^ (S * XS)), *xs2 = from + (x_at ^ (S * XS + 64)), *ws = from + C::XB + (w_at ^ (S * 64));
-    u32x4 w[TJ];
-    int sw[TJ];
 #pragma unroll
     for (int j = 0; j < TJ; ++j) {   // f is the same for all: 32 and 4 leave its bits alone
       const int row = 32 * (j >> 1) + 4 * (j & 1);
@@ -424,40 +433,87 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linea
     }
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
-      u32x4 x[2];
-      x[0] = *reinterpret_cast<const u32x4*>(xs + i * (XP * 256));
-      if constexpr (XF == NS_MX_FP8) x[1] = *reinterpret_cast<const u32x4*>(xs2 + i * (XP * 256));
-      const int sx = sc[sx_at + i * 256];
-#pragma unroll
-      for (int j = 0; j < TJ; ++j) acc[i][j] = products<XF>(w[j], x, sw[j], sx, acc[i][j]);
+      x[i][0] = *reinterpret_cast<const u32x4*>(xs + i * (XP * 256));
+      if constexpr (XF == NS_MX_FP8) x[i][1] = *reinterpret_cast<const u32x4*>(xs2 + i * (XP * 256));
+      sx[i] = sc[sx_at + i * 256];
     }
   };
-  // stage st, at position AT of the unrolled loop; with TAIL the last one's columns past k are left out
-  const auto stage = [&](auto at, auto tail, int st) {
-    constexpr int AT = decltype(at)::value;
-    // the share of this stage is there, and this wave's reads of the place that is filled next are done
-    __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(C::newer(AT)) & ~(15 << 8));
+  const auto multiply = [&](auto number) {
+    constexpr int i = decltype(number)::value;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) acc[i][j] = products<XF>(w[j], x[i], sw[j], sx[i], acc[i][j]);
+  };
+  const auto meet = [&] {
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-    issue(at, st);
-    unrolled<SUB>([&](auto sub) {
-      constexpr int S = decltype(sub)::value;
-      if (decltype(tail)::value && S > 0 && st * SUB + S >= n128) return;
-      // the accumulators of the large tiles leave no room for the operands of two
-      if (S > 0 && TI * TJ >= 32) __builtin_amdgcn_sched_barrier(0);
-      multiply(at, sub);
-    });
   };
-  load_scales(0, c0);
-  load(0, s0);
-  if constexpr (P > 2) load(1, s1);
-  if constexpr (P > 3) load(2, s2);
-  int st = 0;
-  for (; (st + C::UNROLL) * SUB <= n128; st += C::UNROLL)
-    unrolled<C::UNROLL>([&](auto at) { stage(at, std::false_type{}, st + decltype(at)::value); });
-  unrolled<C::UNROLL>([&](auto at) {
-    if (st + decltype(at)::value < nst) stage(at, std::true_type{}, st + decltype(at)::value);
-  });
+  // Stage st, at position AT of the unrolled loop; with TAIL the last one's columns past k are left out.
+  const auto stage = [&](auto behind, auto at, auto tail, int st) {
+    constexpr int AT = decltype(at)::value;
+    constexpr bool TAIL = decltype(tail)::value, LATE = decltype(behind)::value;
+    if constexpr (!PAIRED) {
+      // the share of this stage is there, and this wave's reads of the place that is filled next are done
+      __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(C::newer(AT)) & ~(15 << 8));
+      meet();
+      issue(at, all, at_once, st);
+      unrolled<SUB>([&](auto sub) {
+        if (TAIL && decltype(sub)::value > 0 && st * SUB + decltype(sub)::value >= n128) return;
+        if (decltype(sub)::value > 0 && TI * TJ >= 32) __builtin_amdgcn_sched_barrier(0);
+        read(at, sub);
+        unrolled<TI>(multiply);
+      });
+    } else {
+      constexpr std::integral_constant<int, (AT + 1) % C::UNROLL> after{};
+      unrolled<SUB>([&](auto sub) {
+        constexpr int S = decltype(sub)::value;
+        const bool skip = TAIL && S > 0 && st * SUB + S >= n128;
+        if (!skip) read(at, sub);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (S == 0 && !LATE && AMONG_READS) issue(at, all, at_once, st);
+        if constexpr (S == SUB - 1 && LATE) __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(C::newer(AT + 1)) & ~(15 << 8));
+        else __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(63) & ~(15 << 8));
+        meet();
+        __builtin_amdgcn_s_setprio(1);
+        unrolled<TI>([&](auto i) {
+          if (!skip) multiply(i);
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (S == SUB - 1 && LATE) issue(after, i, std::integral_constant<int, TI>{}, st + 1);
+          if constexpr (S == 0 && !LATE && !AMONG_READS) issue(at, i, std::integral_constant<int, TI>{}, st);
+        });
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (S == SUB - 1 && !LATE) __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(C::newer(AT + 1)));
+        meet();
+      });
+    }
+  };
+  const auto run = [&](auto behind) {
+    unrolled<C::SL>([&](auto i) { load_scales(i, 0, c0); });
+    unrolled<P - 1>([&](auto p) {
+      unrolled<C::XL + C::WL>([&](auto i) { load(i, decltype(p)::value, place(p)); });
+    });
+    if constexpr (PAIRED) {
+      __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(C::newer(0)));
+      meet();
+      if constexpr (decltype(behind)::value) {
+        issue(all, all, at_once, 0);
+        meet();
+      }
+    }
+    int st = 0;
+    for (; (st + C::UNROLL) * SUB <= n128; st += C::UNROLL)
+      unrolled<C::UNROLL>([&](auto at) { stage(behind, at, std::false_type{}, st + decltype(at)::value); });
+    unrolled<C::UNROLL>([&](auto at) {
+      if (st + decltype(at)::value < nst) stage(behind, at, std::true_type{}, st + decltype(at)::value);
+    });
+    if constexpr (PAIRED && !decltype(behind)::value) meet();
+  };
+  if constexpr (PAIRED) {
+    if (wave >= C::WAVES / 2) run(std::true_type{});
+    else run(std::false_type{});
+  } else {
+    run(std::false_type{});
+  }
   __builtin_amdgcn_s_waitcnt(0);   // nothing may land in LDS after the workgroup ends
   // operand pair q, token r: outputs 32 q + 8 g .. + 7
 #pragma unroll
