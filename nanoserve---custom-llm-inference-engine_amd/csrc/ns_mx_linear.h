@@ -135,10 +135,25 @@ __device__ __forceinline__ void store8(void* base, int64_t at, int left, const f
 
 // ---- operands ---------------------------------------------------------------------------------------------------
 
-template <int XF> __device__ __forceinline__ f32x4 products(u32x4 w, const u32x4 (&x)[2], int sw, int sx, f32x4 c) {
+// The instruction adds products of eight neighbours with 13 bits below the largest one's exponent and cuts the rest off (from
+// there on float32's 24 bits).  An e4m3 code times an e2m1 code has up to 21 bits, so results of 8-bit rows are off by about
+// 2^-17 of their size: far below a 16-bit result's rounding, which takes them as they are.  Float32 results (WHOLE) take the
+// codes in two halves, those of 2 and above (the exponent's highest bit) and those below, a product each: neither spans
+// more than 13 bits, and what is added is whole.  4-bit products span 7 bits.
+template <int XF, bool WHOLE> __device__ __forceinline__ f32x4 products(u32x4 w, const u32x4 (&x)[2], int sw, int sx, f32x4 c) {
   const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
   if constexpr (XF == NS_MX_FP8) {
-    const i32x8 b = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
+    i32x8 b = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
+    if constexpr (WHOLE) {
+      i32x8 low;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t v = (uint32_t)b[i], t = v >> 6 & 0x01010101u, high = (t << 8) - t;   // 255 where a byte has bit 6
+        low[i] = (int)(v & ~high);
+        b[i] = (int)(v & high);
+      }
+      c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, low, c, 4, 0, 0, sw, 0, sx);
+    }
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, 0, sw, 0, sx);
   } else {
     const i32x8 b = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], 0, 0, 0, 0};
@@ -178,7 +193,7 @@ __device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, unsigned cha
 // 16-row operands, row 8 a + 4 p + e is row 4 a + e of operand p.
 //
 // LDS rows are a stage's codes of a matrix row, pieces of 16 bytes.  Piece c of x's row r lies at c ^ f(r), so that the lanes of
-// a read that the banks serve together meet each bank once.
+// a read spread over the banks: such a read takes 4.0 to 4.8 cycles of the 4 that its 1024 bytes need, 16 in the rows' own order.
 template <int PIECES> __device__ __forceinline__ int x_swizzle(int row) {
   return PIECES == 16 ? row & 15 : PIECES == 8 ? (row & 7) ^ (row >> 3 & 1) : (row >> 1 & 3) ^ (row >> 3 & 1);
 }
@@ -259,7 +274,7 @@ __global__ __launch_bounds__(64 * kFew) void few_kernel(const ns_mx_linear_args 
           if constexpr (XP == 8) x[1] = *reinterpret_cast<const u32x4*>(xs + st * STEP + at1);
           const int sx = sc[st * 64 + r * 4 + g];
 #pragma unroll
-          for (int p = 0; p < 2; ++p) acc[p] = products<XF>(w[s][p], x, (int)(scale[p][s] >> (8 * g)), sx, acc[p]);
+          for (int p = 0; p < 2; ++p) acc[p] = products<XF, sizeof(T) == 4>(w[s][p], x, (int)(scale[p][s] >> (8 * g)), sx, acc[p]);
         }
         load_stage(s, q + kFew);
       }
@@ -441,7 +456,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linea
   const auto multiply = [&](auto number) {
     constexpr int i = decltype(number)::value;
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) acc[i][j] = products<XF>(w[j], x[i], sw[j], sx[i], acc[i][j]);
+    for (int j = 0; j < TJ; ++j) acc[i][j] = products<XF, sizeof(T) == 4>(w[j], x[i], sw[j], sx[i], acc[i][j]);
   };
   const auto meet = [&] {
     __builtin_amdgcn_s_barrier();
@@ -540,21 +555,32 @@ const char* launch_tile(const ns_mx_linear_args& a, hipStream_t stream) {
   return nullptr;
 }
 
+// Which kernel, by sizes and types alone (times of bf16 results, 8-bit rows, in microseconds, both sides measured):
+// - up to 16 rows and 8192 outputs: few_kernel, 5.4 at 1 x 8192 x 2048 where a 64 x 64 tile takes 9; above that the tiles have
+//   workgroups enough to keep the memory busy, 38 at 64 x 128256 x 2048.
+// - the largest tile that leaves at least kFull of them, as it reads the operands from the caches least often: 4096 x 16384 x
+//   4096 takes 204 with 256 x 256 and 280 with 128 x 256; 1024 x 4096 x 4096 has 64 of the first and takes 24 with 64 x 128.
+// - 64 x 128 in two forms: two places a workgroup and two workgroups a unit where there are that many, else three places.
+// Float32 results of 8-bit rows hold two halves of x (products()): the 256 x 256 tile and the three places spill registers
+// there (489 against 425 with 128 x 256 at 4096 x 16384 x 4096, 505 against 24 at 512 x 4096 x 4096) and are left out.
 template <typename T, int XF> const char* launch_linear_t(const ns_mx_linear_args& a, hipStream_t stream) {
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
   constexpr int64_t kFull = 200;   // tiles that keep most of the 256 compute units busy
+  constexpr bool HALVES = XF == NS_MX_FP8 && sizeof(T) == 4;
   if (a.m <= 16 && a.n <= 32 * 256) return launch_few<T, XF>(a, stream);
   if (a.m > 64) {
     if constexpr (XF == NS_MX_FP8) {
-      if (a.m > 128 && tiles(256, 256) >= kFull) return launch_tile<T, XF, 256, 256, 4, 2, 128, 3, 3>(a, stream);
+      if constexpr (!HALVES)
+        if (a.m > 128 && tiles(256, 256) >= kFull) return launch_tile<T, XF, 256, 256, 4, 2, 128, 3, 3>(a, stream);
       if (tiles(128, 256) >= kFull) return launch_tile<T, XF, 128, 256, 2, 2, 128, 2, 4>(a, stream);
     } else {
       if (a.m > 128 && tiles(256, 256) >= kFull) return launch_tile<T, XF, 256, 256, 4, 2, 256, 2, 2>(a, stream);
     }
     if (tiles(128, 128) >= kFull) return launch_tile<T, XF, 128, 128, 2, 2, 256, 2, 2>(a, stream);
   }
-  if (tiles(64, 128) >= 2 * 256) return launch_tile<T, XF, 64, 128, 2, 2, 256, 2, 2>(a, stream);
-  if (tiles(64, 128) >= kFull) return launch_tile<T, XF, 64, 128, 2, 2, 256, 3, 4>(a, stream);
+  if (tiles(64, 128) >= (HALVES ? kFull : 2 * 256)) return launch_tile<T, XF, 64, 128, 2, 2, 256, 2, 2>(a, stream);
+  if constexpr (!HALVES)
+    if (tiles(64, 128) >= kFull) return launch_tile<T, XF, 64, 128, 2, 2, 256, 3, 4>(a, stream);
   return launch_tile<T, XF, 64, 64, 2, 2, 256, 4, 4>(a, stream);
 }
 template <typename T> const char* launch_linear_x(const ns_mx_linear_args& a, hipStream_t stream) {

@@ -12,7 +12,8 @@ Bounds, with u = 2^-24 (float32 rounds a result by at most u of it):
 * a result in MX rows: the value before rounding is within those bounds, so the block's exponent is one of the two ends',
   and under it each code lies between the codes of the two ends.
 * products: values exact, so k terms in float32 in any order lose at most (k - 1) u of the sum of their magnitudes where
-  each addition rounds, twice that where it cuts; 2 k u is taken."""
+  each addition rounds, twice that where it cuts; 2 k u is taken.  A 16-bit result of 8-bit rows may lose each product's part
+  below 2^-13 of the largest of its eight neighbours besides: at most 7 2^-13 of that one, which has a test of its own."""
 import numpy as np
 import torch
 

@@ -332,6 +332,31 @@ def test_linear_scales_at_the_ends(device):
             assert torch.equal(MX.mx_linear_hip((x.codes, s), (w.codes, t), dtype=torch.float32).cpu().double(), torch.from_numpy(xv @ wv.T))
 
 
+@pytest.mark.parametrize("m,n", [(1, 64), (40, 90), (64, 25600), (128, 25600), (200, 25600)])
+def test_linear_large_and_small_products_together(device, m, n):
+    """Eight neighbours from e4m3's smallest value to its largest: their float32 sum is exact (magnitudes under 448 * 4 * 8 <
+    2^14, whole multiples of 2^-9 / 2), and a 16-bit result loses at most 2^-13 of the largest product for each other one."""
+    gen = torch.Generator().manual_seed(m)
+    xc = torch.zeros(m, 128, dtype=torch.uint8)
+    for i in range(m):
+        some = torch.randint(0, 127, (8,), generator=gen) + 128 * torch.randint(0, 2, (8,), generator=gen)
+        some[i % 8], some[(i + 3) % 8] = 126, 1                                   # 448 and 2^-9
+        xc[i, 8 * (i % 16):8 * (i % 16) + 8] = some.to(torch.uint8)
+    nibbles = torch.randint(0, 7, (n, 128), generator=gen) + 8 * torch.randint(0, 2, (n, 128), generator=gen)
+    value = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64)
+    xv, wv = xc.view(torch.float8_e4m3fn).double(), value[nibbles]
+    one = lambda rows: torch.full((rows, 4), 127, dtype=torch.uint8).view(torch.float8_e8m0fnu).to(device)
+    x = (xc.view(torch.float8_e4m3fn).to(device), one(m))
+    w = ((nibbles[:, 0::2] | nibbles[:, 1::2] << 4).to(torch.uint8).view(torch.float4_e2m1fn_x2).to(device), one(n))
+    want = xv @ wv.T
+    assert torch.equal(MX.mx_linear_hip(x, w, dtype=torch.float32).cpu().double(), want)
+    largest = torch.full((m, 1), 448.0 * 4, dtype=torch.float64)
+    for dtype in (torch.bfloat16, torch.float16):
+        got = MX.mx_linear_hip(x, w, dtype=dtype).cpu().double()
+        lost = 7 * 2.0 ** -13 * largest
+        assert ((got - want).abs() <= lost + (want.abs() + lost) * torch.finfo(dtype).eps / 2).all()
+
+
 @pytest.mark.parametrize("m", [3, 33, 140])
 def test_linear_strided_operands_and_out(device, m):
     x, w, want = check_exact(m, 200, 384, "mxfp8", device, torch.bfloat16)
@@ -386,7 +411,10 @@ def test_rows_past_32_bits(device):
     got = MX.mx_linear_hip(q, few)
     part = MX.MxTensor(q.codes[-300:].clone(), q.scales[-300:].clone(), cols)
     assert torch.equal(got[-300:].isnan(), torch.zeros_like(got[-300:], dtype=torch.bool))
-    assert_near(got[-300:], *[f64(t) for t in [MX.mx_linear_hip(part, few, dtype=torch.float32)]], torch.bfloat16, 2.0 ** -8)
+    # every tile adds the columns in their order, 128 at a time: the same sums, the same bits.  (A bound relative to a float32
+    # result would not hold: that one keeps what a 16-bit one leaves out of an octet, up to 7 2^-13 of the sum of magnitudes,
+    # and a result may be as small as it likes beside that sum.)
+    assert torch.equal(got[-300:], MX.mx_linear_hip(part, few))
     del q, got, x, out
     long = torch.randint(0, 256, (140000, cols // 2), dtype=torch.uint8, device=device).view(torch.float4_e2m1fn_x2)
     scales = torch.full((140000, cols // 32), 120, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
