@@ -105,6 +105,8 @@ struct Divide {
 // Thread t takes the row's values 8 (c group + t) .. + 7 for c < CH and keeps them, as they were rounded to the type,
 // until the row's sum is known, so memory is read once; CH = 0 reads a row of any width a second time.  The squares are
 // added in float64: a float32's square neither overflows nor vanishes there.
+// Bound by memory: 8192 x 4096 bfloat16 rows with residual and sum to 8-bit MX rows move 236 MB in 45 us, 5.2 TB/s, a large
+// copy's rate; 4096 rows of 40 float16 heads of 128, 84 MB in 19 us, 17.6 one after another.  One row of 4096 takes 3.2 us.
 template <typename T, int CH>
 __global__ __launch_bounds__(1024) void norm_kernel(ns_mx_norm_args a, int group, int width, double one_over_cols, Divide by_heads) {
   __shared__ double s_part[16];
@@ -281,8 +283,9 @@ __device__ __forceinline__ float exp_minus(float x) {
   return fmaf(p, rest * kLn2, p);
 }
 
-// A workgroup takes kGate / across rows by `across` (a power of two) threads' 8 values; blockIdx.y: the next ones along
-// the rows.
+// A workgroup takes kGate / 2^shift rows by 2^shift threads' 8 values; blockIdx.y: the next ones along the rows.  A quad of
+// lanes has an MX block, so no value passes through LDS.  Bound by memory: 4096 x 16384 bfloat16 gates to 8-bit rows
+// move 338 MB in 63 us, 5.4 TB/s; 128256 x 2048 bfloat16 weights to 4-bit rows 665 MB in 119 us, 5.6 TB/s (a large copy: 5.2).
 template <typename T, bool GATED>
 __global__ __launch_bounds__(kGate) void gate_kernel(ns_mx_gate_args a, int shift, int width) {
   const int chunk = (int)(threadIdx.x & ((1u << shift) - 1)) + ((int)blockIdx.y << shift);
@@ -338,7 +341,8 @@ template <typename T, bool GATED> int launch_gate(const ns_mx_gate_args& a, hipS
 
 // ---- dequantisation -------------------------------------------------------------------------------------------
 
-// With PAST the values are stored past the caches.
+// With PAST the values are stored past the caches: results larger than these hold push out what is read.  Bound by memory: 128256
+// x 2048 values of 4 bits to bfloat16, 665 MB in 122 us, 5.4 TB/s.
 template <typename T, bool PAST>
 __global__ __launch_bounds__(kGate) void values_kernel(ns_mx_rows r, int64_t n, int cols, void* out, int64_t stride_out, int shift) {
   const int chunk = (int)(threadIdx.x & ((1u << shift) - 1)) + ((int)blockIdx.y << shift);

@@ -201,7 +201,8 @@ template <int PIECES> __device__ __forceinline__ int x_swizzle(int row) {
 // A workgroup of eight waves computes 16 rows of x by 32 outputs.  The columns are dealt out to the waves in groups of U stages
 // of 128; x's of KS stages at a time lie in LDS, the weight goes from memory into the operand registers of the one wave
 // that uses it, a stage's registers refilled with the wave's next group as soon as its products are issued.  The waves' sums
-// meet in LDS and are added in their order.
+// meet in LDS and are added in their order.  Bound by latency: 1 x 8192 x 2048 has 9 MB to read, 1.7 us at a copy's rate, and
+// takes 4.7 us in 256 workgroups, 2.5 of them a launch's: the first loads, x's way through LDS, the sums' way through LDS.
 constexpr int kFew = 8;
 
 template <typename T, int XF, int U, int KS>
