@@ -84,9 +84,8 @@ typedef struct ns_mx_gate_args {
   int32_t        cols, dtype;
 } ns_mx_gate_args;
 
-/* out[i][j] = sum over c of x[i][c] w[j][c], the products and their sums in float32, rounded once to out's type.  With
- * a 16-bit out and 8-bit rows, of eight neighbouring columns' products what lies 2^-13 below the largest is left out (about
- * 1e-5 of the sum).  Strides of x and weight are below 2^23 bytes. */
+/* out[i][j] = sum over c of x[i][c] w[j][c], products whole, their sums float32, rounded once to out's type.  Strides of x
+ * and weight are below 2^23 bytes. */
 typedef struct ns_mx_linear_args {
   ns_mx_rows     x;                /* (m) rows, either format */
   ns_mx_rows     weight;           /* (n) rows, NS_MX_FP4 */

@@ -136,24 +136,18 @@ __device__ __forceinline__ void store8(void* base, int64_t at, int left, const f
 // ---- operands ---------------------------------------------------------------------------------------------------
 
 // The instruction adds products of eight neighbours with 13 bits below the largest one's exponent and cuts the rest off (from
-// there on float32's 24 bits).  An e4m3 code times an e2m1 code has up to 21 bits, so results of 8-bit rows are off by about
-// 2^-17 of their size: far below a 16-bit result's rounding, which takes them as they are.  Float32 results (WHOLE) take the
-// codes in two halves, those of 2 and above (the exponent's highest bit) and those below, a product each: neither spans
-// more than 13 bits, and what is added is whole.  4-bit products span 7 bits.
-template <int XF, bool WHOLE> __device__ __forceinline__ f32x4 products(u32x4 w, const u32x4 (&x)[2], int sw, int sx, f32x4 c) {
+// there on float32's 24 bits).  4-bit products span 7 bits.  An e4m3 code times an e2m1 code has up to 21, so 8-bit rows are
+// taken in two halves, the codes below 2 and those of 2 and above (the exponent's highest bit), a product each: neither
+// spans more than 13 bits, and what is added is whole.  (One product alone loses up to 7 2^-13 of the largest of eight
+// neighbours, which nothing bounds relative to a sum that cancels: 0.5% of the bfloat16 results came out a step off.)
+__device__ __forceinline__ uint32_t below_2(uint32_t v) {
+  // selectors 8 to 11 spread the top bits of the operands' bytes 1 and 3 over a byte: bit 6 of v's bytes 0 to 3
+  return v ^ (v & __builtin_amdgcn_perm(v << 1, v << 9, 0x0b090a08u));
+}
+template <int XF> __device__ __forceinline__ f32x4 product(u32x4 w, const u32x4 (&x)[2], int sw, int sx, f32x4 c) {
   const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
   if constexpr (XF == NS_MX_FP8) {
-    i32x8 b = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
-    if constexpr (WHOLE) {
-      i32x8 low;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t v = (uint32_t)b[i], t = v >> 6 & 0x01010101u, high = (t << 8) - t;   // 255 where a byte has bit 6
-        low[i] = (int)(v & ~high);
-        b[i] = (int)(v & high);
-      }
-      c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, low, c, 4, 0, 0, sw, 0, sx);
-    }
+    const i32x8 b = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, 0, sw, 0, sx);
   } else {
     const i32x8 b = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], 0, 0, 0, 0};
@@ -274,8 +268,18 @@ __global__ __launch_bounds__(64 * kFew) void few_kernel(const ns_mx_linear_args 
           x[0] = *reinterpret_cast<const u32x4*>(xs + st * STEP + at0);
           if constexpr (XP == 8) x[1] = *reinterpret_cast<const u32x4*>(xs + st * STEP + at1);
           const int sx = sc[st * 64 + r * 4 + g];
+          if constexpr (XP == 8) {
+            u32x4 low[2];
 #pragma unroll
-          for (int p = 0; p < 2; ++p) acc[p] = products<XF, sizeof(T) == 4>(w[s][p], x, (int)(scale[p][s] >> (8 * g)), sx, acc[p]);
+            for (int c = 0; c < 8; ++c) {
+              low[c >> 2][c & 3] = below_2(x[c >> 2][c & 3]);
+              x[c >> 2][c & 3] ^= low[c >> 2][c & 3];
+            }
+#pragma unroll
+            for (int p = 0; p < 2; ++p) acc[p] = product<XF>(w[s][p], low, (int)(scale[p][s] >> (8 * g)), sx, acc[p]);
+          }
+#pragma unroll
+          for (int p = 0; p < 2; ++p) acc[p] = product<XF>(w[s][p], x, (int)(scale[p][s] >> (8 * g)), sx, acc[p]);
         }
         load_stage(s, q + kFew);
       }
@@ -313,11 +317,9 @@ template <typename T, int XF> const char* launch_few(const ns_mx_linear_args& a,
 // sliver of a 128-byte line that is fetched again every time.  Every place is an array and the loop is unrolled until all
 // recur: the compiler sees that a stage's reads touch none that a direct load is filling, and waits for none of those.
 //
-// Eight waves (the tiles of 256 x 256) work in two halves, one wave of each on every SIMD: while one half multiplies, the
-// other reads its next operands, and a barrier changes places.  A half's loads are issued among its products, where no one
-// waits for them to be taken; the first half's of 8-bit rows, whose products take twice as long, behind its reads.
-// 4096 x 16384 x 4096 (8-bit rows): 203 us, 222 with all eight waves in step, 185 without the results' stores and 152 without
-// loads, of 112 us that the matrix units need at the rate they reach by themselves (4900 TFLOP/s).
+// Eight waves (the tiles of 256 x 256, 4-bit rows) work in two halves, one wave of each on every SIMD: while one half
+// multiplies, the other reads its next operands, and a barrier changes places.  A half's loads are issued among its
+// products, where no one waits for them to be taken.
 //
 // Pieces of 16 bytes lie in LDS as above: c ^ f(r), x's 16 rows of a read one after the other, the weight's in the order of its
 // operands.
@@ -347,7 +349,8 @@ template <int XF, int BM, int BN, int WM, int WN, int BK, int P, int SP> struct 
     for (int i = t - P + 1; i < t; ++i) n += ((i % SP) + SP) % SP == 0 ? SL : 0;
     return n;
   }
-  static_assert(XL * 1024 * WAVES == XB && WL * 1024 * WAVES == WB && TJ % 2 == 0 && BM % 64 == 0 && BN % 64 == 0, "tiling");
+  static_assert(XL * 1024 * WAVES == XB && WL * 1024 * WAVES == WB && TJ % 2 == 0 && BM % 64 == 0 && BN % 32 == 0, "tiling");
+  static_assert(XF == NS_MX_FP4 || (TJ <= 8 && WAVES == 4), "8-bit rows: halves of x's operands are formed a register or more a product");
   static_assert(SP >= P && P >= 2 && P <= 4, "a group of scales is older than the stages in flight");
   static_assert(P * BYTES + 2 * SB <= 160 * 1024 && newer(0) + SL < 63, "LDS, counter");
 };
@@ -356,7 +359,7 @@ template <typename T, int XF, int BM, int BN, int WM, int WN, int BK, int P, int
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linear_args a, int gm) {
   using C = Tile<XF, BM, BN, WM, WN, BK, P, SP>;
   constexpr int TI = C::TI, TJ = C::TJ, XP = C::XP, WP = C::WP, SUB = C::SUB;
-  constexpr bool PAIRED = C::WAVES == 8, AMONG_READS = XF == NS_MX_FP8;
+  constexpr bool PAIRED = C::WAVES == 8;
   __shared__ __attribute__((aligned(16))) unsigned char s0[C::BYTES], s1[C::BYTES], s2[P > 2 ? C::BYTES : 16], s3[P > 3 ? C::BYTES : 16];
   __shared__ __attribute__((aligned(16))) unsigned char c0[C::SB], c1[C::SB];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -454,10 +457,34 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linea
       sx[i] = sc[sx_at + i * 256];
     }
   };
-  const auto multiply = [&](auto number) {
+  // Products of x's operand number i.  8-bit codes: those below 2, formed among the previous number's products, then the
+  // others, which take x's registers: 8 registers more than one product needs, and instructions that wait for none.
+  u32x4 low[2];
+  const auto form_low = [&](auto number, auto from, auto to) {
     constexpr int i = decltype(number)::value;
+    if constexpr (XF == NS_MX_FP8 && i < TI)
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) acc[i][j] = products<XF, sizeof(T) == 4>(w[j], x[i], sw[j], sx[i], acc[i][j]);
+      for (int c = decltype(from)::value; c < decltype(to)::value; ++c) low[c >> 2][c & 3] = below_2(x[i][c >> 2][c & 3]);
+  };
+  const auto multiply = [&](auto number) {
+    constexpr int i = decltype(number)::value, EACH = 8 / TJ;
+    if constexpr (XF == NS_MX_FP8) {
+      if constexpr (i == 0) form_low(number, all, std::integral_constant<int, 8>{});
+      unrolled<TJ>([&](auto at) {
+        constexpr int j = decltype(at)::value;
+        acc[i][j] = product<XF>(w[j], low, sw[j], sx[i], acc[i][j]);
+#pragma unroll
+        for (int c = j * EACH; c < (j + 1) * EACH; ++c) x[i][c >> 2][c & 3] ^= low[c >> 2][c & 3];
+      });
+      unrolled<TJ>([&](auto at) {
+        constexpr int j = decltype(at)::value;
+        acc[i][j] = product<XF>(w[j], x[i], sw[j], sx[i], acc[i][j]);
+        form_low(std::integral_constant<int, i + 1>{}, std::integral_constant<int, j * EACH>{}, std::integral_constant<int, (j + 1) * EACH>{});
+      });
+    } else {
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[i][j] = product<XF>(w[j], x[i], sw[j], sx[i], acc[i][j]);
+    }
   };
   const auto meet = [&] {
     __builtin_amdgcn_s_barrier();
@@ -485,7 +512,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linea
         const bool skip = TAIL && S > 0 && st * SUB + S >= n128;
         if (!skip) read(at, sub);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (S == 0 && !LATE && AMONG_READS) issue(at, all, at_once, st);
         if constexpr (S == SUB - 1 && LATE) __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(C::newer(AT + 1)) & ~(15 << 8));
         else __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(63) & ~(15 << 8));
         meet();
@@ -494,7 +520,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linea
           if (!skip) multiply(i);
           __builtin_amdgcn_sched_barrier(0);
           if constexpr (S == SUB - 1 && LATE) issue(after, i, std::integral_constant<int, TI>{}, st + 1);
-          if constexpr (S == 0 && !LATE && !AMONG_READS) issue(at, i, std::integral_constant<int, TI>{}, st);
+          if constexpr (S == 0 && !LATE) issue(at, i, std::integral_constant<int, TI>{}, st);
         });
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
@@ -556,33 +582,39 @@ const char* launch_tile(const ns_mx_linear_args& a, hipStream_t stream) {
   return nullptr;
 }
 
-// Which kernel, by sizes and types alone (times of bf16 results, 8-bit rows, in microseconds, both sides measured):
-// - up to 16 rows and 8192 outputs: few_kernel, 5.4 at 1 x 8192 x 2048 where a 64 x 64 tile takes 9; above that the tiles have
-//   workgroups enough to keep the memory busy, 38 at 64 x 128256 x 2048.
-// - the largest tile that leaves at least kFull of them, as it reads the operands from the caches least often: 4096 x 16384 x
-//   4096 takes 204 with 256 x 256 and 280 with 128 x 256; 1024 x 4096 x 4096 has 64 of the first and takes 24 with 64 x 128.
-// - 64 x 128 in two forms: two places a workgroup and two workgroups a unit where there are that many, else three places.
-// Float32 results of 8-bit rows hold two halves of x (products()): the 256 x 256 tile and the three places spill registers
-// there (489 against 425 with 128 x 256 at 4096 x 16384 x 4096, 505 against 24 at 512 x 4096 x 4096) and are left out.
+// Which kernel, by sizes and the rows' format alone.  Times of bfloat16 results in microseconds, both sides measured.
+//
+// 4-bit rows:
+// - up to 16 rows and 8192 outputs, one workgroup a compute unit: few_kernel, 4.2 at 1 x 8192 x 2048 where a 64 x 64 tile takes
+//   4.8; beyond, 5.9 against 5.0 at 1 x 12288 x 2048.
+// - the largest tile that leaves at least kFull of them, as it reads the operands from the caches least often; 64 x 128 in two
+//   forms: two places a workgroup and two workgroups a unit where there are that many, else three places.
+//
+// 8-bit rows, which form two halves of x (below_2()), the more often the fewer outputs a wave has:
+// - up to 16 rows and 16384 outputs: few_kernel, 6.4 at 1 x 16384 x 2048 and 19.9 at 1 x 16384 x 8192 where 64 x 64 takes 7.8 and
+//   26.6; beyond, 24.9 against 18.3 at 1 x 32768 x 4096.
+// - 128 x 256 where there are kFull of them: 340 at 4096 x 16384 x 4096 (64 x 128 425, 128 x 128 396, 256 x 256 with spilled
+//   registers 386), 55.0 against 56.2 at 1024 x 8192 x 4096 (256 tiles), 54.4 against 42.6 at 700 x 8192 x 4096 (192).
+// - 64 x 32 while each has a unit for itself: 10.0 at 64 x 8192 x 4096 where 64 x 64 takes 12.9; 17.8 against 13.2 at 64 x 12288.
+// - 64 x 64, two places and two workgroups a unit, while all run at once: 18.3 at 64 x 24576 x 4096 where 64 x 128 takes 20.0; then
+//   64 x 128: 33.4 at 64 x 40960 x 4096 where 64 x 64 takes 39.2.
 template <typename T, int XF> const char* launch_linear_t(const ns_mx_linear_args& a, hipStream_t stream) {
   const auto tiles = [&](int64_t bm, int64_t bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
-  constexpr int64_t kFull = 200;   // tiles that keep most of the 256 compute units busy
-  constexpr bool HALVES = XF == NS_MX_FP8 && sizeof(T) == 4;
-  if (a.m <= 16 && a.n <= 32 * 256) return launch_few<T, XF>(a, stream);
-  if (a.m > 64) {
-    if constexpr (XF == NS_MX_FP8) {
-      if constexpr (!HALVES)
-        if (a.m > 128 && tiles(256, 256) >= kFull) return launch_tile<T, XF, 256, 256, 4, 2, 128, 3, 3>(a, stream);
-      if (tiles(128, 256) >= kFull) return launch_tile<T, XF, 128, 256, 2, 2, 128, 2, 4>(a, stream);
-    } else {
-      if (a.m > 128 && tiles(256, 256) >= kFull) return launch_tile<T, XF, 256, 256, 4, 2, 256, 2, 2>(a, stream);
-    }
-    if (tiles(128, 128) >= kFull) return launch_tile<T, XF, 128, 128, 2, 2, 256, 2, 2>(a, stream);
-  }
-  if (tiles(64, 128) >= (HALVES ? kFull : 2 * 256)) return launch_tile<T, XF, 64, 128, 2, 2, 256, 2, 2>(a, stream);
-  if constexpr (!HALVES)
+  constexpr int64_t kUnits = 256, kFull = 200;   // compute units, and the tiles that keep most of them busy
+  if constexpr (XF == NS_MX_FP8) {
+    if (a.m <= 16 && a.n <= 2 * 32 * kUnits) return launch_few<T, XF>(a, stream);
+    if (a.m > 64 && tiles(128, 256) >= kFull) return launch_tile<T, XF, 128, 256, 2, 2, 128, 2, 4>(a, stream);
+    if (tiles(64, 32) <= kUnits) return launch_tile<T, XF, 64, 32, 4, 1, 256, 4, 4>(a, stream);
+    if (tiles(64, 64) <= 2 * kUnits) return launch_tile<T, XF, 64, 64, 4, 1, 256, 2, 2>(a, stream);
+    return launch_tile<T, XF, 64, 128, 2, 2, 256, 2, 2>(a, stream);
+  } else {
+    if (a.m <= 16 && a.n <= 32 * kUnits) return launch_few<T, XF>(a, stream);
+    if (a.m > 128 && tiles(256, 256) >= kFull) return launch_tile<T, XF, 256, 256, 4, 2, 256, 2, 2>(a, stream);
+    if (a.m > 64 && tiles(128, 128) >= kFull) return launch_tile<T, XF, 128, 128, 2, 2, 256, 2, 2>(a, stream);
+    if (tiles(64, 128) >= 2 * kUnits) return launch_tile<T, XF, 64, 128, 2, 2, 256, 2, 2>(a, stream);
     if (tiles(64, 128) >= kFull) return launch_tile<T, XF, 64, 128, 2, 2, 256, 3, 4>(a, stream);
-  return launch_tile<T, XF, 64, 64, 2, 2, 256, 4, 4>(a, stream);
+    return launch_tile<T, XF, 64, 64, 2, 2, 256, 4, 4>(a, stream);
+  }
 }
 template <typename T> const char* launch_linear_x(const ns_mx_linear_args& a, hipStream_t stream) {
   return a.x.format == NS_MX_FP8 ? launch_linear_t<T, NS_MX_FP8>(a, stream) : launch_linear_t<T, NS_MX_FP4>(a, stream);

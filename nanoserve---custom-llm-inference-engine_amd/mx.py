@@ -247,9 +247,7 @@ def dequantize_mx_hip(t, dtype=torch.bfloat16, *, out=None, stream=None):
 
 def mx_linear_hip(x, weight, *, dtype=torch.bfloat16, out=None, stream=None):
     """x @ weight.T, (m, n) of ``dtype``: x MX rows in either format, (m, cols), and weight MX rows in 4 bits, (n, cols).
-    The products of the values that the codes stand for are exact, their sums are float32, rounded once.  A 16-bit result
-    of 8-bit rows leaves out what lies 2^-13 below the largest product of eight neighbouring columns, about 1e-5 of the
-    sum; a float32 result has it."""
+    The products of the values that the codes stand for are exact, their sums are float32, rounded once to ``dtype``."""
     if _LIB is None:
         load()
     host, calls = _HOST
