@@ -57,7 +57,8 @@ class MxError(RuntimeError):
 
 
 class MxTensor(NamedTuple):
-    """MX rows; the calls also take a pair (codes, scales)."""
+    """MX rows; the calls also take a pair (codes, scales).  Products run over whole rows: what lies past ``cols`` are zero
+    codes and scales that are no NaN, as every call here and ``mx_tensor`` leave them."""
 
     codes: torch.Tensor
     scales: torch.Tensor
@@ -261,7 +262,9 @@ def mx_linear_hip(x, weight, *, dtype=torch.bfloat16, out=None, stream=None):
 def mx_tensor(codes, scales, cols: Optional[int] = None) -> MxTensor:
     """MX rows as other programs store them, laid out for these calls (a copy where they are not so already): codes
     (rows, k), ``float8_e4m3fn``, or (rows, k / 2), ``float4_e2m1fn_x2`` or uint8 of the same bits, scales (rows, k / 32),
-    ``float8_e8m0fnu`` or uint8, for any k that is a multiple of 32; ``cols`` (default k): the values in use."""
+    ``float8_e8m0fnu`` or uint8, for any k that is a multiple of 32; ``cols`` (default k): the values in use.  What is stored
+    past them is left out: with ``cols`` below k device tensors are copied (nothing is read on the host to see whether there
+    is anything), host tensors where it would enter a product."""
     if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
         raise MxError("codes and scales must be tensors")
     if codes.dtype is torch.uint8:
@@ -280,13 +283,19 @@ def mx_tensor(codes, scales, cols: Optional[int] = None) -> MxTensor:
     if not 0 < cols <= k:
         raise MxError(f"cols must lie in 1 .. {k}, not {cols}")
 
-    def laid_out(t, width, unit):
+    def laid_out(t, width, unit, used, last, harmful):
+        """Rows of ``width`` bytes, those from ``used`` on zero and of the one before only the bits of ``last``."""
         b = t.view(torch.uint8)
-        if t.shape[1] == width and t.stride(1) == 1 and (n < 2 or t.stride(0) % unit == 0) and t.data_ptr() % unit == 0:
+        fits = t.shape[1] == width and t.stride(1) == 1 and (n < 2 or t.stride(0) % unit == 0) and t.data_ptr() % unit == 0
+        if fits and (cols == k or not (t.is_cuda or harmful(b[:, used:]).any() or (b[:, used - 1] & (255 - last)).any())):
             return t
         new = torch.zeros((n, width), dtype=torch.uint8, device=t.device)
-        new[:, :t.shape[1]] = b
+        new[:, :used] = b[:, :used]
+        if last != 255:
+            new[:, used - 1] &= last
         return new.view(t.dtype)
 
     wide = -(-k // ROW_ALIGN) * ROW_ALIGN
-    return MxTensor(laid_out(codes, wide // per, 16), laid_out(scales, wide // 32, 4), cols)
+    half = per == 2 and cols % 2 == 1        # the last value in use shares its byte with one that is not
+    return MxTensor(laid_out(codes, wide // per, 16, -(-cols // per), 15 if half else 255, lambda past: past != 0),
+                    laid_out(scales, wide // 32, 4, -(-cols // 32), 255, lambda past: past == 255), cols)
