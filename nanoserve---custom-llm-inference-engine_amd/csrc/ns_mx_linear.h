@@ -249,9 +249,12 @@ __global__ __launch_bounds__(64 * kFew) void few_kernel(const ns_mx_linear_args 
     if (base > 0) __syncthreads();
     fill(base);
     if (base == 0) {
+      // the wait counts the weight's 2 + 2 U loads: x's are all issued before them, and they before the wait
+      __builtin_amdgcn_sched_barrier(0);
       load_scale(scale, q);
 #pragma unroll
       for (int s = 0; s < U; ++s) load_stage(s, q);
+      __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(2 + 2 * U));   // x is there, the weight may be on its way
     } else {
       __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(0));

@@ -1,0 +1,56 @@
+"""The layer operators' kernels as built: orders of instructions that their waits count on, read from the code object."""
+import os
+import re
+import subprocess
+
+import pytest
+
+from conftest import pkg
+
+MX = pkg("mx")
+
+
+@pytest.fixture(scope="module")
+def listing(tmp_path_factory):
+    """{kernel: its instructions} of the built library."""
+    if not os.path.exists(MX.LIB_PATH):
+        pytest.skip("library not built (run __graft_entry__.build())")
+    at = tmp_path_factory.mktemp("code")
+    llvm = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin")
+    fat, code = str(at / "fat"), str(at / "code")
+    subprocess.run([f"{llvm}/llvm-objcopy", "--dump-section", f".hip_fatbin={fat}", MX.LIB_PATH, str(at / "copy")], check=True)
+    subprocess.run([f"{llvm}/clang-offload-bundler", "--unbundle", "--type=o", f"--input={fat}", f"--output={code}",
+                    "--targets=hipv4-amdgcn-amd-amdhsa--gfx950"], check=True)
+    text = subprocess.run([f"{llvm}/llvm-objdump", "-d", "--no-show-raw-insn", code], check=True, capture_output=True, text=True).stdout
+    kernels = {}
+    for part in re.split(r"\n(?=[0-9a-f]+ <)", text):
+        head = re.match(r"[0-9a-f]+ <(\w+)>:", part)
+        if head:
+            kernels[head.group(1)] = [line.split("//")[0].strip() for line in part.split("\n")[1:]]
+    return kernels
+
+
+def first_loads(instructions):
+    """From the first direct load to LDS to the barrier after it: "lds" and "load" for buffer loads, a number for a wait."""
+    events, begun = [], False
+    for i in instructions:
+        if i.startswith("buffer_load"):
+            events.append("lds" if i.endswith(" lds") else "load")
+            begun = begun or events[-1] == "lds"
+        elif begun and i.startswith("s_waitcnt") and "vmcnt" in i:
+            events.append(int(re.search(r"vmcnt\((\d+)\)", i).group(1)))
+        elif begun and i.startswith("s_barrier"):
+            break
+    return events
+
+
+def test_few_rows_wait_counts_the_loads_behind_x(listing):
+    """few_kernel waits for all but the weight's first 2 + 2 U loads: right where x's direct loads come before those."""
+    few = {n: i for n, i in listing.items() if "few_kernel" in n}
+    assert len(few) == 12
+    for name, instructions in few.items():
+        events = first_loads(instructions)
+        u = int(re.search(r"few_kernelI.*Li[48]ELi(\d)ELi", name).group(1))
+        first = events.index("load")
+        assert "lds" not in events[first:], name
+        assert events.count("load") == events[-1] == 2 + 2 * u, (name, events)
