@@ -202,7 +202,7 @@ constexpr int kFew = 8;
 template <typename T, int XF, int U, int KS>
 __global__ __launch_bounds__(64 * kFew) void few_kernel(const ns_mx_linear_args a) {
   constexpr int XP = XF == NS_MX_FP8 ? 8 : 4, STEP = 16 * XP * 16, FILLS = KS * STEP / 1024 / kFew;
-  static_assert(FILLS * 1024 * kFew == KS * STEP && KS % (U * kFew) == 0, "tiling");
+  static_assert(FILLS * 1024 * kFew == KS * STEP && KS % (U * kFew) == 0 && (U == 2 || U == 4), "tiling");
   __shared__ __attribute__((aligned(16))) unsigned char xs[KS * STEP], sc[KS * 64];
   __shared__ float sums[kFew * 8 * 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
@@ -233,10 +233,17 @@ __global__ __launch_bounds__(64 * kFew) void few_kernel(const ns_mx_linear_args 
     wso[p] = (uint32_t)(row * a.weight.stride_scales);
   }
   // a row's scales of a group are 4 U bytes; a group past the last is read behind the buffers' ends, where nothing is
-  u32x4 w[U][2], scale[2], next[2];
-  const auto load_scale = [&](u32x4 (&to)[2], int q) {
+  u32x4 w[U][2];
+  typedef uint32_t words __attribute__((ext_vector_type(U)));
+  words scale[2], next[2];
+  // (scales no wider than that: registers that nothing reads are taken for the next loads' addresses, which then wait for them)
+  const auto load_scale = [&](words (&to)[2], int q) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) to[p] = load16(wsr, wso[p] | (q < ng ? 0u : 1u << 31), q * (4 * U));
+    for (int p = 0; p < 2; ++p) {
+      const uint32_t at = wso[p] | (q < ng ? 0u : 1u << 31);
+      if constexpr (U == 4) to[p] = load16(wsr, at, q * (4 * U));
+      else to[p] = __builtin_bit_cast(words, __builtin_amdgcn_raw_buffer_load_b64(wsr, (int)at, q * (4 * U), 0));
+    }
   };
   const auto load_stage = [&](int s, int q) {
 #pragma unroll

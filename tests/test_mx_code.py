@@ -54,3 +54,13 @@ def test_few_rows_wait_counts_the_loads_behind_x(listing):
         first = events.index("load")
         assert "lds" not in events[first:], name
         assert events.count("load") == events[-1] == 2 + 2 * u, (name, events)
+
+
+def test_few_rows_first_loads_wait_for_none(listing):
+    """Up to the wait for x nothing waits for memory: the weight's first loads go out behind x's, not when x is there."""
+    for name, instructions in listing.items():
+        if "few_kernel" in name:
+            events = first_loads(instructions)
+            # the last of x's loads, the wait of the later rounds (all of x, no weight on its way) and then the weight's
+            tail = events[events.index("load"):]
+            assert [e for e in tail if e != "load"] == [tail[-1]], (name, events)
