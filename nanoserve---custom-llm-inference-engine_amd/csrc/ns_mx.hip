@@ -301,23 +301,32 @@ __global__ __launch_bounds__(kGate) void gate_kernel(ns_mx_gate_args a, int shif
   if constexpr (GATED) {
     float u[8];
     load8<T>(a.up, from * a.stride_up + 8 * chunk, left, u);
-    float most = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
-    // by the exponential of -|gate|, which does not overflow: the far negative gates keep their small products
-    if (most <= 80.0f) {
+    // far negative gates take the exponential that does not overflow, and keep their small products
+    if constexpr (sizeof(T) == 4) {   // float32 results show each rounding: one exponential, one sum, one quotient, one product
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float small = exp_minus(fabsf(v[e])), d = 1.0f + small;
-        float over = __builtin_amdgcn_rcpf(d);             // within 2 units of 2^-24, one step takes it to 1
-        over = fmaf(fmaf(-d, over, 1.0f), over, over);
-        v[e] = v[e] * (v[e] < 0.0f ? small * over : over) * u[e];
+        const bool far = v[e] < -80.0f;
+        const float t = expf(far ? v[e] : -v[e]);
+        v[e] = (far ? v[e] * t : v[e]) / (1.0f + t) * u[e];
       }
-    } else {   // exponentials below the normal numbers, infinities, NaN
+    } else {
+      float most = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float small = expf(-fabsf(v[e]));
-        v[e] = v[e] * ((v[e] < 0.0f ? small : 1.0f) / (1.0f + small)) * u[e];
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+      if (most <= 80.0f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float small = exp_minus(fabsf(v[e])), d = 1.0f + small;
+          float over = __builtin_amdgcn_rcpf(d);             // within 2 units of 2^-24, one step takes it to 1
+          over = fmaf(fmaf(-d, over, 1.0f), over, over);
+          v[e] = v[e] * (v[e] < 0.0f ? small * over : over) * u[e];
+        }
+      } else {   // exponentials below the normal numbers, infinities, NaN
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float small = expf(-fabsf(v[e]));
+          v[e] = v[e] * ((v[e] < 0.0f ? small : 1.0f) / (1.0f + small)) * u[e];
+        }
       }
     }
   }
