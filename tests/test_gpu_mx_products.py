@@ -7,6 +7,7 @@ import torch
 
 from conftest import pkg
 from mx_cases import hidden
+from mx_kernels import SIZES, kernel_of, kernels_of, widths
 
 pytestmark = pytest.mark.gpu
 MX = pkg("mx")
@@ -51,3 +52,71 @@ def test_16_bit_results_are_the_float32_ones_rounded(device, fmt, m, n, k):
     full = MX.mx_linear_hip(x, w, dtype=torch.float32)
     for dtype in (torch.bfloat16, torch.float16):
         assert torch.equal(MX.mx_linear_hip(x, w, dtype=dtype), full.to(dtype)), dtype
+
+
+def whole_numbers(seed, rows, k, fmt, device):
+    """MX rows on the device whose values are whole multiples of 2^-3, below 2^6, and the values in float64: their products'
+    sums, of either sign, stay far below the 2^24 multiples of 2^-6 that float32 adds exactly in any order."""
+    gen = torch.Generator(device=device).manual_seed(seed)
+    pick = lambda lo, hi, *size: torch.randint(lo, hi, size, generator=gen, device=device)  # noqa: E731
+    scales = pick(125, 130, rows, k // 32).to(torch.uint8)
+    if fmt == "mxfp4":
+        codes = pick(0, 256, rows, k // 2).to(torch.uint8)
+        c = codes.long()
+        v = E2M1.to(device)[torch.stack([c & 15, c >> 4], -1).view(rows, k)]
+        codes = codes.view(torch.float4_e2m1fn_x2)
+    else:
+        grid = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 5, 6, 7, 8, -0.5, -1, -1.5, -2, -3, -4, -5, -6, -7, -8], device=device)
+        v = grid[pick(0, len(grid), rows, k)]
+        codes, v = v.to(torch.float8_e4m3fn), v.double()
+    v = v.view(rows, -1, 32) * torch.exp2(scales.double() - 127)[..., None]
+    return (codes, scales.view(torch.float8_e8m0fnu)), v.view(rows, k)
+
+
+@pytest.mark.parametrize("fmt,m,n", SIZES)
+def test_every_kernel_over_its_loop_and_tail(device, fmt, m, n):
+    """The formula's result, rounded once, at widths of one stage up to more than two rounds of the kernel's loop."""
+    for kernel in kernels_of(fmt, m, n):
+        for k in widths(kernel):
+            assert kernel_of(fmt, m, n, k) == kernel
+            x, xv = whole_numbers(m + k, m, k, fmt, device)
+            w, wv = whole_numbers(n + k + 1, n, k, "mxfp4", device)
+            want = xv @ wv.T
+            print(f"linear: m {m} n {n} k {k} {fmt} {kernel}", flush=True)
+            assert want.abs().max() < 2 ** 15
+            for dtype in (torch.bfloat16, torch.float16, torch.float32):
+                got = MX.mx_linear_hip(x, w, dtype=dtype)
+                assert torch.equal(got, want.float().to(dtype)), (kernel, k, dtype, (got.double() - want).abs().max().item())
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_a_row_gives_the_same_bits_in_every_batch_of_tiles(device, fmt):
+    """All tiles add the columns in their order, so a row's results are the same bits wherever it stands and whichever tile
+    its batch takes.  (few_kernel, up to 16 rows, cuts the columns over its waves.)"""
+    seen = set()
+    for n, k in ((1000, 2048), (9000, 1152), (26000, 640)):
+        w = MX.quantize_mx_hip((hidden(n, n, k) * 0.02).to(device), "mxfp4")
+        x = MX.quantize_mx_hip(hidden(k, 1400, k).to(device), fmt)
+        for dtype in (torch.float32, torch.bfloat16):
+            full = MX.mx_linear_hip(x, w, dtype=dtype)
+            for lo, hi in ((0, 1400), (100, 130), (3, 67), (255, 455), (700, 1399), (1383, 1400)):
+                part = MX.MxTensor(x.codes[lo:hi], x.scales[lo:hi], k)
+                seen.add(kernel_of(fmt, hi - lo, n, k))
+                assert torch.equal(MX.mx_linear_hip(part, w, dtype=dtype), full[lo:hi]), (n, lo, hi)
+    assert len(seen) >= 4 and all(name == "tile" for name, *_ in seen)
+
+
+@pytest.mark.parametrize("m,n,k", KERNELS_8)
+def test_nan_codes_and_scales_stay_in_their_row_and_column(device, m, n, k):
+    """e4m3's NaN codes of either sign, and scales of 255, on rows of x and of the weight; every other result is whole."""
+    x, xv = whole_numbers(m, m, k, "mxfp8", device)
+    w, wv = whole_numbers(n, n, k, "mxfp4", device)
+    codes = x[0].view(torch.uint8)
+    codes[m - 1, 7], codes[0, k - 1] = 0x7f, 0xff
+    for row, block in ((0, 1), (n - 1, k // 32 - 1)):
+        w[1].view(torch.uint8)[row, block] = 255
+    nan = torch.zeros(m, n, dtype=torch.bool, device=device)
+    nan[[0, m - 1]], nan[:, [0, n - 1]] = True, True
+    got = MX.mx_linear_hip(x, w, dtype=torch.float32)
+    assert torch.equal(got.isnan(), nan)
+    assert torch.equal(got[~nan], (xv @ wv.T).float()[~nan])

@@ -6,6 +6,7 @@ import subprocess
 import pytest
 
 from conftest import pkg
+from mx_kernels import SIZES, kernels_of, round_of, widths
 
 MX = pkg("mx")
 
@@ -64,3 +65,18 @@ def test_few_rows_first_loads_wait_for_none(listing):
             # the last of x's loads, the wait of the later rounds (all of x, no weight on its way) and then the weight's
             tail = events[events.index("load"):]
             assert [e for e in tail if e != "load"] == [tail[-1]], (name, events)
+
+
+def test_every_kernel_that_is_built_is_reached_and_tested(listing):
+    """The sizes of the product tests take every kernel of the library, and no kernel is built that none of them can take."""
+    built = set()
+    for name in listing:
+        m = re.match(r"_ZN5ns_mx\d+(few|tile)_kernelI(?:f|NS_\d\w+?E)(Li.*)EE", name)
+        if m:
+            built.add((m.group(1), *(int(v) for v in re.findall(r"Li(\d+)E", m.group(2) + "E"))))
+    reached = {k for size in SIZES for k in kernels_of(*size)}
+    assert built == reached
+    for kernel in reached:
+        at, r = widths(kernel), round_of(kernel)
+        assert min(at) <= max(128, r // 4) or kernel[:3] == ("few", kernel[1], 4)
+        assert r in at and (max(at) > 2 * r or kernel[0] == "few" and kernel[2] == 2)
