@@ -501,7 +501,7 @@ struct Result {
       bool fits = out->dim() == like.dim() && out->size(0) == n && out->scalar_type() == like.scalar_type();
       for (int64_t i = 1; fits && i < like.dim(); ++i) fits = out->size(i) == like.size(i);
       if (!fits) throw Refused{"out " + shape_of(*out) + " must have the result's shape and dtype"};
-      if (out->stride(-1) != 1) throw Refused{std::string("out") + kNoStride};
+      if (out->stride(-1) != 1 && out->size(-1) > 1) throw Refused{std::string("out") + kNoStride};
     } else {
       ns_mx_rows r;
       const int64_t k = mx_rows_of(*out, *scales, "out", &r);
