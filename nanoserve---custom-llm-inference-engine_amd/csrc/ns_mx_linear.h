@@ -329,7 +329,8 @@ template <typename T, int XF> const char* launch_few(const ns_mx_linear_args& a,
 //
 // Eight waves (the tiles of 256 x 256, 4-bit rows) work in two halves, one wave of each on every SIMD: while one half
 // multiplies, the other reads its next operands, and a barrier changes places.  A half's loads are issued among its
-// products, where no one waits for them to be taken.
+// products, where no one waits for them to be taken.  8192^3: 280 us, 295 with all eight waves in step; 1777 x 5120 x 8192: 55 and
+// 61.  The code of its last stages spills registers (96 bytes a lane), its loop none.
 //
 // Pieces of 16 bytes lie in LDS as above: c ^ f(r), x's 16 rows of a read one after the other, the weight's in the order of its
 // operands.
@@ -597,14 +598,20 @@ const char* launch_tile(const ns_mx_linear_args& a, hipStream_t stream) {
 // 4-bit rows:
 // - up to 16 rows and 8192 outputs, one workgroup a compute unit: few_kernel, 4.2 at 1 x 8192 x 2048 where a 64 x 64 tile takes
 //   4.8; beyond, 5.9 against 5.0 at 1 x 12288 x 2048.
-// - the largest tile that leaves at least kFull of them, as it reads the operands from the caches least often; 64 x 128 in two
-//   forms: two places a workgroup and two workgroups a unit where there are that many, else three places.
+// - 256 x 256, which reads the operands from the caches least often, where the tiles of 128 x 128, two a unit, would not all run
+//   at once: 54.7 at 1777 x 5120 x 8192 where those take 62.8 (560 of them); 32.4 against 26.7 at 2048 x 4096 x 4096 (512).
+// - 128 x 128 for more than 64 rows where the tiles of 64 x 128 are more than the units: 15.1 at 700 x 4000 x 4096 where those take
+//   20.8 and 64 x 64 16.5; 14.1 against 10.9 at 129 x 8600 x 4096 (204 of 64 x 128).
+// - 64 x 128, three places and one workgroup a unit, for about as many tiles as units: 18.5 at 256 x 8192 x 8192 where 64 x 64 takes
+//   20.2, 12.3 against 13.1 at 64 x 25700 x 4096.
+// - 64 x 128, two places and two workgroups a unit, where that many tiles are there: 33.5 at 64 x 65536 x 4096 where 64 x 64 takes
+//   39.2; 28.8 against 25.7 at 64 x 40960 x 4096 (320).
 //
 // 8-bit rows, which form two halves of x (below_2()), the more often the fewer outputs a wave has:
-// - up to 16 rows and 16384 outputs: few_kernel, 6.4 at 1 x 16384 x 2048 and 19.9 at 1 x 16384 x 8192 where 64 x 64 takes 7.8 and
-//   26.6; beyond, 24.9 against 18.3 at 1 x 32768 x 4096.
-// - 128 x 256 where there are kFull of them: 340 at 4096 x 16384 x 4096 (64 x 128 425, 128 x 128 396, 256 x 256 with spilled
-//   registers 386), 55.0 against 56.2 at 1024 x 8192 x 4096 (256 tiles), 54.4 against 42.6 at 700 x 8192 x 4096 (192).
+// - up to 16 rows and 16384 outputs: few_kernel, 6.4 at 1 x 16384 x 2048 and 20 at 1 x 16384 x 8192 where 64 x 64 takes 7.8 and
+//   26.5; beyond, 24.9 against 18.3 at 1 x 32768 x 4096.
+// - 128 x 256 where there are kFull of them: 340 at 4096 x 16384 x 4096 (64 x 128 425, 128 x 128 396, 256 x 256 with registers
+//   spilled in its loop 386), 55.0 against 56.2 at 1024 x 8192 x 4096 (256 tiles), 54.4 against 42.6 at 700 x 8192 x 4096 (192).
 // - 64 x 32 while each has a unit for itself: 10.0 at 64 x 8192 x 4096 where 64 x 64 takes 12.9; 17.8 against 13.2 at 64 x 12288.
 // - 64 x 64, two places and two workgroups a unit, while all run at once: 18.3 at 64 x 24576 x 4096 where 64 x 128 takes 20.0; then
 //   64 x 128: 33.4 at 64 x 40960 x 4096 where 64 x 64 takes 39.2.
@@ -619,10 +626,11 @@ template <typename T, int XF> const char* launch_linear_t(const ns_mx_linear_arg
     return launch_tile<T, XF, 64, 128, 2, 2, 256, 2, 2>(a, stream);
   } else {
     if (a.m <= 16 && a.n <= 32 * kUnits) return launch_few<T, XF>(a, stream);
-    if (a.m > 128 && tiles(256, 256) >= kFull) return launch_tile<T, XF, 256, 256, 4, 2, 256, 2, 2>(a, stream);
-    if (a.m > 64 && tiles(128, 128) >= kFull) return launch_tile<T, XF, 128, 128, 2, 2, 256, 2, 2>(a, stream);
-    if (tiles(64, 128) >= 2 * kUnits) return launch_tile<T, XF, 64, 128, 2, 2, 256, 2, 2>(a, stream);
-    if (tiles(64, 128) >= kFull) return launch_tile<T, XF, 64, 128, 2, 2, 256, 3, 4>(a, stream);
+    const int64_t some = tiles(64, 128);
+    if (a.m > 128 && tiles(128, 128) > 2 * kUnits) return launch_tile<T, XF, 256, 256, 4, 2, 256, 2, 2>(a, stream);
+    if (a.m > 64 && some > kUnits) return launch_tile<T, XF, 128, 128, 2, 2, 256, 2, 2>(a, stream);
+    if (some >= 2 * kUnits) return launch_tile<T, XF, 64, 128, 2, 2, 256, 2, 2>(a, stream);
+    if (some >= kFull && some <= kUnits) return launch_tile<T, XF, 64, 128, 2, 2, 256, 3, 4>(a, stream);
     return launch_tile<T, XF, 64, 64, 2, 2, 256, 4, 4>(a, stream);
   }
 }

@@ -19,13 +19,13 @@ def kernel_of(fmt, m, n, k):
         return ("tile", 8, 64, 128, 2, 2, 256, 2, 2)
     if m <= 16 and n <= 32 * UNITS:
         return few(4)
-    if m > 128 and tiles(256, 256) >= FULL:
+    if m > 128 and tiles(128, 128) > 2 * UNITS:
         return ("tile", 4, 256, 256, 4, 2, 256, 2, 2)
-    if m > 64 and tiles(128, 128) >= FULL:
+    if m > 64 and tiles(64, 128) > UNITS:
         return ("tile", 4, 128, 128, 2, 2, 256, 2, 2)
     if tiles(64, 128) >= 2 * UNITS:
         return ("tile", 4, 64, 128, 2, 2, 256, 2, 2)
-    if tiles(64, 128) >= FULL:
+    if FULL <= tiles(64, 128) <= UNITS:
         return ("tile", 4, 64, 128, 2, 2, 256, 3, 4)
     return ("tile", 4, 64, 64, 2, 2, 256, 4, 4)
 
@@ -59,7 +59,7 @@ SIZES = [("mxfp8", m, n) for m, n in
           (65, 51250), (300, 17000), (2600, 2400))] + [        # 128 x 256
          ("mxfp4", m, n) for m, n in
          ((1, 33), (16, 97), (5, 8192),                        # few rows
-          (17, 70), (64, 12000), (300, 3000), (16, 8300),      # 64 x 64
+          (17, 70), (64, 12000), (300, 3000), (50, 40000),     # 64 x 64
           (64, 25700), (129, 8600),                            # 64 x 128, three places
           (64, 65600), (33, 65700),                            # 64 x 128, two places
           (140, 12900), (700, 4300),                           # 128 x 128
