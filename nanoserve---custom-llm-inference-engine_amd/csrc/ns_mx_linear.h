@@ -187,7 +187,8 @@ __device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t r, unsigned cha
 // 16-row operands, row 8 a + 4 p + e is row 4 a + e of operand p.
 //
 // LDS rows are a stage's codes of a matrix row, pieces of 16 bytes.  Piece c of x's row r lies at c ^ f(r), so that the lanes of
-// a read spread over the banks: such a read takes 4.0 to 4.8 cycles of the 4 that its 1024 bytes need, 16 in the rows' own order.
+// a read spread over the banks.  By the LDS counters a read takes 4 cycles, which its 1024 bytes need, where the rows have 16
+// pieces, and 8 where they have 8 or 4: two of the lanes that go together meet on a bank (16 cycles in the rows' own order).
 template <int PIECES> __device__ __forceinline__ int x_swizzle(int row) {
   return PIECES == 16 ? row & 15 : PIECES == 8 ? (row & 7) ^ (row >> 3 & 1) : (row >> 1 & 3) ^ (row >> 3 & 1);
 }
@@ -196,7 +197,8 @@ template <int PIECES> __device__ __forceinline__ int x_swizzle(int row) {
 // of 128; x's of KS stages at a time lie in LDS, the weight goes from memory into the operand registers of the one wave
 // that uses it, a stage's registers refilled with the wave's next group as soon as its products are issued.  The waves' sums
 // meet in LDS and are added in their order.  Bound by latency: 1 x 8192 x 2048 has 9 MB to read, 1.7 us at a copy's rate, and
-// takes 4.7 us in 256 workgroups, 2.5 of them a launch's: the first loads, x's way through LDS, the sums' way through LDS.
+// takes 4.4 us in 256 workgroups (8-bit rows; in a graph), 2.5 of them a launch's: the first loads, x's way through LDS, the
+// sums' way through LDS.
 constexpr int kFew = 8;
 
 template <typename T, int XF, int U, int KS>
@@ -333,7 +335,9 @@ template <typename T, int XF> const char* launch_few(const ns_mx_linear_args& a,
 // 61.  The code of its last stages spills registers (96 bytes a lane), its loop none.
 //
 // Pieces of 16 bytes lie in LDS as above: c ^ f(r), x's 16 rows of a read one after the other, the weight's in the order of its
-// operands.
+// operands, whose reads take 4 cycles with 8 pieces a row and 8 with 4.  A read of scale bytes takes 4 cycles of x's rows and 8
+// of the weight's, where 2 would do.  Over the 28 reads of 128 columns of a 64 x 128 part of a tile that makes 120 of 208 LDS cycles
+// conflicts (stages of 128 columns, 8-bit rows).
 template <int PIECES> __device__ __forceinline__ int w_swizzle(int row) {
   return PIECES == 8 ? ((row >> 3 & 3) * 2 + (row >> 1 & 1)) ^ (row & 1) * 4 : (row >> 3 & 3) ^ (row & 2);
 }
@@ -541,9 +545,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(const ns_mx_linea
     }
   };
   const auto run = [&](auto behind) {
+    // in this order, which the waits count on: no load may change places with one of another stage's
     unrolled<C::SL>([&](auto i) { load_scales(i, 0, c0); });
+    __builtin_amdgcn_sched_barrier(0);
     unrolled<P - 1>([&](auto p) {
       unrolled<C::XL + C::WL>([&](auto i) { load(i, decltype(p)::value, place(p)); });
+      __builtin_amdgcn_sched_barrier(0);
     });
     if constexpr (PAIRED) {
       __builtin_amdgcn_s_waitcnt(NS_MX_VMCNT(C::newer(0)));

@@ -80,3 +80,31 @@ def test_every_kernel_that_is_built_is_reached_and_tested(listing):
         at, r = widths(kernel), round_of(kernel)
         assert min(at) <= max(128, r // 4) or kernel[:3] == ("few", kernel[1], 4)
         assert r in at and (max(at) > 2 * r or kernel[0] == "few" and kernel[2] == 2)
+
+
+def test_tiles_first_loads_come_stage_by_stage(listing):
+    """The first wait of a tile with three places or more leaves the loads of all stages but the first in flight: right where
+    each stage's loads, from the same rows one stage further, are issued together."""
+    seen = 0
+    for name, instructions in listing.items():
+        m = re.match(r".*tile_kernelI(?:f|NS_\d\w+?E)Li(\d)ELi(\d+)ELi(\d+)ELi(\d)ELi(\d)ELi(\d+)ELi(\d)ELi(\d)EE", name)
+        if not m or int(m.group(7)) < 3:
+            continue
+        fmt, bm, bn, wm, wn, bk, p, _ = (int(v) for v in m.groups())
+        each = (bm * bk * (1 if fmt == 8 else 0.5) + bn * bk / 2) / 1024 / (wm * wn)     # direct loads of a wave and stage
+        assert each == int(each)
+        each = int(each)
+        loads, wait = [], None
+        for i in instructions:
+            if i.startswith("buffer_load"):
+                assert i.endswith(" lds"), name
+                loads.append(re.match(r"\S+ (v\d+), (s\[\d+:\d+\])", i).groups())
+            elif i.startswith("s_waitcnt") and "vmcnt" in i:
+                wait = int(re.search(r"vmcnt\((\d+)\)", i).group(1))
+            elif i.startswith("s_barrier"):
+                break
+        stages = loads[-(p - 1) * each:]
+        stages = [sorted(stages[s * each:(s + 1) * each]) for s in range(p - 1)]
+        assert wait == (p - 2) * each and all(s == stages[0] for s in stages) and len(set(stages[0])) == each, (name, loads)
+        seen += 1
+    assert seen == 9     # three tiles, three types
