@@ -107,6 +107,8 @@ struct Divide {
 // added in float64: a float32's square neither overflows nor vanishes there.
 // Bound by memory: 8192 x 4096 bfloat16 rows with residual and sum to 8-bit MX rows move 236 MB in 45 us, 5.2 TB/s, a large
 // copy's rate; 4096 rows of 40 float16 heads of 128, 84 MB in 19 us, 17.6 one after another.  One row of 4096 takes 3.2 us.
+// Float32 rows of 32 values a thread keep ten registers in scratch (a workgroup of 1024 threads has 128 for each): 8192 x 8192 to
+// float32 take 111 us, 4.8 TB/s, 8192 x 4096 by 16 values 48, 5.6.
 template <typename T, int CH>
 __global__ __launch_bounds__(1024) void norm_kernel(ns_mx_norm_args a, int group, int width, double one_over_cols, Divide by_heads) {
   __shared__ double s_part[16];
