@@ -120,3 +120,24 @@ def test_nan_codes_and_scales_stay_in_their_row_and_column(device, m, n, k):
     got = MX.mx_linear_hip(x, w, dtype=torch.float32)
     assert torch.equal(got.isnan(), nan)
     assert torch.equal(got[~nan], (xv @ wv.T).float()[~nan])
+
+
+@pytest.mark.parametrize("m,n,k", KERNELS_8)
+def test_halves_at_their_ends_are_whole(device, m, n, k):
+    """The widest octets of either half: 448 or 1.875 times 6 beside the half's least codes (2.25 above, 2^-9 below) times 0.5.
+    Whole multiples of 2^-3 or 2^-10 whose sums stay below 2^24 of them."""
+    gen = torch.Generator().manual_seed(n)
+    for most, least, other in ((0x7e, 0x41, 0x47), (0x3f, 0x01, 0x0f)):
+        xc = torch.where(torch.rand(m, k // 8, 8, generator=gen) < 0.5, least, other)
+        xc[..., 3] = most
+        xc = (xc + 128 * torch.randint(0, 2, xc.shape, generator=gen)).view(m, k).to(torch.uint8)
+        nibbles = torch.full((n, k // 8, 8), 1)
+        nibbles[..., 3] = 7
+        nibbles = (nibbles + 8 * torch.randint(0, 2, nibbles.shape, generator=gen)).view(n, k)
+        one = lambda rows: torch.full((rows, k // 32), 127, dtype=torch.uint8).view(torch.float8_e8m0fnu).to(device)  # noqa: E731
+        x = (xc.view(torch.float8_e4m3fn).to(device), one(m))
+        w = ((nibbles[:, 0::2] | nibbles[:, 1::2] << 4).to(torch.uint8).view(torch.float4_e2m1fn_x2).to(device), one(n))
+        want = x[0].double() @ E2M1[nibbles].to(device).T
+        print(f"ends: m {m} n {n} k {k} most {most}", flush=True)
+        for dtype in (torch.float32, torch.bfloat16):
+            assert torch.equal(MX.mx_linear_hip(x, w, dtype=dtype), want.float().to(dtype)), (most, dtype)
